@@ -48,6 +48,23 @@ _i64 = ctypes.c_int64
 _i32 = ctypes.c_int
 _f32 = ctypes.c_float
 
+# limits and codes of the rotation (VBH_ROPE_*)
+ROPE_MAX_AXES, ROPE_MAX_DIM = 4, 1024
+ROPE_HALF, ROPE_ADJACENT = 0, 1
+ROPE_BLOCKS, ROPE_CYCLE = 0, 1
+
+
+class RopeDesc(ctypes.Structure):
+    """vbh_rope_desc."""
+    _fields_ = ([(n, _i64) for n in ("batch", "seq", "q_heads", "k_heads", "head_dim", "n_freq")] +
+                [(n, _i64 * 3) for n in ("q_stride", "k_stride", "dq_stride", "dk_stride",
+                                         "pos_stride")] +
+                [("sections", _i64 * ROPE_MAX_AXES)] +
+                [(n, _i32) for n in ("axes", "section_order", "pairing", "dtype", "w_dtype",
+                                     "pos_dtype", "f64_freq")] +
+                [("scale", _f32), ("eps", _f32)])
+
+
 # name -> (restype, argtypes); kept in the order of include/vbhip.h
 SIGNATURES = {
     "vbh_abi_version": (_i32, []),
@@ -86,6 +103,11 @@ SIGNATURES = {
     "vbh_reduce_fwd_ws": (_i32, [_vp, _vp, _vp, _i64, _i64, _i64, _i32, _i32, _i32, _vp, _i64,
                                  _vp]),
     "vbh_reduce_workspace_bytes": (_i64, [_i64, _i64, _i64, _i32, _i32]),
+    "vbh_rope_fwd": (_i32, [_vp] * 8),
+    "vbh_rope_bwd": (_i32, [_vp] * 8),
+    "vbh_qk_norm_rope_fwd": (_i32, [_vp] * 10),
+    "vbh_qk_norm_rope_bwd": (_i32, [_vp] * 14 + [_i64, _vp]),
+    "vbh_qk_norm_rope_workspace_bytes": (_i64, [ctypes.POINTER(RopeDesc)]),
     "vbh_stream_copy": (_i32, [_vp, _vp, _i64, _vp]),
     "vbh_stream_read": (_i32, [_vp, _i64, _vp, _i64, _vp]),
     "vbh_stream_read_partial_bytes": (_i64, [_i64]),
@@ -101,7 +123,8 @@ FAST_ENTRY_POINTS = (
     "vbh_softmax_dim_fwd",
     "vbh_logsumexp_fwd", "vbh_logsumexp_fwd_ws", "vbh_cross_entropy_fwd",
     "vbh_cross_entropy_fwd_ws", "vbh_cross_entropy_fwd_noalloc", "vbh_cross_entropy_bwd",
-    "vbh_reduce_fwd", "vbh_reduce_fwd_ws", "vbh_stream_copy", "vbh_stream_read",
+    "vbh_reduce_fwd", "vbh_reduce_fwd_ws", "vbh_rope_fwd", "vbh_rope_bwd",
+    "vbh_qk_norm_rope_fwd", "vbh_qk_norm_rope_bwd", "vbh_stream_copy", "vbh_stream_read",
 )
 
 

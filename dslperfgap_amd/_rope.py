@@ -1,0 +1,248 @@
+"""Host side of the query / key operators (``viperbench/rope``, ``viperbench/qk_norm_rope``):
+the checks of their arguments and the descriptors of their launches, cached by what
+decides them.
+
+Every argument rule is checked where a plan is made, without a GPU; a call with
+tensors the plan knows goes straight to the entry point.
+"""
+from __future__ import annotations
+
+import ctypes
+import math
+
+import torch
+
+from . import _bridge, _lib
+
+POSITION_CODES = {torch.int32: _lib.I32, torch.int64: _lib.I64, torch.float32: _lib.F32}
+ORDERS = {"blocks": _lib.ROPE_BLOCKS, "cycle": _lib.ROPE_CYCLE}
+PAIRINGS = {"half": _lib.ROPE_HALF, "adjacent": _lib.ROPE_ADJACENT}
+
+_PLANS = _bridge.PlanCache()
+
+
+class Plan:
+    """The descriptor of one launch, its address, and the outputs' shapes."""
+    __slots__ = ("desc", "addr", "q_shape", "q_strides", "k_shape", "k_strides", "ws_bytes")
+
+
+def _strides(t):
+    st = t.stride()
+    return st[:3] if len(st) == 4 else (0, *st[:2])
+
+
+def _check_pair(q, k, what, names, like=None):
+    for t, name in zip((q, k), names):
+        if t.dim() not in (3, 4):
+            raise ValueError(f"{what}: {name} must be [tokens, heads, head_dim] or [batch, tokens, "
+                             f"heads, head_dim], got {list(t.shape)}")
+        _bridge.float_code(t, what)
+        if t.dtype != q.dtype:
+            raise TypeError(f"{what}: {names[0]} and {names[1]} dtypes differ")
+    if k.dim() != q.dim() or k.shape[:-2] != q.shape[:-2] or k.shape[-1] != q.shape[-1]:
+        raise ValueError(f"{what}: {names[0]} {list(q.shape)} and {names[1]} {list(k.shape)} must "
+                         "have the same tokens and head_dim")
+    if like is not None:
+        for t, x, name in zip((q, k), like, names):
+            if t.shape != x.shape:
+                raise ValueError(f"{what}: {name} must have shape {list(x.shape)}, got "
+                                 f"{list(t.shape)}")
+            if t.dtype != x.dtype:
+                raise TypeError(f"{what}: {name} must be {x.dtype}, got {t.dtype}")
+
+
+def _position_strides(positions, lead, axes, what):
+    """(axis, batch, token) strides of the positions of [batch, tokens] = `lead`."""
+    if positions.dtype not in POSITION_CODES:
+        raise TypeError(f"{what}: positions must be int32, int64 or float32, got "
+                        f"{positions.dtype}")
+    shape, st = tuple(positions.shape), positions.stride()
+    axis = 0
+    if axes > 1:
+        if not shape or shape[0] != axes:
+            raise ValueError(f"{what}: positions of {axes} axes must have shape [{axes}, ...], "
+                             f"got {list(shape)}")
+        axis, shape, st = st[0], shape[1:], st[1:]
+    if shape == lead:
+        return (axis, 0, st[0]) if len(lead) == 1 else (axis, *st)
+    if shape == lead[1:] and len(lead) == 2:  # one row for the whole batch
+        return (axis, 0, st[0])
+    front = f"{axes}, " if axes > 1 else ""
+    want = " or ".join(f"[{front}{', '.join(map(str, s))}]" for s in {lead, lead[-1:]})
+    raise ValueError(f"{what}: positions must have shape {want}, got {list(positions.shape)}")
+
+
+def make_plan(what, q, k, positions, inv_freq, sections, section_order, pairing, scale, eps,
+              weights, grads):
+    """The Plan of a call, or the error its arguments deserve.  `weights`: None (no
+    norm) or (q_weight, k_weight); `grads`: None or (dq_out, dk_out)."""
+    # the vectors that run through the rotation, under the name the caller knows
+    names = ("dq_out", "dk_out") if what == "rope_bwd" else ("q", "k")
+    _check_pair(q, k, what, names)
+    if grads is not None:
+        _check_pair(*grads, what, ("dq_out", "dk_out"), like=(q, k))
+    lead, dim = tuple(q.shape[:-2]), q.shape[-1]
+    if inv_freq.dim() != 1 or not inv_freq.is_contiguous():
+        raise ValueError(f"{what}: inv_freq must be a contiguous vector")
+    if inv_freq.dtype not in (torch.float32, torch.float64):
+        raise TypeError(f"{what}: inv_freq must be float32 or float64, got {inv_freq.dtype}")
+    n = inv_freq.shape[0]
+    if not 1 <= dim <= _lib.ROPE_MAX_DIM:
+        raise ValueError(f"{what}: head_dim must be 1..{_lib.ROPE_MAX_DIM}, got {dim}")
+    if not 1 <= n <= dim // 2:
+        raise ValueError(f"{what}: inv_freq of {n} does not fit a head_dim of {dim}")
+    if section_order not in ORDERS:
+        raise ValueError(f"{what}: section_order must be one of {sorted(ORDERS)}, got "
+                         f"{section_order!r}")
+    if pairing not in PAIRINGS:
+        raise ValueError(f"{what}: pairing must be one of {sorted(PAIRINGS)}, got {pairing!r}")
+    parts = (n,) if sections is None else tuple(int(s) for s in sections)
+    if not 1 <= len(parts) <= _lib.ROPE_MAX_AXES:
+        raise ValueError(f"{what}: sections must name 1..{_lib.ROPE_MAX_AXES} axes, got "
+                         f"{list(parts)}")
+    if min(parts) < 0 or sum(parts) != n:
+        raise ValueError(f"{what}: sections {list(parts)} must add up to the {n} frequencies")
+    if section_order == "cycle" and any(len(parts) * s > n for s in parts[1:]):
+        raise ValueError(f"{what}: sections {list(parts)} do not fit {n} frequencies in turn")
+    d = _lib.RopeDesc()
+    d.batch, d.seq = lead if len(lead) == 2 else (1, lead[0])
+    d.q_heads, d.k_heads, d.head_dim, d.n_freq = q.shape[-2], k.shape[-2], dim, n
+    d.q_stride[:], d.k_stride[:] = _strides(q), _strides(k)
+    if grads is not None:
+        d.dq_stride[:], d.dk_stride[:] = (_strides(g) for g in grads)
+    d.pos_stride[:] = _position_strides(positions, lead, len(parts), what)
+    d.sections[:len(parts)] = parts
+    d.axes, d.section_order, d.pairing = len(parts), ORDERS[section_order], PAIRINGS[pairing]
+    d.dtype, d.w_dtype = _bridge.FLOAT_CODES[q.dtype], _lib.F32
+    d.pos_dtype, d.f64_freq = POSITION_CODES[positions.dtype], inv_freq.dtype == torch.float64
+    if not math.isfinite(scale):
+        raise ValueError(f"{what}: scale must be finite, got {scale}")
+    if not (math.isfinite(eps) and eps >= 0.0):
+        raise ValueError(f"{what}: eps must be finite and not negative, got {eps}")
+    d.scale, d.eps = scale, eps
+    if weights is not None:
+        for w, name in zip(weights, ("q_weight", "k_weight")):
+            if w is None:
+                continue
+            if tuple(w.shape) != (dim,):
+                raise ValueError(f"{what}: {name} must have shape [{dim}], got {list(w.shape)}")
+            d.w_dtype = _bridge.FLOAT_CODES[w.dtype]
+    p = Plan()
+    p.desc, p.addr = d, ctypes.addressof(d)
+    p.q_shape, p.k_shape = tuple(q.shape), tuple(k.shape)
+    p.q_strides = _bridge.contiguous_strides(p.q_shape)
+    p.k_strides = _bridge.contiguous_strides(p.k_shape)
+    p.ws_bytes = (_lib.lib().vbh_qk_norm_rope_workspace_bytes(ctypes.byref(d))
+                  if grads is not None else 0)
+    return p
+
+
+def _weight(w, dtype, what, name):
+    """A weight the kernels read as it is: contiguous, of the vectors' dtype or fp32."""
+    if w is None:
+        return None
+    if not w.dtype.is_floating_point:
+        raise TypeError(f"{what}: {name} must be a floating tensor, got {w.dtype}")
+    return w.contiguous() if w.dtype is dtype or w.dtype is torch.float32 else w.float()
+
+
+def _weights(q_weight, k_weight, dtype, what):
+    qw, kw = _weight(q_weight, dtype, what, "q_weight"), _weight(k_weight, dtype, what, "k_weight")
+    if qw is not None and kw is not None and qw.dtype is not kw.dtype:
+        return qw.float(), kw.float()
+    return qw, kw
+
+
+def _form(w):
+    return None if w is None else (w.shape, w.dtype)
+
+
+def plan(what, q, k, positions, inv_freq, sections, section_order, pairing, scale, eps=0.0,
+         weights=None, grads=None):
+    """The cached Plan of a call whose vectors and weights the kernels read as they are."""
+    if type(sections) is list:
+        sections = tuple(sections)
+    key = (what, q.shape, q.stride(), q.dtype, k.shape, k.stride(), k.dtype, positions.shape,
+           positions.stride(), positions.dtype, inv_freq.shape, inv_freq.stride(), inv_freq.dtype,
+           sections, section_order, pairing, scale)
+    if weights is not None:
+        key += (eps, _form(weights[0]), _form(weights[1]))
+    if grads is not None:
+        g, h = grads
+        key += (g.shape, g.stride(), g.dtype, h.shape, h.stride(), h.dtype)
+    p = _PLANS.get(key)
+    if p is None:
+        p = _PLANS.put(key, make_plan(what, q, k, positions, inv_freq, sections, section_order,
+                                      pairing, float(scale), float(eps), weights, grads))
+    return p
+
+
+def _device(what, *tensors):
+    """The GPU all tensors lie on."""
+    dev = tensors[0].get_device()
+    for t in tensors:
+        if t is not None and (dev < 0 or t.get_device() != dev):
+            return _bridge.require_gpu(what, *tensors)
+    return dev
+
+
+def _outputs(q, p):
+    return (q.new_empty_strided(p.q_shape, p.q_strides),
+            q.new_empty_strided(p.k_shape, p.k_strides))
+
+
+def _vectors(t):
+    """`t` with vectors that are contiguous."""
+    st = t.stride()
+    return t if not st or st[-1] == 1 else t.contiguous()
+
+
+def rotate(what, q, k, positions, inv_freq, sections, section_order, pairing, scale):
+    """rope_fwd, and rope_bwd with q and k the incoming gradients."""
+    q, k = _vectors(q), _vectors(k)
+    p = plan(what, q, k, positions, inv_freq, sections, section_order, pairing, scale)
+    dev = _device(what, q, k, positions, inv_freq)
+    q_out, k_out = _outputs(q, p)
+    _bridge.launch("vbh_" + what, dev, p.addr, q.data_ptr(), k.data_ptr(), positions.data_ptr(),
+                   inv_freq.data_ptr(), q_out.data_ptr(), k_out.data_ptr())
+    return q_out, k_out
+
+
+def norm_rotate(q, k, q_weight, k_weight, positions, inv_freq, eps, sections, section_order,
+                pairing, scale):
+    what = "qk_norm_rope_fwd"
+    q, k = _vectors(q), _vectors(k)
+    qw, kw = _weights(q_weight, k_weight, q.dtype, what)
+    p = plan(what, q, k, positions, inv_freq, sections, section_order, pairing, scale, eps,
+             (qw, kw))
+    dev = _device(what, q, k, qw, kw, positions, inv_freq)
+    q_out, k_out = _outputs(q, p)
+    _bridge.launch("vbh_qk_norm_rope_fwd", dev, p.addr, q.data_ptr(), k.data_ptr(),
+                   _bridge.ptr(qw), _bridge.ptr(kw), positions.data_ptr(), inv_freq.data_ptr(),
+                   q_out.data_ptr(), k_out.data_ptr())
+    return q_out, k_out
+
+
+def norm_rotate_grads(dq_out, dk_out, q, k, q_weight, k_weight, positions, inv_freq, eps,
+                      sections, section_order, pairing, scale):
+    what = "qk_norm_rope_bwd"
+    q, k = _vectors(q), _vectors(k)
+    dq_out, dk_out = _vectors(dq_out), _vectors(dk_out)
+    qw, kw = _weights(q_weight, k_weight, q.dtype, what)
+    p = plan(what, q, k, positions, inv_freq, sections, section_order, pairing, scale, eps,
+             (qw, kw), (dq_out, dk_out))
+    dev = _device(what, q, k, dq_out, dk_out, qw, kw, positions, inv_freq)
+    dq, dk = _outputs(q, p)
+    dqw = None if qw is None else torch.empty_like(qw)
+    dkw = None if kw is None else torch.empty_like(kw)
+    n = p.ws_bytes if qw is not None or kw is not None else 0
+    ws = _bridge.empty(q, (n,), torch.uint8) if n else None
+    _bridge.launch("vbh_qk_norm_rope_bwd", dev, p.addr, dq_out.data_ptr(), dk_out.data_ptr(),
+                   q.data_ptr(), k.data_ptr(), _bridge.ptr(qw), _bridge.ptr(kw),
+                   positions.data_ptr(), inv_freq.data_ptr(), dq.data_ptr(), dk.data_ptr(),
+                   _bridge.ptr(dqw), _bridge.ptr(dkw), _bridge.ptr(ws), n)
+    if dqw is not None and dqw.dtype is not q_weight.dtype:
+        dqw = dqw.to(q_weight.dtype)
+    if dkw is not None and dkw.dtype is not k_weight.dtype:
+        dkw = dkw.to(k_weight.dtype)
+    return dq, dk, dqw, dkw

@@ -7,6 +7,8 @@
 
 #include <algorithm>
 #include <atomic>
+#include <cmath>
+#include <initializer_list>
 #include <mutex>
 #include <unordered_map>
 #include <vector>
@@ -662,7 +664,7 @@ ColGeometry softmax_col_geometry(int64_t outer, int64_t n, int64_t inner, int es
 // stored before its key, with release / acquire ordering); inserts take the mutex.
 namespace {
 constexpr int kFnDevices = 16;
-constexpr int kFnSlots = 2048;  // a power of two, well above the library's kernel count
+constexpr int kFnSlots = 4096;  // a power of two, well above the library's kernel count
 struct FnSlot {
   std::atomic<const void*> key{nullptr};
   std::atomic<hipFunction_t> fn{nullptr};
@@ -874,6 +876,12 @@ int register_bounds_record(const char* file, BoundsRecordFn fn) {
   return 1;
 }
 #endif
+
+// Limits of the rotation's operands: heads of each side, and the elements from an
+// operand's first to its last (so that byte offsets fit 64 bits with room).
+constexpr int kRopeMaxHeads = 1 << 16;
+constexpr int64_t kRopeMaxExtent = int64_t(1) << 58;
+constexpr int64_t kRopeMaxValues = int64_t(1) << 46;  // of q and k, beyond any memory
 
 }  // namespace vbh
 
@@ -1513,6 +1521,215 @@ int vbh_reduce_fwd(const void* x, void* values, void* indices, int64_t outer, in
                    int64_t inner, int in_dtype, int out_dtype, int op, void* stream) {
   return vbh_reduce_fwd_ws(x, values, indices, outer, n, inner, in_dtype, out_dtype, op, nullptr,
                            0, stream);
+}
+
+// The arguments of the rotation kernels from a descriptor: 0 with *a filled (tokens
+// or heads may be 0), or an error.  `norm`: weights and eps are used; `grads`: so
+// are the strides of the incoming gradients.
+static int rope_args(const vbh_rope_desc* d, const char* what, bool norm, bool grads,
+                     RopeArgs* a) {
+  if (!d) return fail(VBH_E_INVALID, "%s: null descriptor", what);
+  if (!is_float(d->dtype)) return fail(VBH_E_DTYPE, "%s: unsupported dtype %d", what, d->dtype);
+  if (norm && d->w_dtype != d->dtype && d->w_dtype != kF32)
+    return fail(VBH_E_DTYPE, "%s: weight dtype %d must equal dtype %d or be fp32", what,
+                d->w_dtype, d->dtype);
+  if (d->pos_dtype != kI32 && d->pos_dtype != kI64 && d->pos_dtype != kF32)
+    return fail(VBH_E_DTYPE, "%s: positions must be int32, int64 or fp32, got %d", what,
+                d->pos_dtype);
+  if (d->batch < 0 || d->seq < 0 || d->q_heads < 0 || d->k_heads < 0)
+    return fail(VBH_E_INVALID, "%s: negative size", what);
+  if (d->head_dim < 1 || d->head_dim > VBH_ROPE_MAX_DIM)
+    return fail(VBH_E_RANGE, "%s: head_dim %lld outside 1..%d", what,
+                static_cast<long long>(d->head_dim), VBH_ROPE_MAX_DIM);
+  if (d->n_freq < 1 || d->n_freq > d->head_dim / 2)
+    return fail(VBH_E_INVALID, "%s: %lld frequencies for a head_dim of %lld", what,
+                static_cast<long long>(d->n_freq), static_cast<long long>(d->head_dim));
+  if (d->q_heads > kRopeMaxHeads || d->k_heads > kRopeMaxHeads)
+    return fail(VBH_E_RANGE, "%s: more than %d heads", what, kRopeMaxHeads);
+  if (mul_sat(d->batch, d->seq) > kMaxCols)
+    return fail(VBH_E_RANGE, "%s: 2^31 tokens or more", what);
+  if (d->axes < 1 || d->axes > VBH_ROPE_MAX_AXES)
+    return fail(VBH_E_INVALID, "%s: %d position axes, 1..%d are taken", what, d->axes,
+                VBH_ROPE_MAX_AXES);
+  if (d->section_order != VBH_ROPE_BLOCKS && d->section_order != VBH_ROPE_CYCLE)
+    return fail(VBH_E_INVALID, "%s: bad section_order %d", what, d->section_order);
+  if (d->pairing != VBH_ROPE_HALF && d->pairing != VBH_ROPE_ADJACENT)
+    return fail(VBH_E_INVALID, "%s: bad pairing %d", what, d->pairing);
+  int64_t sum = 0;
+  for (int i = 0; i < d->axes; ++i) {
+    const int64_t n = d->sections[i];
+    if (n < 0 || n > d->n_freq)
+      return fail(VBH_E_INVALID, "%s: section %lld of %lld frequencies", what,
+                  static_cast<long long>(n), static_cast<long long>(d->n_freq));
+    if (d->section_order == VBH_ROPE_CYCLE && i > 0 && d->axes * n > d->n_freq)
+      return fail(VBH_E_INVALID,
+                  "%s: a section of %lld in turn needs %lld frequencies, there are %lld", what,
+                  static_cast<long long>(n), static_cast<long long>(d->axes * n),
+                  static_cast<long long>(d->n_freq));
+    sum += n;
+    a->ends[i] = static_cast<int>(d->section_order == VBH_ROPE_CYCLE ? d->axes * n : sum);
+  }
+  if (sum != d->n_freq)
+    return fail(VBH_E_INVALID, "%s: sections hold %lld frequencies, inv_freq %lld", what,
+                static_cast<long long>(sum), static_cast<long long>(d->n_freq));
+  if (!std::isfinite(d->scale)) return fail(VBH_E_INVALID, "%s: scale is not finite", what);
+  if (norm && !(std::isfinite(d->eps) && d->eps >= 0.0f))
+    return fail(VBH_E_INVALID, "%s: eps must be finite and not negative", what);
+
+  a->batch = static_cast<int>(d->batch);
+  a->seq = static_cast<int>(d->seq);
+  a->tokens = d->batch * d->seq;
+  a->dim = static_cast<int>(d->head_dim);
+  a->n_freq = static_cast<int>(d->n_freq);
+  a->slots = (a->dim + 1) / 2;
+  a->axes = d->axes;
+  a->section_order = d->section_order;
+  a->pos_dt = d->pos_dtype;
+  a->f64_freq = d->f64_freq != 0;
+  a->w_f32 = d->w_dtype == kF32;
+  a->scale = a->sin_scale = d->scale;
+  a->eps = d->eps;
+  a->q.heads = static_cast<int>(d->q_heads);
+  a->k.heads = static_cast<int>(d->k_heads);
+  // strides; tokens lie one stride apart where both dims of every operand allow it,
+  // so that no kernel divides by seq
+  bool flat = d->batch == 1 || d->seq == 1;
+  bool ok = true, collapses = true;
+  auto take = [&](const int64_t (&from)[3], int64_t heads, int64_t* to) {
+    for (int i = 0; i < 3; ++i) to[i] = from[i];
+    if (heads == 0 || a->tokens == 0) return;
+    int64_t extent = 0;
+    const int64_t n[3] = {d->batch, d->seq, heads};
+    for (int i = 0; i < 3; ++i) {
+      if (from[i] < 0) ok = false;
+      else extent = std::min(extent + std::min(mul_sat(n[i] - 1, from[i]), kRopeMaxExtent),
+                             kRopeMaxExtent);
+    }
+    if (extent >= kRopeMaxExtent) ok = false;
+    if (from[0] != mul_sat(d->seq, from[1])) collapses = false;
+  };
+  take(d->q_stride, d->q_heads, a->q.xs);
+  take(d->k_stride, d->k_heads, a->k.xs);
+  if (grads) {
+    take(d->dq_stride, d->q_heads, a->q.gs);
+    take(d->dk_stride, d->k_heads, a->k.gs);
+  }
+  const int64_t pos[3] = {d->pos_stride[1], d->pos_stride[2], d->pos_stride[0]};
+  int64_t got[3];
+  take(pos, d->axes, got);
+  if (!ok)
+    return fail(VBH_E_RANGE, "%s: strides must not be negative nor span 2^58 elements", what);
+  a->pos_stride[0] = got[2];
+  a->pos_stride[1] = got[0];
+  a->pos_stride[2] = got[1];
+  a->pos_elems = a->tokens == 0 ? 0
+                                : (d->batch - 1) * got[0] + (d->seq - 1) * got[1] +
+                                      (d->axes - 1) * got[2] + 1;
+  if ((flat || collapses) && a->tokens > 0) {
+    if (d->seq == 1) {  // the batch is the only token dim
+      for (int64_t* st : {a->q.xs, a->k.xs, a->q.gs, a->k.gs}) st[1] = st[0];
+      a->pos_stride[2] = a->pos_stride[1];
+    }
+    a->seq = static_cast<int>(a->tokens);
+    a->batch = 1;
+  }
+  if (mul_sat(a->tokens, (d->q_heads + d->k_heads) * d->head_dim) > kRopeMaxValues)
+    return fail(VBH_E_RANGE, "%s: more than 2^46 values", what);
+  return 0;
+}
+
+// The operands of one side are there unless it has no heads.
+static bool rope_side_ok(int heads, std::initializer_list<const void*> ptrs) {
+  if (heads == 0) return true;
+  for (const void* p : ptrs)
+    if (!p) return false;
+  return true;
+}
+
+static int rope_run(const vbh_rope_desc* d, const char* what, bool norm, bool back, const void* q,
+                    const void* k, const void* qw, const void* kw, const void* positions,
+                    const void* inv_freq, void* q_out, void* k_out, void* stream) {
+  RopeArgs a;
+  if (int rc = rope_args(d, what, norm, false, &a)) return rc;
+  if (a.tokens == 0 || a.q.heads + a.k.heads == 0) return 0;  // empty outputs
+  if (!rope_side_ok(a.q.heads, {q, q_out}) || !rope_side_ok(a.k.heads, {k, k_out}) ||
+      !positions || !inv_freq)
+    return fail(VBH_E_INVALID, "%s: null pointer", what);
+  a.q.x = q;
+  a.k.x = k;
+  a.q.y = q_out;
+  a.k.y = k_out;
+  a.q.w = qw;
+  a.k.w = kw;
+  a.pos = positions;
+  a.freq = inv_freq;
+  if (back) a.sin_scale = -a.scale;
+  return hip_status(launch_rope(a, d->dtype, d->pairing == VBH_ROPE_ADJACENT, norm,
+                                static_cast<hipStream_t>(stream)),
+                    what);
+}
+
+int vbh_rope_fwd(const vbh_rope_desc* desc, const void* q, const void* k, const void* positions,
+                 const void* inv_freq, void* q_out, void* k_out, void* stream) {
+  return rope_run(desc, "rope_fwd", false, false, q, k, nullptr, nullptr, positions, inv_freq,
+                  q_out, k_out, stream);
+}
+
+int vbh_rope_bwd(const vbh_rope_desc* desc, const void* dq_out, const void* dk_out,
+                 const void* positions, const void* inv_freq, void* dq, void* dk, void* stream) {
+  return rope_run(desc, "rope_bwd", false, true, dq_out, dk_out, nullptr, nullptr, positions,
+                  inv_freq, dq, dk, stream);
+}
+
+int vbh_qk_norm_rope_fwd(const vbh_rope_desc* desc, const void* q, const void* k,
+                         const void* q_weight, const void* k_weight, const void* positions,
+                         const void* inv_freq, void* q_out, void* k_out, void* stream) {
+  return rope_run(desc, "qk_norm_rope_fwd", true, false, q, k, q_weight, k_weight, positions,
+                  inv_freq, q_out, k_out, stream);
+}
+
+int64_t vbh_qk_norm_rope_workspace_bytes(const vbh_rope_desc* desc) {
+  RopeArgs a;
+  if (rope_args(desc, "qk_norm_rope_workspace_bytes", true, true, &a) != 0) return 0;
+  return static_cast<int64_t>(sizeof(float)) *
+         rope_bwd_part_floats(a, desc->dtype, desc->pairing == VBH_ROPE_ADJACENT);
+}
+
+int vbh_qk_norm_rope_bwd(const vbh_rope_desc* desc, const void* dq_out, const void* dk_out,
+                         const void* q, const void* k, const void* q_weight,
+                         const void* k_weight, const void* positions, const void* inv_freq,
+                         void* dq, void* dk, void* dq_weight, void* dk_weight, void* workspace,
+                         int64_t workspace_bytes, void* stream) {
+  const char* what = "qk_norm_rope_bwd";
+  RopeArgs a;
+  if (int rc = rope_args(desc, what, true, true, &a)) return rc;
+  if (workspace_bytes < 0) return fail(VBH_E_INVALID, "%s: negative workspace size", what);
+  const bool adjacent = desc->pairing == VBH_ROPE_ADJACENT;
+  const bool empty = a.tokens == 0 || a.q.heads + a.k.heads == 0;
+  if (!empty && (!rope_side_ok(a.q.heads, {q, dq_out, dq}) ||
+                 !rope_side_ok(a.k.heads, {k, dk_out, dk}) || !positions || !inv_freq))
+    return fail(VBH_E_INVALID, "%s: null pointer", what);
+  const int64_t need = static_cast<int64_t>(sizeof(float)) *
+                       rope_bwd_part_floats(a, desc->dtype, adjacent);
+  if ((dq_weight || dk_weight) && need > 0 &&
+      (!workspace || workspace_bytes < need || !aligned16(workspace)))
+    return fail(VBH_E_INVALID, "%s: the weights' gradients need an aligned workspace of %lld bytes",
+                what, static_cast<long long>(need));
+  a.q.x = q;
+  a.k.x = k;
+  a.q.g = dq_out;
+  a.k.g = dk_out;
+  a.q.y = dq;
+  a.k.y = dk;
+  a.q.w = q_weight;
+  a.k.w = k_weight;
+  a.pos = positions;
+  a.freq = inv_freq;
+  a.sin_scale = -a.scale;
+  return hip_status(launch_qk_norm_rope_bwd(a, desc->dtype, adjacent, dq_weight, dk_weight,
+                                            static_cast<float*>(workspace),
+                                            static_cast<hipStream_t>(stream)),
+                    what);
 }
 
 int vbh_stream_copy(const void* src, void* dst, int64_t bytes, void* stream) {

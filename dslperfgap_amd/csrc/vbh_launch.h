@@ -139,6 +139,12 @@ bool dispatch_float_type(int dt, Fn&& fn) {
   }
 }
 
+template <typename Fn>
+void dispatch_bool(bool b, Fn&& fn) {
+  if (b) fn(std::true_type{});
+  else fn(std::false_type{});
+}
+
 // maxit buckets for the register-resident path (1..lane_cap(v))
 template <typename Fn>
 bool dispatch_maxit(int maxit, Fn&& fn) {
@@ -305,6 +311,67 @@ hipError_t launch_cross_entropy_bwd(const CeBwdArgs& a, hipStream_t s);
 
 hipError_t launch_reduce(const void* x, void* vals, int64_t* idx, int64_t outer, int n, int idt,
                          int odt, int op, const Geometry& g, hipStream_t s);
+
+// Rotation of queries and keys, and the norm ahead of it (rope.h, rope.hip,
+// rope_bwd.hip).  Strides are in elements: batch, token, head.
+constexpr int kRopeMaxAxes = 4;
+struct RopeSide {
+  const void* x = nullptr;  // vectors (rope_bwd: the incoming gradients)
+  const void* g = nullptr;  // incoming gradients of the norm's backward
+  void* y = nullptr;        // output, contiguous
+  const void* w = nullptr;  // weight or null
+  int64_t xs[3] = {0, 0, 0}, gs[3] = {0, 0, 0};
+  int heads = 0;
+};
+struct RopeArgs {
+  RopeSide q, k;
+  const void* pos = nullptr;
+  const void* freq = nullptr;
+  int64_t pos_stride[3] = {0, 0, 0};  // axis, batch, token
+  int64_t pos_elems = 0;              // from the first position to the last
+  int64_t tokens = 0;                 // batch * seq, at least 1
+  int batch = 1, seq = 1;
+  int dim = 0, n_freq = 0;
+  int slots = 0;                      // pairs of a vector, passing ones too: ceil(dim / 2)
+  int axes = 1, section_order = 0;
+  int ends[kRopeMaxAxes] = {0, 0, 0, 0};  // axis_of
+  int pos_dt = 0, f64_freq = 0, w_f32 = 0;
+  float scale = 1.0f, sin_scale = 1.0f;   // of cos and of sin (backward: -scale)
+  float eps = 0.0f;
+  int64_t first = 0;                  // token that the launch begins with
+  // set by the launcher: lanes per vector and slots as powers of two, waves that
+  // share a token
+  int group_log2 = 0, slot_log2 = 0, chunks = 1;
+};
+// Longest walk of a lane over a vector whose values no wider piece fits.
+constexpr int kRopeMaxK = 8;
+// Launches of fewer waves, at a token each, give a wave one token.
+constexpr int64_t kRopeFewWaves = 4096;
+// How vectors lie over lanes: v values per piece, k pieces per lane, the
+// powers of two that RopeArgs names.
+struct RopeShape {
+  int v = 1, k = 1;
+  int group_log2 = 0, slot_log2 = 0, chunks = 1;
+};
+RopeShape rope_shape(const RopeArgs& a, int dt, bool adjacent);
+// Chunks of a token that hold queries and that hold keys (one may hold both), and
+// the first of the latter.
+struct RopeRows {
+  int q, k, k_from;
+};
+__host__ __device__ inline RopeRows rope_rows_of(int q_heads, int k_heads, int per_wave) {
+  RopeRows r;
+  r.q = (q_heads + per_wave - 1) / per_wave;
+  r.k_from = q_heads / per_wave;
+  r.k = k_heads > 0 ? (q_heads + k_heads + per_wave - 1) / per_wave - r.k_from : 0;
+  return r;
+}
+hipError_t launch_rope(const RopeArgs& a, int dt, bool adjacent, bool norm, hipStream_t s);
+// The norm's backward.  With a.q.w / a.k.w wanted (dq_weight, dk_weight not null)
+// `parts` holds rope_bwd_part_floats(a, dt, adjacent) floats.
+int64_t rope_bwd_part_floats(const RopeArgs& a, int dt, bool adjacent);
+hipError_t launch_qk_norm_rope_bwd(const RopeArgs& a, int dt, bool adjacent, void* dq_weight,
+                                   void* dk_weight, float* parts, hipStream_t s);
 
 // Reduction over the middle axis.  With c.segs > 1, `parts` holds
 // outer * inner * segs fp32 results, and as many int32 rows for max / argmax.

@@ -130,6 +130,15 @@ ENTRY(vbh_reduce_fwd, "pppqqqiiip",
 ENTRY(vbh_reduce_fwd_ws, "pppqqqiiipqp",
       fn_vbh_reduce_fwd_ws(P(0), P(1), P(2), Q(3), Q(4), Q(5), I(6), I(7), I(8), P(9), Q(10),
                            P(11)))
+ENTRY(vbh_rope_fwd, "pppppppp",
+      fn_vbh_rope_fwd(P(0), P(1), P(2), P(3), P(4), P(5), P(6), P(7)))
+ENTRY(vbh_rope_bwd, "pppppppp",
+      fn_vbh_rope_bwd(P(0), P(1), P(2), P(3), P(4), P(5), P(6), P(7)))
+ENTRY(vbh_qk_norm_rope_fwd, "pppppppppp",
+      fn_vbh_qk_norm_rope_fwd(P(0), P(1), P(2), P(3), P(4), P(5), P(6), P(7), P(8), P(9)))
+ENTRY(vbh_qk_norm_rope_bwd, "ppppppppppppppqp",
+      fn_vbh_qk_norm_rope_bwd(P(0), P(1), P(2), P(3), P(4), P(5), P(6), P(7), P(8), P(9), P(10),
+                              P(11), P(12), P(13), Q(14), P(15)))
 ENTRY(vbh_stream_copy, "ppqp", fn_vbh_stream_copy(P(0), P(1), Q(2), P(3)))
 ENTRY(vbh_stream_read, "pqpqp", fn_vbh_stream_read(P(0), Q(1), P(2), Q(3), P(4)))
 
@@ -148,6 +157,8 @@ static const struct {
     SLOT(vbh_cross_entropy_fwd_noalloc),
     SLOT(vbh_reduce_fwd),
     SLOT(vbh_reduce_fwd_ws),     SLOT(vbh_stream_copy),      SLOT(vbh_stream_read),
+    SLOT(vbh_rope_fwd),          SLOT(vbh_rope_bwd),         SLOT(vbh_qk_norm_rope_fwd),
+    SLOT(vbh_qk_norm_rope_bwd),
 };
 #define N_SLOTS (sizeof(slots) / sizeof(slots[0]))
 
@@ -185,6 +196,8 @@ static PyMethodDef methods[] = {
     METHOD(vbh_cross_entropy_fwd_noalloc),
     METHOD(vbh_cross_entropy_bwd), METHOD(vbh_reduce_fwd),
     METHOD(vbh_reduce_fwd_ws),     METHOD(vbh_stream_copy),       METHOD(vbh_stream_read),
+    METHOD(vbh_rope_fwd),          METHOD(vbh_rope_bwd),          METHOD(vbh_qk_norm_rope_fwd),
+    METHOD(vbh_qk_norm_rope_bwd),
     {NULL, NULL, 0, NULL},
 };
 

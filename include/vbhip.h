@@ -246,6 +246,78 @@ int vbh_reduce_fwd_ws(const void* x, void* values, void* indices, int64_t outer,
 int64_t vbh_reduce_workspace_bytes(int64_t outer, int64_t n, int64_t inner, int in_dtype,
                                    int op);
 
+/* Queries and keys: the rotation by positions and the per-head norm ahead of it.
+ *
+ * The tokens are batch x seq; a token has q_heads query and k_heads key vectors
+ * of head_dim values.  The first 2 * n_freq values of a vector turn in pairs, by
+ * the angle positions[axis of p][token] * inv_freq[p] for pair p, and are scaled
+ * by `scale`; the others pass:
+ *   y_a = scale * (a cos - b sin), y_b = scale * (b cos + a sin).
+ * The angle is formed in 64 bits and reduced before it is rounded to 32.
+ * Strides are in elements and may be zero (inputs) or those of any view whose
+ * vectors are contiguous; outputs are contiguous [batch, seq, heads, head_dim]. */
+#define VBH_ROPE_MAX_AXES 4
+#define VBH_ROPE_MAX_DIM 1024
+
+/* pairing: pair p is values (p, n_freq + p), or (2 p, 2 p + 1) */
+#define VBH_ROPE_HALF 0
+#define VBH_ROPE_ADJACENT 1
+/* section_order: the axes' frequencies in blocks of sections[axis], or in turn
+ * (pair p has axis p % axes while p < axes * sections[that axis], else axis 0;
+ * then axes * sections[axis] <= n_freq for every axis but the first) */
+#define VBH_ROPE_BLOCKS 0
+#define VBH_ROPE_CYCLE 1
+
+typedef struct vbh_rope_desc {
+  int64_t batch, seq;
+  int64_t q_heads, k_heads;
+  int64_t head_dim, n_freq;
+  int64_t q_stride[3], k_stride[3];   /* batch, token, head of q and k (rope_bwd: of
+                                         the incoming gradients)                  */
+  int64_t dq_stride[3], dk_stride[3]; /* the same of dq_out and dk_out
+                                         (qk_norm_rope_bwd only)                  */
+  int64_t pos_stride[3];              /* axis, batch, token of positions         */
+  int64_t sections[VBH_ROPE_MAX_AXES]; /* frequencies of each axis, n_freq in all */
+  int axes;                           /* 1 .. VBH_ROPE_MAX_AXES                  */
+  int section_order, pairing;
+  int dtype;      /* of q, k, their gradients and outputs: F32, F16 or BF16       */
+  int w_dtype;    /* of the weights and their gradients: `dtype` or F32           */
+  int pos_dtype;  /* I32, I64 or F32                                             */
+  int f64_freq;   /* inv_freq holds doubles, else floats                         */
+  float scale;
+  float eps;      /* of the norm                                                 */
+} vbh_rope_desc;
+
+/* The rotation of queries and keys, and its gradient (the rotation back).  The
+ * descriptor is host memory, read during the call.  No reference counterpart (the
+ * reference has no kernel that takes positions). */
+int vbh_rope_fwd(const vbh_rope_desc* desc, const void* q, const void* k, const void* positions,
+                 const void* inv_freq, void* q_out, void* k_out, void* stream);
+int vbh_rope_bwd(const vbh_rope_desc* desc, const void* dq_out, const void* dk_out,
+                 const void* positions, const void* inv_freq, void* dq, void* dk, void* stream);
+
+/* RMSNorm of every query and key vector (as vbh_rms_norm_fwd over head_dim, with
+ * q_weight or k_weight [head_dim]; null: ones), then the rotation, in one pass:
+ * fp32 throughout, rounded once. */
+int vbh_qk_norm_rope_fwd(const vbh_rope_desc* desc, const void* q, const void* k,
+                         const void* q_weight, const void* k_weight, const void* positions,
+                         const void* inv_freq, void* q_out, void* k_out, void* stream);
+
+/* Its gradients: dq, dk [batch, seq, heads, head_dim] of `dtype`, dq_weight and
+ * dk_weight [head_dim] of `w_dtype` (each null: not wanted).  The weights'
+ * gradients are summed in fp32 in a fixed order, through a workspace of
+ * vbh_qk_norm_rope_workspace_bytes(desc) bytes (16-byte aligned scratch of this
+ * call, stream-ordered; not needed where neither is wanted). */
+int vbh_qk_norm_rope_bwd(const vbh_rope_desc* desc, const void* dq_out, const void* dk_out,
+                         const void* q, const void* k, const void* q_weight,
+                         const void* k_weight, const void* positions, const void* inv_freq,
+                         void* dq, void* dk, void* dq_weight, void* dk_weight, void* workspace,
+                         int64_t workspace_bytes, void* stream);
+
+/* Workspace bytes of vbh_qk_norm_rope_bwd with the weights' gradients, a pure
+ * function of the descriptor (0 for an invalid or empty one). */
+int64_t vbh_qk_norm_rope_workspace_bytes(const vbh_rope_desc* desc);
+
 /* Device-to-device stream copy of `bytes` (16-byte aligned pointers and size),
  * the kernel whose sustained rate is the measured HBM peak.
  * Replaces: the vendor-spec PEAKS table of experiments/exp_cliff_roofline.py:192-218
