@@ -1581,7 +1581,6 @@ static int rope_args(const vbh_rope_desc* d, const char* what, bool norm, bool g
   a->tokens = d->batch * d->seq;
   a->dim = static_cast<int>(d->head_dim);
   a->n_freq = static_cast<int>(d->n_freq);
-  a->slots = (a->dim + 1) / 2;
   a->axes = d->axes;
   a->section_order = d->section_order;
   a->pos_dt = d->pos_dtype;
@@ -1655,6 +1654,8 @@ static int rope_run(const vbh_rope_desc* d, const char* what, bool norm, bool ba
   if (!rope_side_ok(a.q.heads, {q, q_out}) || !rope_side_ok(a.k.heads, {k, k_out}) ||
       !positions || !inv_freq)
     return fail(VBH_E_INVALID, "%s: null pointer", what);
+  if (!aligned16(q_out) || !aligned16(k_out))
+    return fail(VBH_E_INVALID, "%s: outputs must be 16-byte aligned", what);
   a.q.x = q;
   a.k.x = k;
   a.q.y = q_out;
@@ -1709,6 +1710,8 @@ int vbh_qk_norm_rope_bwd(const vbh_rope_desc* desc, const void* dq_out, const vo
   if (!empty && (!rope_side_ok(a.q.heads, {q, dq_out, dq}) ||
                  !rope_side_ok(a.k.heads, {k, dk_out, dk}) || !positions || !inv_freq))
     return fail(VBH_E_INVALID, "%s: null pointer", what);
+  if (!aligned16(dq) || !aligned16(dk))
+    return fail(VBH_E_INVALID, "%s: outputs must be 16-byte aligned", what);
   const int64_t need = static_cast<int64_t>(sizeof(float)) *
                        rope_bwd_part_floats(a, desc->dtype, adjacent);
   if ((dq_weight || dk_weight) && need > 0 &&

@@ -1,18 +1,29 @@
-// What the rotation kernels (rope.hip, rope_bwd.hip) share: their arguments, a
-// lane's place among a token's heads, and the angles.
+// What the rotation kernels (rope.hip, rope_bwd.hip) share.
 //
-// A token has H = q_heads + k_heads vectors of D values.  A vector belongs to a
-// group of lanes (a power of two up to 64); a lane holds two pieces of it, A and
-// B, of V values each, chosen so that both members of every pair are its own:
-//   half pairing:      A[i] turns with B[i] (B lies n_freq values behind A)
-//   adjacent pairing:  A[2i] with A[2i+1], B[2i] with B[2i+1] (B lies D / 2 behind
-//                      A, so that the loads run over the vector as in the other)
-// and nothing crosses lanes but the norm's sums.  The values that do not turn are
-// paired the same way among themselves.  A wave holds 64 / G vectors of one
-// token at a time, heads [chunk * 64 / G, ...) for its whole life.
+// A token has q_heads + k_heads vectors of D values.  A wave takes a share of one
+// token's queries or of its keys, so that the angles are made once (one sincos per
+// lane for 64 pairs, through the LDS) for up to 8 passes over vectors.  In a pass
+// the wave holds `per_pass` vectors side by side, each lane V consecutive values:
+// the accesses of a pass run over memory without gaps wherever the heads do.  (Both members of every pair in one lane, as two pieces of half the vector
+// each, costs no exchange, but pieces of less than a 128-byte line cost more: on
+// MI355X 38 us against 27 for 16384 tokens of 40 bf16 heads of 64.)
+//   adjacent pairing: a lane's values pair among themselves
+//   half pairing:     the partners lie in other lanes of the vector's, n_freq / V
+//                     away, whose 16 bytes come over the LDS crossbar as they are
+//                     stored; both lanes then widen both vectors.  Half accesses
+//                     (of V / 2 values) have partners of their own, so that n_freq
+//                     need only be a multiple of V / 2
+// Per value y_i = (x_i C_i + x_partner S_i) r: the cosines and sines, their signs,
+// the scale and the weights meet in C and S once per wave, so that the norm adds
+// one product per value and its sum of squares.
+//
+// Vectors that no lane access of 2 values or more fits (odd sizes, half pairings
+// of an odd number of pairs, more than 64 lanes) go pair by pair: a lane holds
+// both members of a pair (rope_values, qk_norm_rope_value_grads).
 #pragma once
 
 #include <hip/hip_runtime.h>
+#include <limits.h>
 #include <stdint.h>
 
 #include "vbh_device.h"
@@ -22,149 +33,43 @@ namespace vbh {
 
 constexpr int kRopeWaves = 4;  // waves per workgroup
 constexpr int kRopeBlock = kRopeWaves * kWave;
+constexpr int kRopePairs = 8;  // pairs of a lane that goes pair by pair
+constexpr int kRopePasses = 4; // passes of a wave's share, at most
 
-// A lane's vector: head `head` of the token's q_heads + k_heads, place `at` in the
-// group.
-struct RopeLane {
-  int head, at;
-  bool live, is_q;
-};
+// How a launch treats memory (rope_mem): kRopeCached, kRopeOnce: nontemporal loads,
+// kRopeStream: nontemporal loads and stores.
+enum RopeMem : int { kRopeCached = 0, kRopeOnce = 1, kRopeStream = 2 };
 
-__device__ __forceinline__ RopeLane rope_lane(const RopeArgs& a, int chunk) {
-  const int lane = static_cast<int>(threadIdx.x) & (kWave - 1);
-  RopeLane l;
-  l.head = chunk * (kWave >> a.group_log2) + (lane >> a.group_log2);
-  l.at = lane & ((1 << a.group_log2) - 1);
-  l.live = l.head < a.q.heads + a.k.heads;
-  l.is_q = l.head < a.q.heads;
-  return l;
+// What a launch reads and writes, against the 256 MiB cache in front of the memory.
+// MI355X, 16384 tokens of 40 bf16 heads (168 MB in, as much out; three sets of inputs
+// in turn), us by loads / stores, nt: nontemporal:
+//   forward, 168 MB in and out   nt / nt 55.6, nt / plain 51.8, plain / plain 61.1
+//   the same, 336 MB             nt / nt 108.4, nt / plain 116
+//   the same, 84 MB              nt / nt 29.8, nt / plain 29.3, plain / plain 29.0
+//   the same, 42 MB              nt / nt 16.8, nt / plain 16.7, plain / plain 15.1
+//   backward, 336 MB in, 168 out nt / nt 97.0, nt / plain 91.3, plain / plain 105
+//   the same, 168 MB in, 84 out  nt / nt 52.6, nt / plain 50.2, plain / plain 51.2
+//   the same, 84 MB in, 42 out   nt / nt 31.0, nt / plain 31.6, plain / plain 30.6
+constexpr int64_t kRopeCachedBytes = int64_t(128) << 20;  // read
+constexpr int64_t kRopeOnceBytes = int64_t(224) << 20;    // written
+inline RopeMem rope_mem(int64_t read, int64_t written) {
+  if (written > kRopeOnceBytes) return kRopeStream;
+  return read > kRopeCachedBytes ? kRopeOnce : kRopeCached;
+}
+template <typename Fn>
+void dispatch_rope_mem(RopeMem m, Fn&& fn) {
+  if (m == kRopeCached) fn(std::integral_constant<int, kRopeCached>{});
+  else if (m == kRopeOnce) fn(std::integral_constant<int, kRopeOnce>{});
+  else fn(std::integral_constant<int, kRopeStream>{});
 }
 
-// The lane's k-th pieces: places of A and B in the vector, its first pair slot,
-// and which of them there are.
-struct RopePiece {
-  int a, b, slot;
-  bool has_a, has_b;
-};
-
-template <int V, bool ADJ>
-__device__ __forceinline__ RopePiece rope_piece(const RopeArgs& a, const RopeLane& l, int k) {
-  RopePiece p;
-  p.slot = (l.at + k * kWave) * V;
-  if constexpr (ADJ && V == 1) {
-    p.a = 2 * p.slot;
-    p.b = p.a + 1;
-  } else if constexpr (ADJ) {
-    p.a = p.slot;
-    p.b = a.slots + p.slot;
-  } else {
-    const bool turns = p.slot < a.n_freq;
-    p.a = turns ? p.slot : a.n_freq + p.slot;
-    p.b = p.a + (turns ? a.n_freq : a.slots - a.n_freq);
-  }
-  p.has_a = l.live && p.slot < a.slots;
-  p.has_b = p.has_a && (V > 1 || p.b < a.dim);
-  return p;
-}
-
-// Pair of the i-th (A, B) values of a piece (half pairing) or of the i-th pair of
-// its 2 V values (adjacent pairing: V / 2 pairs in A, then V / 2 in B).
-template <int V, bool ADJ>
-__device__ __forceinline__ int rope_pair(const RopeArgs& a, const RopePiece& p, int i) {
-  if constexpr (ADJ && V > 1)
-    return (p.slot >> 1) + (i < V / 2 ? i : (a.slots >> 1) + i - V / 2);
-  else
-    return p.slot + i;
-}
-
-__device__ __forceinline__ Span pick_span(bool first, const Span& a, const Span& b) {
-  return first ? a : b;
-}
-
-// n consecutive (cos, sin) of the table (16-byte aligned where n is even)
-template <int N>
-__device__ __forceinline__ void read_angles(const float2* table, float* c, float* s) {
-  if constexpr (N % 2 == 0) {
-#pragma unroll
-    for (int i = 0; i < N; i += 2) {
-      const float4 v = *reinterpret_cast<const float4*>(table + i);
-      c[i] = v.x;
-      s[i] = v.y;
-      c[i + 1] = v.z;
-      s[i + 1] = v.w;
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      c[i] = table[i].x;
-      s[i] = table[i].y;
-    }
-  }
-}
-
-// The V pairs' (cos, sin) of a piece, in rope_pair's order.
-template <int V, bool ADJ>
-__device__ __forceinline__ void piece_angles(const RopeArgs& a, const RopePiece& p,
-                                             const float2* table, float (&c)[V], float (&s)[V]) {
-  if constexpr (ADJ && V > 1) {
-    read_angles<V / 2>(table + (p.slot >> 1), c, s);
-    read_angles<V / 2>(table + (a.slots >> 1) + (p.slot >> 1), c + V / 2, s + V / 2);
-  } else {
-    read_angles<V>(table + p.slot, c, s);
-  }
-}
-
-// The two values of pair i among a piece's 2 V values (A first).
-template <int V, bool ADJ>
-__device__ __forceinline__ void pair_at(int i, int& first, int& second) {
-  first = ADJ && V > 1 ? 2 * i : i;
-  second = ADJ && V > 1 ? 2 * i + 1 : V + i;
-}
-
-template <typename T, int V>
-__device__ __forceinline__ void load_piece(const T* x, const RopePiece& p,
-                                           typename Raw<T, V>::type& ra,
-                                           typename Raw<T, V>::type& rb, const Span& s) {
-  ra = p.has_a ? load_any<T, V>(x + p.a, s) : typename Raw<T, V>::type{};
-  rb = p.has_b ? load_any<T, V>(x + p.b, s) : typename Raw<T, V>::type{};
-}
-
-// A piece's 2 V weights (ones without a weight), widened.
-template <typename T, int V>
-__device__ __forceinline__ void load_weights(const RopeArgs& a, const RopeLane& l,
-                                             const RopePiece& p, float (&w)[2 * V]) {
-  const void* from = l.is_q ? a.q.w : a.k.w;
-#pragma unroll
-  for (int i = 0; i < 2 * V; ++i) w[i] = 1.0f;
-  if (from == nullptr || !p.has_a) return;
-  auto widen = [&](auto tag) {
-    using W = typename decltype(tag)::type;
-    const W* wp = static_cast<const W*>(from);
-    const Span s = VBH_SPAN(wp, a.dim);
-    const typename Raw<W, V>::type wa = load_any<W, V, false>(wp + p.a, s);
-#pragma unroll
-    for (int i = 0; i < V; ++i) w[i] = raw_at<W, V>(wa, i);
-    if (!p.has_b) return;
-    const typename Raw<W, V>::type wb = load_any<W, V, false>(wp + p.b, s);
-#pragma unroll
-    for (int i = 0; i < V; ++i) w[V + i] = raw_at<W, V>(wb, i);
-  };
-  if (a.w_f32) widen(TypeTag<float>{});
-  else widen(TypeTag<T>{});
-}
+// Floats of a wave's table of angles, a whole number of 16-byte vectors.
+__host__ __device__ constexpr int rope_table_floats(int n_freq) { return (2 * n_freq + 3) & ~3; }
 
 // Values of an operand with strides `st` (for Spans).
 __device__ __forceinline__ int64_t rope_extent(const RopeArgs& a, const int64_t (&st)[3],
                                                int heads) {
   return heads > 0 ? (a.batch - 1) * st[0] + (a.seq - 1) * st[1] + (heads - 1) * st[2] + a.dim : 0;
-}
-
-// Sums of N values over each group of 2^group_log2 lanes, in every lane of it.
-template <int N>
-__device__ __forceinline__ void group_sums(float (&v)[N], int group_log2) {
-  const int width = 1 << group_log2;
-#pragma unroll
-  for (int i = 0; i < N; ++i) v[i] = wave_allreduce<Sum>(v[i], width);
 }
 
 // 1 / sqrt(m) for m >= 0; v_rsq_f32 takes no subnormal operand.
@@ -178,6 +83,22 @@ __device__ __forceinline__ float inverse_root(float m) {
 __device__ __forceinline__ void wave_lds_fence() {
   __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   __builtin_amdgcn_wave_barrier();
+}
+
+__device__ __forceinline__ int wave_lane() {
+  return static_cast<int>(threadIdx.x) & (kWave - 1);
+}
+__device__ __forceinline__ int wave_index() {
+  return __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / kWave);
+}
+
+// The kernel's RopeArgs (its first parameter) where the launch left them: scalar
+// loads from there, a side's by its number.  Read through the parameter itself, both
+// sides' fields are loaded ahead of every choice between them, and over a hundred of
+// the backward's scalars spill.
+__device__ __forceinline__ const RopeArgs& launch_args() {
+  return *reinterpret_cast<const RopeArgs*>(
+      (const void*)__builtin_amdgcn_kernarg_segment_ptr());
 }
 
 // ---------------------------------------------------------------------------
@@ -220,10 +141,9 @@ __device__ __forceinline__ double load_position(const RopeArgs& a, int64_t at, c
   return VBH_IN_SPAN(s, p, 4) ? static_cast<double>(*p) : 0.0;
 }
 
-// Turns per unit of position of pair p (0 where the pair passes).
+// Turns per unit of position of pair p.
 __device__ __forceinline__ double load_turns(const RopeArgs& a, int p, const Span& s) {
   constexpr double kInvTwoPi = 0.15915494309189535;
-  if (p >= a.n_freq) return 0.0;
   if (a.f64_freq) {
     const double* f = static_cast<const double*>(a.freq) + p;
     return VBH_IN_SPAN(s, f, 8) ? *f * kInvTwoPi : 0.0;
@@ -248,42 +168,367 @@ __device__ __forceinline__ int axis_of(const RopeArgs& a, int p) {
   return p < end ? ax : 0;
 }
 
-// The wave's table of (cos, sin) * scale of `slots` pairs for each of U tokens, in
-// its own part of the LDS: every lane makes one pair's at a time, however many
-// heads then read it.  Pairs that pass are (1, 0).
-template <int U>
-__device__ __forceinline__ void make_angles(const RopeArgs& a, int64_t t0, int b0, int s0,
-                                            float2* table) {
-  const int lane = static_cast<int>(threadIdx.x) & (kWave - 1);
-  const Span sf = VBH_SPAN(static_cast<const char*>(a.freq),
-                           static_cast<int64_t>(a.n_freq) * (a.f64_freq ? 8 : 4));
-  const Span sp = VBH_SPAN(static_cast<const char*>(a.pos),
-                           a.pos_elems * (a.pos_dt == kI64 ? 8 : 4));
-  // slot_log2: slots rounded up to a power of two, at most the wave
-  const int per = kWave >> a.slot_log2;  // tokens at a time
-  const int du = lane >> a.slot_log2;
-  for (int p = lane & ((1 << a.slot_log2) - 1); p < a.slots; p += kWave) {
-    const double turns = load_turns(a, p, sf);
-    const int64_t from = axis_of(a, p) * a.pos_stride[0];
-    for (int u = du; u < U; u += per) {
-      int b = b0, s = s0 + u;
-      while (s >= a.seq) {
-        s -= a.seq;
-        ++b;
-      }
-      if (t0 + u >= a.tokens) break;
-      float2 cs = make_float2(1.0f, 0.0f);
-      if (p < a.n_freq) {
-        const double pos =
-            load_position(a, from + b * a.pos_stride[1] + s * a.pos_stride[2], sp);
-        const double f = pos * turns;
-        cs = cos_sin_turns(f - __builtin_rint(f));
-        cs.x *= a.scale;
-        cs.y *= a.sin_scale;
-      }
-      table[u * a.slots + p] = cs;
+// Where token t lies: element offsets from its batch and place in it.
+struct RopeToken {
+  int64_t t;
+  int b, s;
+};
+__device__ __forceinline__ RopeToken rope_token(const RopeArgs& a, int64_t t) {
+  RopeToken r{t, 0, static_cast<int>(t)};
+  if (a.batch > 1) {
+    r.b = static_cast<int>(static_cast<uint32_t>(t) / static_cast<uint32_t>(a.seq));
+    r.s = static_cast<int>(t) - r.b * a.seq;
+  }
+  return r;
+}
+__device__ __forceinline__ int64_t token_offset(const RopeToken& t, const int64_t (&st)[3]) {
+  return t.b * st[0] + t.s * st[1];
+}
+
+// (cos, sin) * scale of pairs lane, lane + 64, ... of a token, one lane each, into
+// the wave's table.  What the first of them needs of memory is loaded by itself, so
+// that a wave that walks over tokens may ask for it ahead of its other loads, which
+// return in order.
+struct RopeAngles {
+  double turns;    // per unit of position, of pair `lane`
+  int64_t axis_at; // its axis's offset among the positions
+  Span sf, sp;
+  __device__ __forceinline__ explicit RopeAngles(const RopeArgs& a) {
+    sf = VBH_SPAN(static_cast<const char*>(a.freq),
+                  static_cast<int64_t>(a.n_freq) * (a.f64_freq ? 8 : 4));
+    sp = VBH_SPAN(static_cast<const char*>(a.pos), a.pos_elems * (a.pos_dt == kI64 ? 8 : 4));
+    const int p = min(wave_lane(), a.n_freq - 1);
+    turns = load_turns(a, p, sf);
+    axis_at = axis_of(a, p) * a.pos_stride[0];
+  }
+  __device__ __forceinline__ double position(const RopeArgs& a, const RopeToken& t) const {
+    return load_position(a, axis_at + t.b * a.pos_stride[1] + t.s * a.pos_stride[2], sp);
+  }
+  __device__ __forceinline__ void put(const RopeArgs& a, float2* table, int p, double f) const {
+    float2 cs = cos_sin_turns(f - __builtin_rint(f));
+    cs.x *= a.scale;
+    cs.y *= a.sin_scale;
+    table[p] = cs;
+  }
+  __device__ __forceinline__ void make(const RopeArgs& a, const RopeToken& t, double pos,
+                                       float2* table) const {
+    if (wave_lane() < a.n_freq) put(a, table, wave_lane(), pos * turns);
+    const int64_t at = t.b * a.pos_stride[1] + t.s * a.pos_stride[2];
+    for (int p = wave_lane() + kWave; p < a.n_freq; p += kWave)
+      put(a, table, p, load_position(a, axis_of(a, p) * a.pos_stride[0] + at, sp) *
+                           load_turns(a, p, sf));
+  }
+};
+
+// ---------------------------------------------------------------------------
+// passes
+// ---------------------------------------------------------------------------
+
+// A lane's place: vector `sub` of the pass, vector access `at` of it.
+struct RopeLane {
+  int sub, at;
+  bool live;
+};
+__device__ __forceinline__ RopeLane rope_lane(const RopeArgs& a) {
+  const int lane = wave_lane();
+  RopeLane l;
+  l.sub = a.tile.lanes_log2 >= 0 ? lane >> a.tile.lanes_log2 : small_quotient(lane, a.tile.lanes);
+  l.at = lane - l.sub * a.tile.lanes;
+  l.live = l.sub < a.tile.per_pass;
+  return l;
+}
+
+// Half pairing: the lanes that hold the partners of this lane's first and second V / 2
+// values, and whether a half's partner is the other half.  Launches without ANY: all
+// values turn and n_freq is a multiple of V, so that the whole access has one partner.
+template <int V>
+struct RopePartner {
+  int lane[2];
+  bool crossed;  // of the launch
+};
+template <int V, bool ANY>
+__device__ __forceinline__ RopePartner<V> rope_partner(const RopeArgs& a, const RopeLane& l) {
+  RopePartner<V> p;
+  if constexpr (!ANY) {
+    const int away = a.n_freq / V;
+    p.lane[0] = p.lane[1] = wave_lane() + (l.at < away ? away : -away);
+    p.crossed = false;
+  } else {
+    const int away = a.n_freq / (V / 2);  // halves
+    p.crossed = (away & 1) != 0;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int mine = 2 * l.at + h;
+      const int theirs = mine < away ? mine + away : mine < 2 * away ? mine - away : mine;
+      p.lane[h] = wave_lane() - l.at + (theirs >> 1);
     }
   }
+  return p;
+}
+
+// The partners' values as they are stored.
+template <typename T, int V, bool ANY>
+__device__ __forceinline__ typename Raw<T, V>::type partners(const typename Raw<T, V>::type& r,
+                                                             const RopePartner<V>& p) {
+  constexpr int N = V * sizeof(T) / 4;
+  if constexpr (N == 1) {
+    return __builtin_bit_cast(
+        typename Raw<T, V>::type,
+        __builtin_amdgcn_ds_bpermute(4 * p.lane[0], __builtin_bit_cast(int, r)));
+  } else {
+    typedef int words __attribute__((ext_vector_type(N)));
+    const words w = __builtin_bit_cast(words, r);
+    words o;
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      o[i] = __builtin_amdgcn_ds_bpermute(4 * p.lane[i / (N / 2)],
+                                          ANY && p.crossed ? w[(i + N / 2) % N] : w[i]);
+    return __builtin_bit_cast(typename Raw<T, V>::type, o);
+  }
+}
+template <int V, bool ANY>
+__device__ __forceinline__ void partners(const float (&w)[V], const RopePartner<V>& p,
+                                         float (&o)[V]) {
+#pragma unroll
+  for (int i = 0; i < V; ++i)
+    o[i] = __int_as_float(__builtin_amdgcn_ds_bpermute(
+        4 * p.lane[i / (V / 2)], __float_as_int(ANY && p.crossed ? w[(i + V / 2) % V] : w[i])));
+}
+
+template <typename W, int V>
+__device__ __forceinline__ void widen_weights(const RopeArgs& a, const RopeSide& side,
+                                              const RopeLane& l, float (&w)[V]) {
+  const W* from = static_cast<const W*>(side.w);
+  const typename Raw<W, V>::type r = load_any<W, V, false>(from + l.at * V, VBH_SPAN(from, a.dim));
+#pragma unroll
+  for (int i = 0; i < V; ++i) w[i] = raw_at<W, V>(r, i);
+}
+// The lane's V weights, widened (ones without weights).
+template <typename T, int V>
+__device__ __forceinline__ void load_weights(const RopeArgs& a, const RopeSide& side,
+                                             const RopeLane& l, float (&w)[V]) {
+#pragma unroll
+  for (int i = 0; i < V; ++i) w[i] = 1.0f;
+  if (side.w == nullptr) return;
+  if (a.w_f32) widen_weights<float, V>(a, side, l, w);
+  else widen_weights<T, V>(a, side, l, w);
+}
+
+// How a lane's V values turn: y_i = x_i c[i] + x_partner s[i], passing[i] where
+// they do not (there are such values only with ANY).
+template <int V>
+struct Turn {
+  float c[V], s[V];
+  bool passing[V];
+};
+
+template <int V, bool ADJ, bool ANY>
+__device__ __forceinline__ void make_turn(const RopeArgs& a, const RopeLane& l,
+                                          const float2* table, Turn<V>& t) {
+  if constexpr (ADJ) {
+#pragma unroll
+    for (int i = 0; i < V; i += 2) {
+      const int p = (l.at * V + i) >> 1;
+      const bool pass = ANY && p >= a.n_freq;
+      const float2 cs = table[ANY ? min(p, a.n_freq - 1) : p];
+      t.passing[i] = t.passing[i + 1] = pass;
+      t.c[i] = t.c[i + 1] = pass ? 1.0f : cs.x;
+      t.s[i] = pass ? 0.0f : -cs.y;
+      t.s[i + 1] = pass ? 0.0f : cs.y;
+    }
+  } else {
+    constexpr int H = ANY ? V / 2 : V;  // values that turn alike
+#pragma unroll
+    for (int h = 0; h < V / H; ++h) {
+      const int at = l.at * V + h * H;
+      const bool pass = ANY && at >= 2 * a.n_freq, first = at < a.n_freq;
+      const float2* from = table + (pass ? 0 : first ? at : at - a.n_freq);
+#pragma unroll
+      for (int i = h * H; i < (h + 1) * H; ++i) {
+        const float2 cs = from[i - h * H];
+        t.passing[i] = pass;
+        t.c[i] = pass ? 1.0f : cs.x;
+        t.s[i] = pass ? 0.0f : first ? -cs.y : cs.y;
+      }
+    }
+  }
+}
+
+// N sums over aligned groups of 2^log2 lanes, step by step for all of them (the
+// steps of wave_allreduce).
+template <int N>
+__device__ __forceinline__ void wave_sums(float (&v)[N], int log2) {
+  if (log2 >= 1) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] += dpp<0xB1>(v[i]);
+  }
+  if (log2 >= 2) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] += dpp<0x4E>(v[i]);
+  }
+  if (log2 >= 3) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] += dpp<0x141>(v[i]);
+  }
+  if (log2 >= 4) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] += dpp<0x140>(v[i]);
+  }
+  if (log2 >= 5) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const auto p = __builtin_amdgcn_permlane16_swap(__float_as_uint(v[i]),
+                                                      __float_as_uint(v[i]), false, false);
+      v[i] = __uint_as_float(p[0]) + __uint_as_float(p[1]);
+    }
+  }
+  if (log2 >= 6) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const auto p = __builtin_amdgcn_permlane32_swap(__float_as_uint(v[i]),
+                                                      __float_as_uint(v[i]), false, false);
+      v[i] = __uint_as_float(p[0]) + __uint_as_float(p[1]);
+    }
+  }
+}
+
+// Sums of N values over the lanes of each vector, in every lane of it.  `scratch`:
+// N * kRopeScratch floats of the wave's own, used where the lanes are no power of
+// two: there each lane leaves its value and adds up its vector's.
+constexpr int kRopeScratch = 128;
+template <int N>
+__device__ __forceinline__ void vector_sums(const RopeArgs& a, const RopeLane& l, float (&v)[N],
+                                            float* scratch) {
+  if (a.tile.lanes_log2 >= 0) {
+    wave_sums<N>(v, a.tile.lanes_log2);
+    return;
+  }
+  const int lanes = a.tile.lanes, line = (lanes + 3) & ~3;  // whole 16-byte reads
+  wave_lds_fence();
+  if (l.live) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) scratch[i * kRopeScratch + l.sub * line + l.at] = v[i];
+  }
+  wave_lds_fence();
+  const float* from = scratch + (l.live ? l.sub : 0) * line;
+#pragma unroll
+  for (int i = 0; i < N; ++i) v[i] = 0.0f;
+  int j = 0;
+  for (; j + 4 <= lanes; j += 4) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const float4 q = *reinterpret_cast<const float4*>(from + i * kRopeScratch + j);
+      v[i] += (q.x + q.y) + (q.z + q.w);
+    }
+  }
+  const int rest = lanes - j;
+  if (rest > 0) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const float4 q = *reinterpret_cast<const float4*>(from + i * kRopeScratch + j);
+      v[i] += q.x + (rest > 1 ? q.y : 0.0f) + (rest > 2 ? q.z : 0.0f);
+    }
+  }
+}
+
+// One token's output vectors of one side, [heads, D] at `base`: stores through a
+// buffer resource whose range check drops what lies behind them, so that lanes
+// without a vector need no branch around the store (which would keep the compiler
+// from overlapping the passes).  `base` is 16-byte aligned where V values are.
+template <typename T, int V, int MEM>
+struct RopeOut {
+  __amdgpu_buffer_rsrc_t rsrc;
+  T* base;
+  Span span;
+  __device__ __forceinline__ RopeOut(const RopeArgs& a, const RopeSide& side, int64_t token) {
+    const int values = side.heads * a.dim;
+    base = static_cast<T*>(side.y) + token * values;
+    span = VBH_SPAN(static_cast<T*>(side.y), a.tokens * values);
+    rsrc = __builtin_amdgcn_make_buffer_rsrc(
+        base, static_cast<short>(0),
+        __builtin_amdgcn_readfirstlane(values * static_cast<int>(sizeof(T))), kRawBufferWord3);
+  }
+  // Values `at` on, rounded to T; not `there`: dropped.
+  __device__ __forceinline__ void store(int at, bool there, const float* o) const {
+    if (!VBH_IN_SPAN(span, there ? base + at : base, V * sizeof(T))) return;
+    typename Raw<T, V>::type r;
+#pragma unroll
+    for (int i = 0; i < V; ++i) r[i] = static_cast<T>(o[i]);
+    const int off = there ? at * static_cast<int>(sizeof(T)) : INT_MAX;
+    constexpr int N = V * sizeof(T) / 4;
+    constexpr int kAux = MEM == kRopeStream ? 2 : 0;  // nt
+    typedef int words __attribute__((ext_vector_type(N)));
+    if constexpr (N == 4)
+      __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(words, r), rsrc, off, 0, kAux);
+    else if constexpr (N == 2)
+      __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(words, r), rsrc, off, 0, kAux);
+    else
+      __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(int, r), rsrc, off, 0, kAux);
+  }
+};
+
+// Sum over a lane's values of x^2; 16-bit pairs on the dot-product unit.
+template <typename T, int V>
+__device__ __forceinline__ float squares(const typename Raw<T, V>::type& r) {
+  float sum = 0.0f;
+  if constexpr (sizeof(T) == 2) {
+#pragma unroll
+    for (int i = 0; i < V; i += 2) {
+      typename Pair<T>::type p;
+      p[0] = r[i];
+      p[1] = r[i + 1];
+      sum = Pair<T>::dot(p, p, sum);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i) sum = fmaf(r[i], r[i], sum);
+  }
+  return sum;
+}
+
+// ---------------------------------------------------------------------------
+// pair by pair
+// ---------------------------------------------------------------------------
+
+// A lane's k-th pair of a vector: its values' places, whether there are both, its
+// number among the turning pairs or -1 where they pass.
+struct RopePair {
+  int a, b, p;
+  bool has_a, has_b;
+};
+template <bool ADJ>
+__device__ __forceinline__ RopePair rope_pair(const RopeArgs& a, const RopeLane& l, int k) {
+  const int slots = (a.dim + 1) / 2, slot = l.at + k * kWave;
+  const bool turns = slot < a.n_freq;
+  RopePair r;
+  r.p = turns ? slot : -1;
+  if constexpr (ADJ) {
+    r.a = 2 * slot;
+    r.b = r.a + 1;
+  } else {
+    r.a = turns ? slot : a.n_freq + slot;
+    r.b = r.a + (turns ? a.n_freq : slots - a.n_freq);
+  }
+  r.has_a = l.live && slot < slots;
+  r.has_b = r.has_a && r.b < a.dim;
+  return r;
+}
+
+// One weight, widened (1 without weights).
+template <typename T>
+__device__ __forceinline__ float load_weight(const RopeArgs& a, const RopeSide& side, int i) {
+  if (side.w == nullptr) return 1.0f;
+  if (a.w_f32) {
+    const float* w = static_cast<const float*>(side.w);
+    return load_any<float, 1, false>(w + i, VBH_SPAN(w, a.dim));
+  }
+  const T* w = static_cast<const T*>(side.w);
+  return static_cast<float>(load_any<T, 1, false>(w + i, VBH_SPAN(w, a.dim)));
+}
+
+template <typename T>
+__device__ __forceinline__ float load_value(const T* x, bool there, const Span& s) {
+  return there ? raw_at<T, 1>(load_any<T, 1>(x, s), 0) : 0.0f;
 }
 
 }  // namespace vbh

@@ -4,11 +4,11 @@
 //   dn = R^T dy (the rotation back, by the same scale),  du = dn w
 //   dx = r (du - u mean(du u)),  dw = sum over tokens and heads of dn u
 //
-// One pass over x and dy: the vector's two sums cross its lanes once, together,
-// and the weights' sums stay in the lane.  A wave keeps its heads for the whole
-// kernel and walks over tokens, so that a lane's 2 V sums belong to one weight;
-// at the end a workgroup adds up its waves' and writes one row of sums per
-// weight, and a second kernel adds the rows, all in a fixed order.
+// One pass over x and dy, the vectors over lanes as in the forward; only dy has
+// partners.  The weights' sums stay in the lane: a wave walks over tokens and
+// keeps V sums for the queries' weight and V for the keys'.  At the end a workgroup
+// adds up its waves' and writes one row of sums per weight, and a second kernel
+// adds the rows, all in a fixed order.
 #include <algorithm>
 
 #include "rope.h"
@@ -17,249 +17,362 @@ namespace vbh {
 
 namespace {
 
-template <typename T, int V, int K, int U, bool ADJ, bool PART>
-__global__ __launch_bounds__(kRopeBlock) void qk_norm_rope_grads(const RopeArgs a, float* parts) {
-  extern __shared__ float2 rope_tables[];
-  const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / kWave);
-  const int chunk = static_cast<int>(blockIdx.x % static_cast<uint32_t>(a.chunks));
-  const int walker = static_cast<int>(blockIdx.x / static_cast<uint32_t>(a.chunks));
-  const int walkers = static_cast<int>(gridDim.x / static_cast<uint32_t>(a.chunks));
-  const RopeLane l = rope_lane(a, chunk);
-  float2* table = rope_tables + wave * U * a.slots;
+#ifndef ZGU
+#define ZGU 2
+#endif
+#ifndef ZGW
+#define ZGW 4
+#endif
+constexpr int kGradPasses = ZGU;  // passes of a wave's share, at most
 
-  const int hh = l.is_q ? l.head : l.head - a.q.heads;
-  const T* x = static_cast<const T*>(l.is_q ? a.q.x : a.k.x) +
-               hh * (l.is_q ? a.q.xs[2] : a.k.xs[2]);
-  const T* g = static_cast<const T*>(l.is_q ? a.q.g : a.k.g) +
-               hh * (l.is_q ? a.q.gs[2] : a.k.gs[2]);
-  T* y = static_cast<T*>(l.is_q ? a.q.y : a.k.y) + static_cast<int64_t>(hh) * a.dim;
-  const Span sx = pick_span(
-      l.is_q, VBH_SPAN(static_cast<const T*>(a.q.x), rope_extent(a, a.q.xs, a.q.heads)),
-      VBH_SPAN(static_cast<const T*>(a.k.x), rope_extent(a, a.k.xs, a.k.heads)));
-  const Span sg = pick_span(
-      l.is_q, VBH_SPAN(static_cast<const T*>(a.q.g), rope_extent(a, a.q.gs, a.q.heads)),
-      VBH_SPAN(static_cast<const T*>(a.k.g), rope_extent(a, a.k.gs, a.k.heads)));
-  const Span sy =
-      pick_span(l.is_q, VBH_SPAN(static_cast<T*>(a.q.y), a.tokens * a.q.heads * a.dim),
-                VBH_SPAN(static_cast<T*>(a.k.y), a.tokens * a.k.heads * a.dim));
+// Workgroups that have queries' waves and that have keys' (one may have both), and
+// the first of the latter.
+struct RopeRows {
+  int q, k, k_from;
+};
+__host__ __device__ inline RopeRows rope_rows_of(const RopeArgs& a) {
+  const int q = a.q.chunks * a.q.walkers, k = a.k.chunks * a.k.walkers;
+  RopeRows r;
+  r.q = (q + kRopeWaves - 1) / kRopeWaves;
+  r.k_from = q / kRopeWaves;
+  r.k = k > 0 ? (q + k + kRopeWaves - 1) / kRopeWaves - r.k_from : 0;
+  return r;
+}
 
-  RopePiece p[K];
-  float w[K][2 * V], dw[K][2 * V];
-#pragma unroll
-  for (int k = 0; k < K; ++k) {
-    p[k] = rope_piece<V, ADJ>(a, l, k);
-    load_weights<T, V>(a, l, p[k], w[k]);
-#pragma unroll
-    for (int i = 0; i < 2 * V; ++i) dw[k][i] = 0.0f;
+// A wave's part of the launch: share `chunk` of one side's passes, of every
+// walkers-th token from `token` on.  Queries' waves come first; none behind them all.
+struct RopeWalk {
+  bool is_q, live;
+  int chunk, token;
+};
+__device__ __forceinline__ RopeWalk rope_walk(const RopeArgs& a, int wave) {
+  const int w = static_cast<int>(blockIdx.x) * kRopeWaves + wave;
+  const int q = a.q.chunks * a.q.walkers, k = a.k.chunks * a.k.walkers;
+  const bool is_q = w < q;
+  const uint32_t i = static_cast<uint32_t>(is_q ? w : w - q);
+  const uint32_t chunks = static_cast<uint32_t>(max(is_q ? a.q.chunks : a.k.chunks, 1));
+  const uint32_t token = i / chunks;
+  return RopeWalk{is_q, w < q + k, static_cast<int>(i - token * chunks),
+                  static_cast<int>(token)};
+}
+
+// The workgroup's row of sums for each weight that its waves have worked on: `sums`
+// holds `each` vectors of every wave's.  parts: q's rows, then k's.
+__device__ __forceinline__ void write_part(const RopeArgs& a, const float* sums, int each,
+                                           float* parts) {
+  const RopeRows rows = rope_rows_of(a);
+  const Span sp = VBH_SPAN(parts, static_cast<int64_t>(rows.q + rows.k) * a.dim);
+  const int block = static_cast<int>(blockIdx.x);
+  const int cut = min(max(a.q.chunks * a.q.walkers - block * kRopeWaves, 0), kRopeWaves);
+  for (int d = static_cast<int>(threadIdx.x); d < a.dim; d += kRopeBlock) {
+    float q = 0.0f, k = 0.0f;
+    for (int v = 0; v < cut * each; ++v) q += sums[v * a.dim + d];
+    for (int v = cut * each; v < kRopeWaves * each; ++v) k += sums[v * a.dim + d];
+    if (block < rows.q)
+      store_any<float, 1, false>(parts + static_cast<int64_t>(block) * a.dim + d, &q, sp);
+    if (block >= rows.k_from && block - rows.k_from < rows.k)
+      store_any<float, 1, false>(
+          parts + static_cast<int64_t>(rows.q + block - rows.k_from) * a.dim + d, &k, sp);
   }
+}
+
+// The wave's share of its tokens, U passes each; dw: the lane's sums.
+template <typename T, int V, int U, bool ADJ, bool ANY, int MEM>
+__device__ __forceinline__ void grad_share(const RopeArgs& a, const RopeSide& side,
+                                           const RopeLane& l, int chunk, int first,
+                                           float2* table, float* scratch, float (&dw)[V]) {
+  const Span sx = VBH_SPAN(static_cast<const T*>(side.x), rope_extent(a, side.xs, side.heads));
+  const Span sg = VBH_SPAN(static_cast<const T*>(side.g), rope_extent(a, side.gs, side.heads));
+  const RopePartner<V> partner = rope_partner<V, ANY>(a, l);
   const float inv_dim = 1.0f / static_cast<float>(a.dim);
+  const int head0 = chunk * U * a.tile.per_pass;
+  float w[V];
+  load_weights<T, V>(a, side, l, w);
+  const T* x0 = static_cast<const T*>(side.x);
+  const T* g0 = static_cast<const T*>(side.g);
+  const int64_t lane_x = (head0 + l.sub) * side.xs[2] + l.at * V;
+  const int64_t lane_g = (head0 + l.sub) * side.gs[2] + l.at * V;
+  const int64_t x_step = a.tile.per_pass * side.xs[2], g_step = a.tile.per_pass * side.gs[2];
+  const int to = (head0 + l.sub) * a.dim + l.at * V, y_step = a.tile.per_pass * a.dim;
+  bool ok[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u)
+    ok[u] = l.live && head0 + u * a.tile.per_pass + l.sub < side.heads;
 
-  const int64_t step = static_cast<int64_t>(walkers) * kRopeWaves * U;
-  for (int64_t t0 = (static_cast<int64_t>(walker) * kRopeWaves + wave) * U; t0 < a.tokens;
-       t0 += step) {
-    const int b0 = a.batch > 1 ? static_cast<int>(static_cast<uint32_t>(t0) /
-                                                  static_cast<uint32_t>(a.seq)) : 0;
-    const int s0 = static_cast<int>(t0 - static_cast<int64_t>(b0) * a.seq);
-    typename Raw<T, V>::type xa[U][K], xb[U][K], ga[U][K], gb[U][K];
-    int b = b0, s = s0;
+  typedef typename Raw<T, V>::type R;
+  auto load = [&](const RopeToken& t, R(&g)[U], R(&x)[U]) {
+    const T* from_x = x0 + token_offset(t, side.xs) + lane_x;
+    const T* from_g = g0 + token_offset(t, side.gs) + lane_g;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const bool there = t0 + u < a.tokens;
-      const int64_t xq = b * a.q.xs[0] + s * a.q.xs[1], xk = b * a.k.xs[0] + s * a.k.xs[1];
-      const int64_t gq = b * a.q.gs[0] + s * a.q.gs[1], gk = b * a.k.gs[0] + s * a.k.gs[1];
-      const T* xt = x + (l.is_q ? xq : xk);
-      const T* gt = g + (l.is_q ? gq : gk);
-#pragma unroll
-      for (int k = 0; k < K; ++k) {
-        const typename Raw<T, V>::type zero{};
-        xa[u][k] = there && p[k].has_a ? load_any<T, V>(xt + p[k].a, sx) : zero;
-        xb[u][k] = there && p[k].has_b ? load_any<T, V>(xt + p[k].b, sx) : zero;
-        ga[u][k] = there && p[k].has_a ? load_any<T, V>(gt + p[k].a, sg) : zero;
-        gb[u][k] = there && p[k].has_b ? load_any<T, V>(gt + p[k].b, sg) : zero;
-      }
-      if (++s == a.seq) {
-        s = 0;
-        ++b;
-      }
+      // lanes without a vector read their values of the first: no branch keeps the
+      // loads apart
+      g[u] = load_any<T, V, MEM != kRopeCached>(ok[u] ? from_g + u * g_step : g0 + l.at * V, sg);
+      x[u] = load_any<T, V, MEM != kRopeCached>(ok[u] ? from_x + u * x_step : x0 + l.at * V, sx);
     }
+  };
+  const RopeAngles angles(a);
+  for (int64_t token = first; token < a.tokens; token += side.walkers) {
+    const RopeToken t = rope_token(a, token);
+    const double pos = angles.position(a, t);
+    R x[U], g[U];
+    load(t, g, x);
     wave_lds_fence();
-    make_angles<U>(a, t0, b0, s0, table);
+    angles.make(a, t, pos, table);
     wave_lds_fence();
-
+    Turn<V> turn;
+    make_turn<V, ADJ, ANY>(a, l, table, turn);
+    const RopeOut<T, V, MEM> out(a, side, t.t);
+    auto finish = [&](int u, const float (&dn)[V], float s0, float s1) {
+      // lanes without a vector add nothing to the sums
+      const float r = ok[u] ? inverse_root(fmaf(s0, inv_dim, a.eps)) : 0.0f;
+      const float mean = s1 * r * inv_dim * r;
+      float o[V];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      if (t0 + u >= a.tokens) break;
-      float dn[K][2 * V];
-      float sums[2] = {0.0f, 0.0f};
-#pragma unroll
-      for (int k = 0; k < K; ++k) {
-        float c[V], si[V];
-        if (p[k].has_a) {
-          piece_angles<V, ADJ>(a, p[k], table + u * a.slots, c, si);
-        } else {
-#pragma unroll
-          for (int i = 0; i < V; ++i) c[i] = si[i] = 0.0f;
-        }
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-          int i0, i1;
-          pair_at<V, ADJ>(i, i0, i1);
-          const float g0 = i0 < V ? raw_at<T, V>(ga[u][k], i0) : raw_at<T, V>(gb[u][k], i0 - V);
-          const float g1 = i1 < V ? raw_at<T, V>(ga[u][k], i1) : raw_at<T, V>(gb[u][k], i1 - V);
-          const float x0 = i0 < V ? raw_at<T, V>(xa[u][k], i0) : raw_at<T, V>(xb[u][k], i0 - V);
-          const float x1 = i1 < V ? raw_at<T, V>(xa[u][k], i1) : raw_at<T, V>(xb[u][k], i1 - V);
-          // sin_scale is that of the rotation back
-          float n0 = fmaf(g0, c[i], -g1 * si[i]), n1 = fmaf(g1, c[i], g0 * si[i]);
-          if (PART && rope_pair<V, ADJ>(a, p[k], i) >= a.n_freq) {
-            n0 = g0;
-            n1 = g1;
-          }
-          dn[k][i0] = n0;
-          dn[k][i1] = n1;
-          sums[0] = fmaf(x0, x0, fmaf(x1, x1, sums[0]));
-          sums[1] = fmaf(n0 * w[k][i0], x0, fmaf(n1 * w[k][i1], x1, sums[1]));
-        }
+      for (int i = 0; i < V; ++i) {
+        const float unit = raw_at<T, V>(x[u], i) * r;
+        dw[i] = fmaf(dn[i], unit, dw[i]);
+        o[i] = fmaf(dn[i] * r, w[i], -unit * mean);
       }
-      group_sums<2>(sums, a.group_log2);
-      const float r = inverse_root(fmaf(sums[0], inv_dim, a.eps));
-      const float mean = sums[1] * r * inv_dim;
-      const int64_t row = (t0 + u) * (l.is_q ? a.q.heads : a.k.heads) * a.dim;
+      out.store(to + u * y_step, ok[u], o);
+    };
+    auto begin = [&](int u, float (&dn)[V], float& s0, float& s1) {
+      R other = g[u];
+      if constexpr (!ADJ) other = partners<T, V, ANY>(g[u], partner);
+      s0 = squares<T, V>(x[u]);
+      s1 = 0.0f;
 #pragma unroll
-      for (int k = 0; k < K; ++k) {
-        float o[2 * V];
+      for (int i = 0; i < V; ++i) {
+        const float gi = raw_at<T, V>(g[u], i);
+        const float gp = raw_at<T, V>(other, ADJ ? i ^ 1 : i);
+        float n = fmaf(gi, turn.c[i], gp * turn.s[i]);
+        if (ANY && turn.passing[i]) n = gi;
+        dn[i] = n;
+        s1 = fmaf(n * w[i], raw_at<T, V>(x[u], i), s1);
+      }
+    };
+    float dn[U][V], sums[2 * U];
 #pragma unroll
-        for (int i = 0; i < 2 * V; ++i) {
-          const float v = i < V ? raw_at<T, V>(xa[u][k], i) : raw_at<T, V>(xb[u][k], i - V);
-          const float unit = v * r;
-          dw[k][i] = fmaf(dn[k][i], unit, dw[k][i]);
-          o[i] = r * fmaf(dn[k][i], w[k][i], -unit * mean);
-        }
-        if (p[k].has_a) store_any<T, V>(y + row + p[k].a, o, sy);
-        if (p[k].has_b) store_any<T, V>(y + row + p[k].b, o + V, sy);
+    for (int u = 0; u < U; ++u) begin(u, dn[u], sums[2 * u], sums[2 * u + 1]);
+    vector_sums<2 * U>(a, l, sums, scratch);
+#pragma unroll
+    for (int u = 0; u < U; ++u) finish(u, dn[u], sums[2 * u], sums[2 * u + 1]);
+  }
+}
+
+template <typename T, int V, bool ADJ, bool ANY, int MEM>
+__global__ __launch_bounds__(kRopeBlock, ZGW) void qk_norm_rope_grads(const RopeArgs,
+                                                                    float* parts) {
+  const RopeArgs& a = launch_args();
+  extern __shared__ __align__(16) float rope_lds[];
+  const int wave = wave_index();
+  const RopeWalk walk = rope_walk(a, wave);
+  const RopeLane l = rope_lane(a);
+  const RopeSide& side = a.side(!walk.is_q);
+  const int table_floats = rope_table_floats(a.n_freq);
+  const int scratch_floats = a.tile.lanes_log2 < 0 ? 2 * kGradPasses * kRopeScratch : 0;
+  float* mine = rope_lds + wave * (table_floats + scratch_floats);
+  float2* table = reinterpret_cast<float2*>(mine);
+  float* scratch = mine + table_floats;
+  float dw[V];
+#pragma unroll
+  for (int i = 0; i < V; ++i) dw[i] = 0.0f;
+  if (walk.live) {
+    if (side.per_wave == 1)
+      grad_share<T, V, 1, ADJ, ANY, MEM>(a, side, l, walk.chunk, walk.token, table, scratch, dw);
+    else
+      grad_share<T, V, kGradPasses, ADJ, ANY, MEM>(a, side, l, walk.chunk, walk.token, table,
+                                                    scratch, dw);
+  }
+  if (parts == nullptr) return;
+  __syncthreads();
+  if (l.live) {
+    float* to = rope_lds + (wave * a.tile.per_pass + l.sub) * a.dim + l.at * V;
+#pragma unroll
+    for (int i = 0; i < V; ++i) to[i] = dw[i];
+  }
+  __syncthreads();
+  write_part(a, rope_lds, a.tile.per_pass, parts);
+}
+
+// Pair by pair (rope.h).
+template <typename T, int K, bool ADJ>
+__global__ __launch_bounds__(kRopeBlock) void qk_norm_rope_value_grads(const RopeArgs a,
+                                                                       float* parts) {
+  extern __shared__ __align__(16) float rope_lds[];
+  const int wave = wave_index();
+  float2* table = reinterpret_cast<float2*>(rope_lds) + wave * a.n_freq;
+  const RopeLane l = rope_lane(a);
+  const float inv_dim = 1.0f / static_cast<float>(a.dim);
+  float dw[2 * K];
+#pragma unroll
+  for (int k = 0; k < 2 * K; ++k) dw[k] = 0.0f;
+  const RopeWalk walk = rope_walk(a, wave);
+  const RopeSide& side = a.side(!walk.is_q);
+  const int head = walk.chunk * a.tile.per_pass + l.sub;
+
+  const RopeAngles angles(a);
+  for (int64_t token = walk.live ? walk.token : a.tokens; token < a.tokens;
+       token += side.walkers) {
+    const RopeToken t = rope_token(a, token);
+    const bool ok = l.live && head < side.heads;
+    const Span sx = VBH_SPAN(static_cast<const T*>(side.x), rope_extent(a, side.xs, side.heads));
+    const Span sg = VBH_SPAN(static_cast<const T*>(side.g), rope_extent(a, side.gs, side.heads));
+    const Span sy = VBH_SPAN(static_cast<T*>(side.y), a.tokens * side.heads * a.dim);
+    const T* x = static_cast<const T*>(side.x) + token_offset(t, side.xs) + head * side.xs[2];
+    const T* g = static_cast<const T*>(side.g) + token_offset(t, side.gs) + head * side.gs[2];
+    T* y = static_cast<T*>(side.y) + (t.t * side.heads + head) * a.dim;
+    wave_lds_fence();
+    angles.make(a, t, angles.position(a, t), table);
+    wave_lds_fence();
+    float xa[K], xb[K], na[K], nb[K], sums[2] = {0.0f, 0.0f};
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const RopePair r = rope_pair<ADJ>(a, l, k);
+      const bool has_a = ok && r.has_a, has_b = ok && r.has_b;
+      xa[k] = load_value<T>(x + r.a, has_a, sx);
+      xb[k] = load_value<T>(x + r.b, has_b, sx);
+      na[k] = load_value<T>(g + r.a, has_a, sg);
+      nb[k] = load_value<T>(g + r.b, has_b, sg);
+      if (has_a && r.p >= 0) {
+        const float2 cs = table[r.p];
+        const float ga = na[k], gb = nb[k];
+        na[k] = fmaf(ga, cs.x, -gb * cs.y);
+        nb[k] = fmaf(gb, cs.x, ga * cs.y);
+      }
+      sums[0] = fmaf(xa[k], xa[k], fmaf(xb[k], xb[k], sums[0]));
+      if (has_a) sums[1] = fmaf(na[k] * load_weight<T>(a, side, r.a), xa[k], sums[1]);
+      if (has_b) sums[1] = fmaf(nb[k] * load_weight<T>(a, side, r.b), xb[k], sums[1]);
+    }
+    vector_sums<2>(a, l, sums, nullptr);
+    const float size = inverse_root(fmaf(sums[0], inv_dim, a.eps));
+    const float mean = sums[1] * size * inv_dim;
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const RopePair r = rope_pair<ADJ>(a, l, k);
+      const float ua = xa[k] * size, ub = xb[k] * size;
+      if (ok && r.has_a) {
+        const float o = size * fmaf(na[k], load_weight<T>(a, side, r.a), -ua * mean);
+        store_any<T, 1>(y + r.a, &o, sy);
+        dw[2 * k] = fmaf(na[k], ua, dw[2 * k]);
+      }
+      if (ok && r.has_b) {
+        const float o = size * fmaf(nb[k], load_weight<T>(a, side, r.b), -ub * mean);
+        store_any<T, 1>(y + r.b, &o, sy);
+        dw[2 * k + 1] = fmaf(nb[k], ub, dw[2 * k + 1]);
       }
     }
   }
   if (parts == nullptr) return;
-
-  // the workgroup's sums: every vector's place in the LDS, then one lane per value
-  const int per_wave = kWave >> a.group_log2;
-  float* sums = reinterpret_cast<float*>(rope_tables);
   __syncthreads();
-  const int mine = (wave * per_wave + (static_cast<int>(threadIdx.x) & (kWave - 1)) /
-                                          (1 << a.group_log2)) * a.dim;
+  float* to = rope_lds + (wave * a.tile.per_pass + l.sub) * a.dim;
 #pragma unroll
   for (int k = 0; k < K; ++k) {
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-      if (p[k].has_a) sums[mine + p[k].a + i] = dw[k][i];
-      if (p[k].has_b) sums[mine + p[k].b + i] = dw[k][V + i];
-    }
+    const RopePair r = rope_pair<ADJ>(a, l, k);
+    if (r.has_a) to[r.a] = dw[2 * k];
+    if (r.has_b) to[r.b] = dw[2 * k + 1];
   }
   __syncthreads();
-  // rows of sums: q's chunks of every walker, then k's
-  const RopeRows rows = rope_rows_of(a.q.heads, a.k.heads, per_wave);
-  const Span sp = VBH_SPAN(parts, static_cast<int64_t>(walkers) * (rows.q + rows.k) * a.dim);
-  const int from = chunk * per_wave;
-  const int cut = min(max(a.q.heads - from, 0), per_wave);                // first k vector
-  const int end = min(max(a.q.heads + a.k.heads - from, 0), per_wave);
-  for (int d = static_cast<int>(threadIdx.x); d < a.dim; d += kRopeBlock) {
-    float q = 0.0f, kk = 0.0f;
-    for (int v = 0; v < kRopeWaves; ++v) {
-      for (int h = 0; h < cut; ++h) q += sums[(v * per_wave + h) * a.dim + d];
-      for (int h = cut; h < end; ++h) kk += sums[(v * per_wave + h) * a.dim + d];
-    }
-    if (cut > 0) {
-      float* to = parts + (static_cast<int64_t>(walker) * rows.q + chunk) * a.dim + d;
-      store_any<float, 1, false>(to, &q, sp);
-    }
-    if (end > cut) {
-      float* to = parts + (static_cast<int64_t>(walkers) * rows.q +
-                           static_cast<int64_t>(walker) * rows.k + chunk - rows.k_from) * a.dim + d;
-      store_any<float, 1, false>(to, &kk, sp);
-    }
-  }
+  write_part(a, rope_lds, a.tile.per_pass, parts);
 }
 
-// Sums over the rows of parts: workgroup (tile, side), 16 columns, 64 lines of lanes.
+// Sums over the rows of parts: a workgroup for 16 values of a side, four to a lane
+// and 16 lines of lanes to a wave, so that a thousand rows take one round of loads.
+// Lines are added up through the wave, then waves through the LDS, in order.
 constexpr int kSumCols = 16;
-constexpr int kSumLines = 64;
+constexpr int kSumWaves = 16;
+constexpr int kSumLines = 16 * kSumWaves;
 
 template <typename W>
-__global__ __launch_bounds__(kSumCols * kSumLines) void qk_weight_grads(
-    const float* parts, int64_t q_rows, int64_t k_rows, int dim, W* dq, W* dk) {
-  __shared__ float lines[kSumLines][kSumCols + 1];
+__global__ __launch_bounds__(kSumWaves* kWave) void qk_weight_grads(const float* parts, int q_rows,
+                                                                    int k_rows, int dim, W* dq,
+                                                                    W* dk) {
+  __shared__ float sums[kSumWaves][kSumCols];
   const bool is_q = blockIdx.y == 0;
   W* out = is_q ? dq : dk;
   if (out == nullptr) return;
-  const Span sp = VBH_SPAN(parts, (q_rows + k_rows) * dim);
+  const Span sp = VBH_SPAN(parts, static_cast<int64_t>(q_rows + k_rows) * dim);
   const Span so = VBH_SPAN(out, dim);
-  const int64_t first = is_q ? 0 : q_rows, rows = is_q ? q_rows : k_rows;
-  const int c = static_cast<int>(threadIdx.x) % kSumCols;
-  const int line = static_cast<int>(threadIdx.x) / kSumCols;
-  const int d = static_cast<int>(blockIdx.x) * kSumCols + c;
-  float sum = 0.0f;
-  if (d < dim) {
-#pragma unroll 8
-    for (int64_t r = line; r < rows; r += kSumLines)
-      sum += load_any<float, 1, false>(parts + (first + r) * dim + d, sp);
+  const int wave = wave_index(), lane = wave_lane();
+  const int d = static_cast<int>(blockIdx.x) * kSumCols + (lane / 16) * 4;
+  const int rows = is_q ? q_rows : k_rows;
+  const float* from = parts + static_cast<int64_t>(is_q ? 0 : q_rows) * dim;
+  float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+  for (int r = wave * 16 + lane % 16; r < rows; r += kSumLines) {
+    const float* row = from + static_cast<int64_t>(r) * dim;
+    if (dim % 4 == 0 && d < dim) {
+      const typename Raw<float, 4>::type x = load_any<float, 4, false>(row + d, sp);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] += x[i];
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (d + i < dim) v[i] += load_any<float, 1, false>(row + d + i, sp);
+    }
   }
-  lines[line][c] = sum;
+  wave_sums<4>(v, 4);
+  if (lane % 16 == 0) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) sums[wave][lane / 4 + i] = v[i];
+  }
   __syncthreads();
-  if (line != 0 || d >= dim) return;
-  for (int i = 1; i < kSumLines; ++i) sum += lines[i][c];
-  store_any<W, 1, false>(out + d, &sum, so);
+  const int c = static_cast<int>(threadIdx.x), to = static_cast<int>(blockIdx.x) * kSumCols + c;
+  if (c >= kSumCols || to >= dim) return;
+  float sum = 0.0f;
+#pragma unroll
+  for (int i = 0; i < kSumWaves; ++i) sum += sums[i][c];
+  store_any<W, 1, false>(out + to, &sum, so);
 }
 
-// Tokens that a wave takes at a time, and the workgroups of a launch: as many as
-// the card holds at once.
-constexpr int kGradTokens = 2;
-constexpr int64_t kGradBlocks = 1024;
+// Waves of a launch: as many as the card holds at once; below some times as many
+// passes a wave takes one at a time.
+constexpr int64_t kGradWaves = 4096;
+constexpr int64_t kGradFewPasses = 4 * kGradWaves;
 
-struct GradShape {
-  RopeShape sh;
-  int u;
-  int64_t walkers;
-};
-
-GradShape grad_shape(const RopeArgs& a, int dt, bool adjacent) {
-  GradShape g;
-  g.sh = rope_shape(a, dt, adjacent);
-  const bool wide = g.sh.k == 1 && g.sh.v == (dt == kF32 ? 4 : 8);
-  g.u = wide && a.tokens * g.sh.chunks >= kRopeFewWaves ? kGradTokens : 1;
-  const int64_t tiles = (a.tokens + kRopeWaves * g.u - 1) / (kRopeWaves * g.u);
-  const int64_t most = std::max<int64_t>(kGradBlocks / std::max(g.sh.chunks, 1), 1);
-  const int64_t turns = (tiles + most - 1) / most;  // of the busiest walker
-  // none of an empty launch: the weights' gradients are then sums of no rows
-  g.walkers = turns > 0 && g.sh.chunks > 0 ? (tiles + turns - 1) / turns : 0;
-  return g;
+// rope_shape, and the walkers of each side: waves in proportion to its work, no more
+// than it has tokens, and none that would only share the last turn of the others.
+void grad_shape(RopeArgs& a, int dt, bool adjacent) {
+  rope_shape(a, dt, adjacent, kGradFewPasses, kGradPasses);
+  auto work = [&](const RopeSide& s) { return int64_t(s.chunks) * (s.per_wave + 2); };
+  const int64_t all = work(a.q) + work(a.k);
+  for (RopeSide* s : {&a.q, &a.k}) {
+    s->walkers = 0;
+    if (s->chunks == 0 || a.tokens == 0) continue;
+    const int64_t most =
+        std::min(a.tokens, std::max<int64_t>(kGradWaves * (s->per_wave + 2) / all, 1));
+    const int64_t turns = (a.tokens + most - 1) / most;
+    s->walkers = static_cast<int>((a.tokens + turns - 1) / turns);
+  }
 }
 
 }  // namespace
 
-int64_t rope_bwd_part_floats(const RopeArgs& a, int dt, bool adjacent) {
-  const GradShape g = grad_shape(a, dt, adjacent);
-  const RopeRows rows = rope_rows_of(a.q.heads, a.k.heads, kWave >> g.sh.group_log2);
-  return g.walkers * (rows.q + rows.k) * a.dim;
+int64_t rope_bwd_part_floats(const RopeArgs& args, int dt, bool adjacent) {
+  RopeArgs a = args;
+  grad_shape(a, dt, adjacent);
+  const RopeRows rows = rope_rows_of(a);
+  return int64_t(rows.q + rows.k) * a.dim;
 }
 
 hipError_t launch_qk_norm_rope_bwd(const RopeArgs& args, int dt, bool adjacent, void* dq_weight,
                                    void* dk_weight, float* parts, hipStream_t s) {
-  const GradShape gs = grad_shape(args, dt, adjacent);
-  const RopeShape& sh = gs.sh;
   RopeArgs a = args;
-  a.group_log2 = sh.group_log2;
-  a.slot_log2 = sh.slot_log2;
-  a.chunks = sh.chunks;
-  const bool part = 2 * a.n_freq < a.dim;
+  grad_shape(a, dt, adjacent);
+  const RopeTile& t = a.tile;
+  const RopeRows rows = rope_rows_of(a);
+  const bool any = 2 * a.n_freq < a.dim || (!adjacent && a.n_freq % t.v != 0);
   const bool sums = dq_weight != nullptr || dk_weight != nullptr;
-  const int per_wave = kWave >> sh.group_log2;
+  const int64_t bytes =
+      a.tokens * (a.q.heads + a.k.heads) * a.dim * (dt == kF32 ? 4 : 2);
+  const int waves = a.q.chunks * a.q.walkers + a.k.chunks * a.k.walkers;
   hipError_t err = hipSuccess;
-  if (gs.walkers * a.chunks > 0) {
-    const size_t lds = std::max(kRopeWaves * gs.u * a.slots * sizeof(float2),
-                                sums ? kRopeWaves * per_wave * a.dim * sizeof(float) : 0);
-    auto go = [&](auto kernel) {
-      launch_kernel(kernel, dim3(static_cast<unsigned>(gs.walkers * a.chunks)), dim3(kRopeBlock),
-                    static_cast<unsigned>(lds), s, a, sums ? parts : nullptr);
+  if (waves > 0) {
+    const size_t row_sums = sums ? size_t(kRopeWaves) * t.per_pass * a.dim : 0;
+    auto go = [&](auto kernel, size_t floats) {
+      launch_kernel(kernel, dim3((waves + kRopeWaves - 1) / kRopeWaves), dim3(kRopeBlock),
+                    static_cast<unsigned>(std::max(floats, row_sums) * sizeof(float)), s, a,
+                    sums ? parts : nullptr);
       err = hipGetLastError();
     };
     dispatch_float_type(dt, [&](auto tt) {
@@ -267,28 +380,32 @@ hipError_t launch_qk_norm_rope_bwd(const RopeArgs& args, int dt, bool adjacent, 
       constexpr int VN = Vec<T>::n;
       dispatch_bool(adjacent, [&](auto ac) {
         constexpr bool A = decltype(ac)::value;
-        if (sh.k > 1) return go(qk_norm_rope_grads<T, 1, kRopeMaxK, 1, A, true>);
-        if (sh.v == VN)
-          return dispatch_bool(part, [&](auto pc) {
-            constexpr bool P = decltype(pc)::value;
-            if (gs.u == 1) go(qk_norm_rope_grads<T, VN, 1, 1, A, P>);
-            else go(qk_norm_rope_grads<T, VN, 1, kGradTokens, A, P>);
-          });
-        if constexpr (VN == 8)
-          if (sh.v == 4) return go(qk_norm_rope_grads<T, 4, 1, 1, A, true>);
-        if (sh.v == 2) return go(qk_norm_rope_grads<T, 2, 1, 1, A, true>);
-        go(qk_norm_rope_grads<T, 1, 1, 1, A, true>);
+        if (t.v == 1) {
+          const size_t floats = size_t(2) * kRopeWaves * a.n_freq;
+          if ((a.dim + 1) / 2 <= kWave) go(qk_norm_rope_value_grads<T, 1, A>, floats);
+          else go(qk_norm_rope_value_grads<T, kRopePairs, A>, floats);
+          return;
+        }
+        const size_t floats =
+            size_t(kRopeWaves) * (rope_table_floats(a.n_freq) +
+                                  (t.lanes_log2 < 0 ? 2 * kGradPasses * kRopeScratch : 0));
+        auto grads = [&](auto mc) {
+          constexpr int M = decltype(mc)::value;
+          if (t.v == VN && !any) go(qk_norm_rope_grads<T, VN, A, false, M>, floats);
+          else if (t.v == VN) go(qk_norm_rope_grads<T, VN, A, true, M>, floats);
+          else if (VN == 8 && t.v == 4) go(qk_norm_rope_grads<T, 4, A, true, M>, floats);
+          else go(qk_norm_rope_grads<T, 2, A, true, M>, floats);
+        };
+        dispatch_rope_mem(rope_mem(2 * bytes, bytes), grads);
       });
     });
   }
   if (err != hipSuccess || !sums) return err;
-  const RopeRows rows = rope_rows_of(a.q.heads, a.k.heads, per_wave);
   auto sum = [&](auto tag) {
     using W = typename decltype(tag)::type;
     launch_kernel(qk_weight_grads<W>, dim3((a.dim + kSumCols - 1) / kSumCols, 2),
-                  dim3(kSumCols * kSumLines), 0, s, parts, gs.walkers * rows.q,
-                  gs.walkers * rows.k, a.dim, static_cast<W*>(dq_weight),
-                  static_cast<W*>(dk_weight));
+                  dim3(kSumWaves * kWave), 0, s, parts, rows.q, rows.k, a.dim,
+                  static_cast<W*>(dq_weight), static_cast<W*>(dk_weight));
     err = hipGetLastError();
   };
   if (a.w_f32) sum(TypeTag<float>{});

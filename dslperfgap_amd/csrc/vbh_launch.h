@@ -322,9 +322,22 @@ struct RopeSide {
   const void* w = nullptr;  // weight or null
   int64_t xs[3] = {0, 0, 0}, gs[3] = {0, 0, 0};
   int heads = 0;
+  // set by the launcher: passes (waves' worth of vectors, RopeTile) that a wave takes
+  // at a time, and how many such shares a token has
+  int per_wave = 1, chunks = 0;
+  int walkers = 0;          // backward: waves of each share, each with every
+                            // walkers-th token
+};
+// How a token's vectors lie over lanes.
+struct RopeTile {
+  int v = 1;          // values per lane access; 1: pair by pair (rope_values)
+  int lanes = 1;      // of a vector
+  int lanes_log2 = 0; // -1: not a power of two
+  int per_pass = 64;  // vectors that a wave holds side by side
 };
 struct RopeArgs {
-  RopeSide q, k;
+  RopeSide q, k;  // side 0, side 1 (side())
+  __host__ __device__ const RopeSide& side(bool is_k) const { return (&q)[is_k ? 1 : 0]; }
   const void* pos = nullptr;
   const void* freq = nullptr;
   int64_t pos_stride[3] = {0, 0, 0};  // axis, batch, token
@@ -332,43 +345,21 @@ struct RopeArgs {
   int64_t tokens = 0;                 // batch * seq, at least 1
   int batch = 1, seq = 1;
   int dim = 0, n_freq = 0;
-  int slots = 0;                      // pairs of a vector, passing ones too: ceil(dim / 2)
   int axes = 1, section_order = 0;
   int ends[kRopeMaxAxes] = {0, 0, 0, 0};  // axis_of
   int pos_dt = 0, f64_freq = 0, w_f32 = 0;
   float scale = 1.0f, sin_scale = 1.0f;   // of cos and of sin (backward: -scale)
   float eps = 0.0f;
+  // set by the launcher
+  RopeTile tile;
   int64_t first = 0;                  // token that the launch begins with
-  // set by the launcher: lanes per vector and slots as powers of two, waves that
-  // share a token
-  int group_log2 = 0, slot_log2 = 0, chunks = 1;
 };
-// Longest walk of a lane over a vector whose values no wider piece fits.
-constexpr int kRopeMaxK = 8;
-// Launches of fewer waves, at a token each, give a wave one token.
-constexpr int64_t kRopeFewWaves = 4096;
-// How vectors lie over lanes: v values per piece, k pieces per lane, the
-// powers of two that RopeArgs names.
-struct RopeShape {
-  int v = 1, k = 1;
-  int group_log2 = 0, slot_log2 = 0, chunks = 1;
-};
-RopeShape rope_shape(const RopeArgs& a, int dt, bool adjacent);
-// Chunks of a token that hold queries and that hold keys (one may hold both), and
-// the first of the latter.
-struct RopeRows {
-  int q, k, k_from;
-};
-__host__ __device__ inline RopeRows rope_rows_of(int q_heads, int k_heads, int per_wave) {
-  RopeRows r;
-  r.q = (q_heads + per_wave - 1) / per_wave;
-  r.k_from = q_heads / per_wave;
-  r.k = k_heads > 0 ? (q_heads + k_heads + per_wave - 1) / per_wave - r.k_from : 0;
-  return r;
-}
 hipError_t launch_rope(const RopeArgs& a, int dt, bool adjacent, bool norm, hipStream_t s);
-// The norm's backward.  With a.q.w / a.k.w wanted (dq_weight, dk_weight not null)
-// `parts` holds rope_bwd_part_floats(a, dt, adjacent) floats.
+// Fills a.tile and the sides' per_wave and chunks; few: launches below this many
+// passes give a wave one.
+void rope_shape(RopeArgs& a, int dt, bool adjacent, int64_t few, int most);
+// The norm's backward.  With the weights' gradients wanted (dq_weight, dk_weight
+// not null) `parts` holds rope_bwd_part_floats(a, dt, adjacent) floats.
 int64_t rope_bwd_part_floats(const RopeArgs& a, int dt, bool adjacent);
 hipError_t launch_qk_norm_rope_bwd(const RopeArgs& a, int dt, bool adjacent, void* dq_weight,
                                    void* dk_weight, float* parts, hipStream_t s);

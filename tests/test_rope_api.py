@@ -267,6 +267,11 @@ def test_entry_points_refuse_null_pointers_and_small_workspaces():
                 continue
             with pytest.raises(_lib.VbhError, match="null pointer|workspace"):
                 _lib.call(name, *args[:i], None, *args[i + 1:])
+    for name, args in _entries(_desc()):
+        outs = (5, 6) if name.startswith("vbh_rope") else (7, 8) if "fwd" in name else (9, 10)
+        for i in outs:
+            with pytest.raises(_lib.VbhError, match="16-byte aligned"):
+                _lib.call(name, *args[:i], 24, *args[i + 1:])
     d = _desc()
     need = _lib.lib().vbh_qk_norm_rope_workspace_bytes(d)
     assert need > 0 and need % (4 * D) == 0
