@@ -224,7 +224,8 @@ struct RopeAngles {
 // passes
 // ---------------------------------------------------------------------------
 
-// A lane's place: vector `sub` of the pass, vector access `at` of it.
+// A lane's place: vector `sub` of the pass, access `at` of it (the last one's for
+// lanes behind it, which are not live).
 struct RopeLane {
   int sub, at;
   bool live;
@@ -233,8 +234,9 @@ __device__ __forceinline__ RopeLane rope_lane(const RopeArgs& a) {
   const int lane = wave_lane();
   RopeLane l;
   l.sub = a.tile.lanes_log2 >= 0 ? lane >> a.tile.lanes_log2 : small_quotient(lane, a.tile.lanes);
-  l.at = lane - l.sub * a.tile.lanes;
-  l.live = l.sub < a.tile.per_pass;
+  const int at = lane - l.sub * a.tile.lanes;
+  l.live = l.sub < a.tile.per_pass && at < a.tile.accesses;
+  l.at = min(at, a.tile.accesses - 1);
   return l;
 }
 
@@ -249,9 +251,10 @@ struct RopePartner {
 template <int V, bool ANY>
 __device__ __forceinline__ RopePartner<V> rope_partner(const RopeArgs& a, const RopeLane& l) {
   RopePartner<V> p;
+  const int first_lane = l.sub * a.tile.lanes;
   if constexpr (!ANY) {
     const int away = a.n_freq / V;
-    p.lane[0] = p.lane[1] = wave_lane() + (l.at < away ? away : -away);
+    p.lane[0] = p.lane[1] = first_lane + (l.at < away ? l.at + away : l.at - away);
     p.crossed = false;
   } else {
     const int away = a.n_freq / (V / 2);  // halves
@@ -260,7 +263,7 @@ __device__ __forceinline__ RopePartner<V> rope_partner(const RopeArgs& a, const 
     for (int h = 0; h < 2; ++h) {
       const int mine = 2 * l.at + h;
       const int theirs = mine < away ? mine + away : mine < 2 * away ? mine - away : mine;
-      p.lane[h] = wave_lane() - l.at + (theirs >> 1);
+      p.lane[h] = first_lane + (theirs >> 1);
     }
   }
   return p;
@@ -400,6 +403,8 @@ template <int N>
 __device__ __forceinline__ void vector_sums(const RopeArgs& a, const RopeLane& l, float (&v)[N],
                                             float* scratch) {
   if (a.tile.lanes_log2 >= 0) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = l.live ? v[i] : 0.0f;
     wave_sums<N>(v, a.tile.lanes_log2);
     return;
   }

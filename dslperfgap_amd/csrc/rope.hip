@@ -14,6 +14,9 @@
 
 namespace vbh {
 
+#ifndef ZPAD
+#define ZPAD 5 * all(t.accesses) > 4 * all(padded)
+#endif
 #ifndef ZFB
 #define ZFB 6
 #endif
@@ -178,7 +181,7 @@ constexpr int64_t kRopeMaxGrid = ((int64_t(1) << 32) - 1) / kRopeBlock;
 
 }  // namespace
 
-void rope_shape(RopeArgs& a, int dt, bool adjacent, int64_t few, int most) {
+void rope_shape(RopeArgs& a, int dt, bool adjacent, bool norm, int64_t few, int most) {
   RopeTile& t = a.tile;
   // the widest access that fits vectors and, in half accesses that are whole words,
   // the way to the partners
@@ -188,24 +191,36 @@ void rope_shape(RopeArgs& a, int dt, bool adjacent, int64_t few, int most) {
     return a.dim % v == 0 && (adjacent || a.n_freq % step == 0);
   };
   while (t.v > 1 && !fits(t.v)) t.v /= 2;
-  t.lanes = a.dim / t.v;
-  if (t.v == 1 || t.lanes > kWave) {  // pair by pair, lanes a power of two
+  t.accesses = a.dim / t.v;
+  if (t.v == 1 || t.accesses > kWave) {  // pair by pair
     t.v = 1;
-    const int slots = std::min((a.dim + 1) / 2, kWave);
-    for (t.lanes = 1; t.lanes < slots;) t.lanes *= 2;
+    t.accesses = std::min((a.dim + 1) / 2, kWave);
     most = 1;
   }
+  int padded = 1;
+  while (padded < t.accesses) padded *= 2;
+  auto passes = [&](const RopeSide& side, int lanes) {
+    return (side.heads + kWave / lanes - 1) / (kWave / lanes);
+  };
+  auto all = [&](int lanes) { return passes(a.q, lanes) + passes(a.k, lanes); };
+  // Vectors of no power of two of accesses: side by side without a gap, or a power of
+  // two of lanes apart, which leaves lanes idle but sums in registers.  MI355X, 16384
+  // tokens of 32 + 8 bf16 heads, passes and us, side by side / apart: heads of 96,
+  // 9 / 10 passes, norm SIDE96 / APART96; heads of 80, 8 / 10 passes, norm SIDE80 / APART80
+  t.lanes = t.v == 1 || (norm && ZPAD) ||
+                    all(t.accesses) == all(padded)
+                ? padded
+                : t.accesses;
   t.lanes_log2 = (t.lanes & (t.lanes - 1)) == 0 ? __builtin_ctz(t.lanes) : -1;
   t.per_pass = kWave / t.lanes;
-  const int pq = (a.q.heads + t.per_pass - 1) / t.per_pass;
-  const int pk = (a.k.heads + t.per_pass - 1) / t.per_pass;
+  const int pq = passes(a.q, t.lanes), pk = passes(a.k, t.lanes);
   if (a.tokens * (pq + pk) < few) most = 1;
-  auto share = [&](RopeSide& side, int passes) {
+  auto share = [&](RopeSide& side, int n) {
     // the fewest passes with a wave's own work (angles and the like) taken for two;
     // the larger share of two alike
     int best = 1 << 30;
     for (int u = 1; u <= most; ++u) {
-      const int chunks = (passes + u - 1) / u;
+      const int chunks = (n + u - 1) / u;
       if (chunks * (u + 2) > best) continue;
       best = chunks * (u + 2);
       side.per_wave = u;
@@ -218,7 +233,7 @@ void rope_shape(RopeArgs& a, int dt, bool adjacent, int64_t few, int most) {
 
 hipError_t launch_rope(const RopeArgs& args, int dt, bool adjacent, bool norm, hipStream_t s) {
   RopeArgs a = args;
-  rope_shape(a, dt, adjacent, kRopeFewPasses, kRopePasses);
+  rope_shape(a, dt, adjacent, norm, kRopeFewPasses, kRopePasses);
   const RopeTile& t = a.tile;
   const int chunks = a.q.chunks + a.k.chunks;
   const bool any = 2 * a.n_freq < a.dim || (!adjacent && a.n_freq % t.v != 0);

@@ -333,7 +333,7 @@ constexpr int64_t kGradFewPasses = 4 * kGradWaves;
 // rope_shape, and the walkers of each side: waves in proportion to its work, no more
 // than it has tokens, and none that would only share the last turn of the others.
 void grad_shape(RopeArgs& a, int dt, bool adjacent) {
-  rope_shape(a, dt, adjacent, kGradFewPasses, kGradPasses);
+  rope_shape(a, dt, adjacent, true, kGradFewPasses, kGradPasses);
   auto work = [&](const RopeSide& s) { return int64_t(s.chunks) * (s.per_wave + 2); };
   const int64_t all = work(a.q) + work(a.k);
   for (RopeSide* s : {&a.q, &a.k}) {

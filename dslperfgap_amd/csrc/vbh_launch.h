@@ -331,7 +331,9 @@ struct RopeSide {
 // How a token's vectors lie over lanes.
 struct RopeTile {
   int v = 1;          // values per lane access; 1: pair by pair (rope_values)
-  int lanes = 1;      // of a vector
+  int accesses = 1;   // of a vector
+  int lanes = 1;      // from one vector of a wave to the next: as many, or the power
+                      // of two behind
   int lanes_log2 = 0; // -1: not a power of two
   int per_pass = 64;  // vectors that a wave holds side by side
 };
@@ -355,9 +357,9 @@ struct RopeArgs {
   int64_t first = 0;                  // token that the launch begins with
 };
 hipError_t launch_rope(const RopeArgs& a, int dt, bool adjacent, bool norm, hipStream_t s);
-// Fills a.tile and the sides' per_wave and chunks; few: launches below this many
-// passes give a wave one.
-void rope_shape(RopeArgs& a, int dt, bool adjacent, int64_t few, int most);
+// Fills a.tile and the sides' per_wave and chunks; norm: vectors are summed over;
+// few: launches below this many passes give a wave one, most: a wave's at most.
+void rope_shape(RopeArgs& a, int dt, bool adjacent, bool norm, int64_t few, int most);
 // The norm's backward.  With the weights' gradients wanted (dq_weight, dk_weight
 // not null) `parts` holds rope_bwd_part_floats(a, dt, adjacent) floats.
 int64_t rope_bwd_part_floats(const RopeArgs& a, int dt, bool adjacent);
