@@ -18,12 +18,9 @@ POSITION_CODES = {torch.int32: _lib.I32, torch.int64: _lib.I64, torch.float32: _
 ORDERS = {"blocks": _lib.ROPE_BLOCKS, "cycle": _lib.ROPE_CYCLE}
 PAIRINGS = {"half": _lib.ROPE_HALF, "adjacent": _lib.ROPE_ADJACENT}
 
+_raw_device, _raw_stream = _bridge._raw_device, _bridge._raw_stream
+# what decides a call (shapes, strides, dtypes, options) -> its plan (make_plan)
 _PLANS = _bridge.PlanCache()
-
-
-class Plan:
-    """The descriptor of one launch, its address, and the outputs' shapes."""
-    __slots__ = ("desc", "addr", "q_shape", "q_strides", "k_shape", "k_strides", "ws_bytes")
 
 
 def _strides(t):
@@ -74,7 +71,9 @@ def _position_strides(positions, lead, axes, what):
 
 def make_plan(what, q, k, positions, inv_freq, sections, section_order, pairing, scale, eps,
               weights, grads):
-    """The Plan of a call, or the error its arguments deserve.  `weights`: None (no
+    """The plan of a call whose vectors and weights the kernels read as they are: (entry
+    point, descriptor's address, shape and strides of the queries' output, of the keys',
+    workspace bytes, descriptor), or the error its arguments deserve.  `weights`: None (no
     norm) or (q_weight, k_weight); `grads`: None or (dq_out, dk_out)."""
     # the vectors that run through the rotation, under the name the caller knows
     names = ("dq_out", "dk_out") if what == "rope_bwd" else ("q", "k")
@@ -127,14 +126,12 @@ def make_plan(what, q, k, positions, inv_freq, sections, section_order, pairing,
             if tuple(w.shape) != (dim,):
                 raise ValueError(f"{what}: {name} must have shape [{dim}], got {list(w.shape)}")
             d.w_dtype = _bridge.FLOAT_CODES[w.dtype]
-    p = Plan()
-    p.desc, p.addr = d, ctypes.addressof(d)
-    p.q_shape, p.k_shape = tuple(q.shape), tuple(k.shape)
-    p.q_strides = _bridge.contiguous_strides(p.q_shape)
-    p.k_strides = _bridge.contiguous_strides(p.k_shape)
-    p.ws_bytes = (_lib.lib().vbh_qk_norm_rope_workspace_bytes(ctypes.byref(d))
-                  if grads is not None else 0)
-    return p
+    q_shape, k_shape = tuple(q.shape), tuple(k.shape)
+    ws_bytes = (_lib.lib().vbh_qk_norm_rope_workspace_bytes(ctypes.byref(d))
+                if grads is not None else 0)
+    return (_lib.entry("vbh_" + what), ctypes.addressof(d), q_shape,
+            _bridge.contiguous_strides(q_shape), k_shape, _bridge.contiguous_strides(k_shape),
+            ws_bytes, d)
 
 
 def _weight(w, dtype, what, name):
@@ -147,100 +144,131 @@ def _weight(w, dtype, what, name):
 
 
 def _weights(q_weight, k_weight, dtype, what):
+    """Both weights as the kernels read them, of one dtype."""
+    if (q_weight is not None and k_weight is not None and q_weight.dtype is k_weight.dtype and
+            (q_weight.dtype is dtype or q_weight.dtype is torch.float32) and
+            q_weight.is_contiguous() and k_weight.is_contiguous()):
+        return q_weight, k_weight
     qw, kw = _weight(q_weight, dtype, what, "q_weight"), _weight(k_weight, dtype, what, "k_weight")
     if qw is not None and kw is not None and qw.dtype is not kw.dtype:
         return qw.float(), kw.float()
     return qw, kw
 
 
-def _form(w):
-    return None if w is None else (w.shape, w.dtype)
+def _contiguous(t):
+    """`t` with vectors that are contiguous."""
+    st = t.stride()
+    return t if not st or st[-1] == 1 else t.contiguous()
 
 
-def plan(what, q, k, positions, inv_freq, sections, section_order, pairing, scale, eps=0.0,
-         weights=None, grads=None):
-    """The cached Plan of a call whose vectors and weights the kernels read as they are."""
-    if type(sections) is list:
-        sections = tuple(sections)
-    key = (what, q.shape, q.stride(), q.dtype, k.shape, k.stride(), k.dtype, positions.shape,
-           positions.stride(), positions.dtype, inv_freq.shape, inv_freq.stride(), inv_freq.dtype,
-           sections, section_order, pairing, scale)
-    if weights is not None:
-        key += (eps, _form(weights[0]), _form(weights[1]))
-    if grads is not None:
-        g, h = grads
-        key += (g.shape, g.stride(), g.dtype, h.shape, h.stride(), h.dtype)
-    p = _PLANS.get(key)
-    if p is None:
-        p = _PLANS.put(key, make_plan(what, q, k, positions, inv_freq, sections, section_order,
-                                      pairing, float(scale), float(eps), weights, grads))
-    return p
-
-
-def _device(what, *tensors):
-    """The GPU all tensors lie on."""
-    dev = tensors[0].get_device()
+def _on(dev, what, *tensors):
+    """The GPU all tensors lie on, `dev` or the error they deserve."""
     for t in tensors:
         if t is not None and (dev < 0 or t.get_device() != dev):
             return _bridge.require_gpu(what, *tensors)
     return dev
 
 
-def _outputs(q, p):
-    return (q.new_empty_strided(p.q_shape, p.q_strides),
-            q.new_empty_strided(p.k_shape, p.k_strides))
-
-
-def _vectors(t):
-    """`t` with vectors that are contiguous."""
-    st = t.stride()
-    return t if not st or st[-1] == 1 else t.contiguous()
+def _run(fn, what, dev, *args):
+    if dev == _raw_device():
+        rc = fn(*args, _raw_stream(dev))
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, _raw_stream(dev))
+    if rc != 0:
+        raise _lib.VbhError("vbh_" + what, rc, _lib.last_error())
 
 
 def rotate(what, q, k, positions, inv_freq, sections, section_order, pairing, scale):
     """rope_fwd, and rope_bwd with q and k the incoming gradients."""
-    q, k = _vectors(q), _vectors(k)
-    p = plan(what, q, k, positions, inv_freq, sections, section_order, pairing, scale)
-    dev = _device(what, q, k, positions, inv_freq)
-    q_out, k_out = _outputs(q, p)
-    _bridge.launch("vbh_" + what, dev, p.addr, q.data_ptr(), k.data_ptr(), positions.data_ptr(),
-                   inv_freq.data_ptr(), q_out.data_ptr(), k_out.data_ptr())
+    if type(sections) is list:
+        sections = tuple(sections)
+    key = (what, q.shape, q.stride(), q.dtype, k.shape, k.stride(), k.dtype, positions.shape,
+           positions.stride(), positions.dtype, inv_freq.shape, inv_freq.stride(), inv_freq.dtype,
+           sections, section_order, pairing, scale)
+    p = _PLANS.get(key)
+    if p is None:
+        qc, kc = _contiguous(q), _contiguous(k)
+        if qc is not q or kc is not k:
+            return rotate(what, qc, kc, positions, inv_freq, sections, section_order, pairing,
+                          scale)
+        p = _PLANS.put(key, make_plan(what, q, k, positions, inv_freq, sections, section_order,
+                                      pairing, float(scale), 0.0, None, None))
+    dev = q.get_device()
+    if (dev < 0 or k.get_device() != dev or positions.get_device() != dev or
+            inv_freq.get_device() != dev):
+        dev = _bridge.require_gpu(what, q, k, positions, inv_freq)
+    fn, desc, q_shape, q_strides, k_shape, k_strides, _, _ = p
+    q_out = q.new_empty_strided(q_shape, q_strides)
+    k_out = k.new_empty_strided(k_shape, k_strides)
+    _run(fn, what, dev, desc, q.data_ptr(), k.data_ptr(), positions.data_ptr(),
+         inv_freq.data_ptr(), q_out.data_ptr(), k_out.data_ptr())
     return q_out, k_out
 
 
 def norm_rotate(q, k, q_weight, k_weight, positions, inv_freq, eps, sections, section_order,
                 pairing, scale):
     what = "qk_norm_rope_fwd"
-    q, k = _vectors(q), _vectors(k)
+    if type(sections) is list:
+        sections = tuple(sections)
     qw, kw = _weights(q_weight, k_weight, q.dtype, what)
-    p = plan(what, q, k, positions, inv_freq, sections, section_order, pairing, scale, eps,
-             (qw, kw))
-    dev = _device(what, q, k, qw, kw, positions, inv_freq)
-    q_out, k_out = _outputs(q, p)
-    _bridge.launch("vbh_qk_norm_rope_fwd", dev, p.addr, q.data_ptr(), k.data_ptr(),
-                   _bridge.ptr(qw), _bridge.ptr(kw), positions.data_ptr(), inv_freq.data_ptr(),
-                   q_out.data_ptr(), k_out.data_ptr())
+    key = (what, q.shape, q.stride(), q.dtype, k.shape, k.stride(), k.dtype, positions.shape,
+           positions.stride(), positions.dtype, inv_freq.shape, inv_freq.stride(), inv_freq.dtype,
+           sections, section_order, pairing, scale, eps, None if qw is None else qw.shape,
+           None if kw is None else kw.shape, (kw if qw is None else qw) is None or
+           (kw if qw is None else qw).dtype)
+    p = _PLANS.get(key)
+    if p is None:
+        qc, kc = _contiguous(q), _contiguous(k)
+        if qc is not q or kc is not k:
+            return norm_rotate(qc, kc, qw, kw, positions, inv_freq, eps, sections,
+                               section_order, pairing, scale)
+        p = _PLANS.put(key, make_plan(what, q, k, positions, inv_freq, sections, section_order,
+                                      pairing, float(scale), float(eps), (qw, kw), None))
+    dev = _on(q.get_device(), what, q, k, qw, kw, positions, inv_freq)
+    fn, desc, q_shape, q_strides, k_shape, k_strides, _, _ = p
+    q_out = q.new_empty_strided(q_shape, q_strides)
+    k_out = k.new_empty_strided(k_shape, k_strides)
+    _run(fn, what, dev, desc, q.data_ptr(), k.data_ptr(), None if qw is None else qw.data_ptr(),
+         None if kw is None else kw.data_ptr(), positions.data_ptr(), inv_freq.data_ptr(),
+         q_out.data_ptr(), k_out.data_ptr())
     return q_out, k_out
 
 
 def norm_rotate_grads(dq_out, dk_out, q, k, q_weight, k_weight, positions, inv_freq, eps,
                       sections, section_order, pairing, scale):
     what = "qk_norm_rope_bwd"
-    q, k = _vectors(q), _vectors(k)
-    dq_out, dk_out = _vectors(dq_out), _vectors(dk_out)
+    if type(sections) is list:
+        sections = tuple(sections)
     qw, kw = _weights(q_weight, k_weight, q.dtype, what)
-    p = plan(what, q, k, positions, inv_freq, sections, section_order, pairing, scale, eps,
-             (qw, kw), (dq_out, dk_out))
-    dev = _device(what, q, k, dq_out, dk_out, qw, kw, positions, inv_freq)
-    dq, dk = _outputs(q, p)
+    key = (what, q.shape, q.stride(), q.dtype, k.shape, k.stride(), k.dtype, positions.shape,
+           positions.stride(), positions.dtype, inv_freq.shape, inv_freq.stride(), inv_freq.dtype,
+           sections, section_order, pairing, scale, eps, None if qw is None else qw.shape,
+           None if kw is None else kw.shape, (kw if qw is None else qw) is None or
+           (kw if qw is None else qw).dtype, dq_out.shape, dq_out.stride(), dq_out.dtype,
+           dk_out.shape, dk_out.stride(), dk_out.dtype)
+    p = _PLANS.get(key)
+    if p is None:
+        args = (dq_out, dk_out, q, k)
+        dense = [_contiguous(t) for t in args]
+        if any(a is not b for a, b in zip(args, dense)):
+            return norm_rotate_grads(*dense, q_weight, k_weight, positions, inv_freq, eps,
+                                     sections, section_order, pairing, scale)
+        p = _PLANS.put(key, make_plan(what, q, k, positions, inv_freq, sections, section_order,
+                                      pairing, float(scale), float(eps), (qw, kw),
+                                      (dq_out, dk_out)))
+    dev = _on(q.get_device(), what, q, k, dq_out, dk_out, qw, kw, positions, inv_freq)
+    fn, desc, q_shape, q_strides, k_shape, k_strides, n, _ = p
+    dq = q.new_empty_strided(q_shape, q_strides)
+    dk = k.new_empty_strided(k_shape, k_strides)
     dqw = None if qw is None else torch.empty_like(qw)
     dkw = None if kw is None else torch.empty_like(kw)
-    n = p.ws_bytes if qw is not None or kw is not None else 0
+    if qw is None and kw is None:
+        n = 0
     ws = _bridge.empty(q, (n,), torch.uint8) if n else None
-    _bridge.launch("vbh_qk_norm_rope_bwd", dev, p.addr, dq_out.data_ptr(), dk_out.data_ptr(),
-                   q.data_ptr(), k.data_ptr(), _bridge.ptr(qw), _bridge.ptr(kw),
-                   positions.data_ptr(), inv_freq.data_ptr(), dq.data_ptr(), dk.data_ptr(),
-                   _bridge.ptr(dqw), _bridge.ptr(dkw), _bridge.ptr(ws), n)
+    _run(fn, what, dev, desc, dq_out.data_ptr(), dk_out.data_ptr(), q.data_ptr(), k.data_ptr(),
+         _bridge.ptr(qw), _bridge.ptr(kw), positions.data_ptr(), inv_freq.data_ptr(),
+         dq.data_ptr(), dk.data_ptr(), _bridge.ptr(dqw), _bridge.ptr(dkw), _bridge.ptr(ws), n)
     if dqw is not None and dqw.dtype is not q_weight.dtype:
         dqw = dqw.to(q_weight.dtype)
     if dkw is not None and dkw.dtype is not k_weight.dtype:

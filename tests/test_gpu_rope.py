@@ -385,8 +385,8 @@ def test_memory_around_the_outputs_is_left_alone(dim, dtype):
     print(f"[gpu] guards {dim} {dtype}", flush=True)
     q, k, gq, gk, w, pos, freq = _case(tokens=67, hq=5, hk=3, dim=dim, dtype=dtype)
     want = qk_norm_rope_bwd(gq, gk, q, k, *w, pos, freq)
-    p = _rope.plan("qk_norm_rope_bwd", q, k, pos, freq, None, "blocks", "half", 1.0, EPS,
-                   tuple(w), (gq, gk))
+    _, desc, _, _, _, _, ws_bytes, _kept = _rope.make_plan(
+        "qk_norm_rope_bwd", q, k, pos, freq, None, "blocks", "half", 1.0, EPS, tuple(w), (gq, gk))
     bufs = []
 
     def guarded(n, dt):
@@ -395,10 +395,10 @@ def test_memory_around_the_outputs_is_left_alone(dim, dtype):
         return b[128:].data_ptr()
 
     ptrs = [guarded(t.numel(), t.dtype) for t in want]
-    ws = guarded(p.ws_bytes // 4, F32)
-    _lib.call("vbh_qk_norm_rope_bwd", p.addr, gq.data_ptr(), gk.data_ptr(), q.data_ptr(),
+    ws = guarded(ws_bytes // 4, F32)
+    _lib.call("vbh_qk_norm_rope_bwd", desc, gq.data_ptr(), gk.data_ptr(), q.data_ptr(),
               k.data_ptr(), w[0].data_ptr(), w[1].data_ptr(), pos.data_ptr(), freq.data_ptr(),
-              *ptrs, ws, p.ws_bytes, torch.cuda.current_stream().cuda_stream)
+              *ptrs, ws, ws_bytes, torch.cuda.current_stream().cuda_stream)
     torch.cuda.synchronize()
     for (b, n), t in zip(bufs, want):
         assert torch.equal(b[128:128 + n], t.reshape(-1))

@@ -181,17 +181,24 @@ def test_plans_hold_the_strides_and_are_kept():
     q, k = whole[:, :, :4], whole[:, :, 4:6]
     pos = torch.zeros(5, dtype=torch.int32)
     freq = ref.inv_freq(N, dtype=torch.float64)
-    args = ("rope_fwd", q, k, pos, freq, None, "blocks", "half", 1.0)
-    p = _rope.plan(*args)
-    d = p.desc
-    assert _rope.plan(*args) is p and p.addr == ctypes.addressof(d)
+    def plan():
+        with pytest.raises(ValueError, match="GPU tensors"):
+            rope_fwd(q, k, pos, freq)
+        return list(_rope._PLANS.values())[-1]
+
+    _rope._PLANS.cache_clear()
+    p = plan()
+    _, address, q_shape, q_strides, k_shape, k_strides, ws_bytes, d = p
+    assert plan() is p and len(_rope._PLANS) == 1 and address == ctypes.addressof(d)
     assert [d.batch, d.seq, d.q_heads, d.k_heads, d.head_dim, d.n_freq] == [2, 5, 4, 2, D, N]
     assert list(d.q_stride) == [5 * 8 * D, 8 * D, D] == list(d.k_stride)
     assert list(d.pos_stride) == [0, 0, 1] and d.pos_dtype == _lib.I32 and d.f64_freq == 1
-    assert p.q_strides == (5 * 4 * D, 4 * D, D, 1)
-    t = torch.randn(2, 4, 5, D).transpose(1, 2)
-    assert list(_rope.plan("rope_fwd", t, t, pos, freq, None, "blocks", "half",
-                           1.0).desc.q_stride) == [20 * D, D, 5 * D]
+    assert q_shape == (2, 5, 4, D) and q_strides == (5 * 4 * D, 4 * D, D, 1)
+    assert k_shape == (2, 5, 2, D) and ws_bytes == 0
+    q = k = torch.randn(2, 4, 5, D).transpose(1, 2)
+    assert list(plan()[-1].q_stride) == [20 * D, D, 5 * D]
+    q = k = torch.randn(2, 5, 4, D, 2)[..., 0]  # copied: the plan is that of the copy
+    assert list(plan()[-1].q_stride) == [20 * D, 4 * D, D]
 
 
 # ---------------------------------------------------------------------------
