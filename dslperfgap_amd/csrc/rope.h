@@ -10,16 +10,14 @@
 //   adjacent pairing: a lane's values pair among themselves
 //   half pairing:     the partners lie in other lanes of the vector's, n_freq / V
 //                     away, whose 16 bytes come over the LDS crossbar as they are
-//                     stored; both lanes then widen both vectors.  Half accesses
-//                     (of V / 2 values) have partners of their own, so that n_freq
-//                     need only be a multiple of V / 2
+//                     stored; both lanes then widen both vectors (RopePartner)
 // Per value y_i = (x_i C_i + x_partner S_i) r: the cosines and sines, their signs,
 // the scale and the weights meet in C and S once per wave, so that the norm adds
 // one product per value and its sum of squares.
 //
-// Vectors that no lane access of 2 values or more fits (odd sizes, half pairings
-// of an odd number of pairs, more than 64 lanes) go pair by pair: a lane holds
-// both members of a pair (rope_values, qk_norm_rope_value_grads).
+// Vectors that no lane access of 2 values or more fits (odd sizes, more than 64
+// lanes) go pair by pair: a lane holds both members of a pair (rope_values,
+// qk_norm_rope_value_grads).
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -31,30 +29,35 @@
 
 namespace vbh {
 
+constexpr int kCacheSc1 = 1 << 4;  // cache-policy operand: device scope
 constexpr int kRopeWaves = 4;  // waves per workgroup
 constexpr int kRopeBlock = kRopeWaves * kWave;
 constexpr int kRopePairs = 8;  // pairs of a lane that goes pair by pair
 constexpr int kRopePasses = 4; // passes of a wave's share, at most
 
 // How a launch treats memory (rope_mem): kRopeCached, kRopeOnce: nontemporal loads,
-// kRopeStream: nontemporal loads and stores.
+// kRopeStream: nontemporal loads and stores.  All write through the L2 at device scope,
+// so that nothing is left to write back when the kernel ends: MI355X, us without / with:
+// 16384 tokens of 40 bf16 heads of 128, rotation 52.1 / 50.5, backward 91.3 / 86.5;
+// 8192 tokens, norm and rotation 29.5 / 28.9; 32768, rotation (kRopeStream) 107.9 / 105.3.
 enum RopeMem : int { kRopeCached = 0, kRopeOnce = 1, kRopeStream = 2 };
 
 // What a launch reads and writes, against the 256 MiB cache in front of the memory.
 // MI355X, 16384 tokens of 40 bf16 heads (168 MB in, as much out; three sets of inputs
 // in turn), us by loads / stores, nt: nontemporal:
+// (without the write-through)
 //   forward, 168 MB in and out   nt / nt 55.6, nt / plain 51.8, plain / plain 61.1
 //   the same, 336 MB             nt / nt 108.4, nt / plain 116
-//   the same, 84 MB              nt / nt 29.8, nt / plain 29.3, plain / plain 29.0
+//   the same with the norm, 84 MB nt / plain 29.5, plain / plain 33.2
 //   the same, 42 MB              nt / nt 16.8, nt / plain 16.7, plain / plain 15.1
 //   backward, 336 MB in, 168 out nt / nt 97.0, nt / plain 91.3, plain / plain 105
 //   the same, 168 MB in, 84 out  nt / nt 52.6, nt / plain 50.2, plain / plain 51.2
 //   the same, 84 MB in, 42 out   nt / nt 31.0, nt / plain 31.6, plain / plain 30.6
-constexpr int64_t kRopeCachedBytes = int64_t(128) << 20;  // read
+constexpr int64_t kRopeCachedBytes = int64_t(128) << 20;  // read and written
 constexpr int64_t kRopeOnceBytes = int64_t(224) << 20;    // written
 inline RopeMem rope_mem(int64_t read, int64_t written) {
   if (written > kRopeOnceBytes) return kRopeStream;
-  return read > kRopeCachedBytes ? kRopeOnce : kRopeCached;
+  return read + written > kRopeCachedBytes ? kRopeOnce : kRopeCached;
 }
 template <typename Fn>
 void dispatch_rope_mem(RopeMem m, Fn&& fn) {
@@ -63,8 +66,20 @@ void dispatch_rope_mem(RopeMem m, Fn&& fn) {
   else fn(std::integral_constant<int, kRopeStream>{});
 }
 
-// Floats of a wave's table of angles, a whole number of 16-byte vectors.
-__host__ __device__ constexpr int rope_table_floats(int n_freq) { return (2 * n_freq + 3) & ~3; }
+// A wave's part of the LDS, in floats (whole 16-byte vectors): its table of angles, the
+// scratch of `sums` sums where vectors are no power of two of lanes, and where a.gather
+// the vectors of `passes` passes.
+struct RopeLds {
+  int table, scratch, rows;
+  __host__ __device__ int all() const { return table + scratch + rows; }
+};
+__host__ __device__ inline RopeLds rope_lds_of(const RopeArgs& a, int sums, int passes) {
+  RopeLds r;
+  r.table = (2 * a.n_freq + 3) & ~3;
+  r.scratch = a.tile.lanes_log2 < 0 ? sums * 128 : 0;
+  r.rows = a.gather ? passes * (kWave * 16 / 4) : 0;
+  return r;
+}
 
 // Values of an operand with strides `st` (for Spans).
 __device__ __forceinline__ int64_t rope_extent(const RopeArgs& a, const int64_t (&st)[3],
@@ -240,19 +255,26 @@ __device__ __forceinline__ RopeLane rope_lane(const RopeArgs& a) {
   return l;
 }
 
-// Half pairing: the lanes that hold the partners of this lane's first and second V / 2
-// values, and whether a half's partner is the other half.  Launches without ANY: all
-// values turn and n_freq is a multiple of V, so that the whole access has one partner.
+// Where the partners of a lane's values are (half pairing), by launch.
+//   kRopeWhole: all values turn and n_freq is a multiple of V: the whole access has its
+//   partners in one lane.
+//   kRopeHalves: some values pass (their own partners), or n_freq is a multiple of V / 2
+//   only: each half of the access has its partners in one lane, in its own half or,
+//   where n_freq is an odd number of halves, in the other (crossed).
+//   kRopeGather: any n_freq; the vectors go through the LDS and every value is read by
+//   itself.
+// Adjacent pairing: kRopeWhole, or kRopeHalves where some values pass.
+enum RopeWay : int { kRopeWhole = 0, kRopeHalves = 1, kRopeGather = 2 };
 template <int V>
 struct RopePartner {
   int lane[2];
   bool crossed;  // of the launch
 };
-template <int V, bool ANY>
+template <int V, int WAY>
 __device__ __forceinline__ RopePartner<V> rope_partner(const RopeArgs& a, const RopeLane& l) {
   RopePartner<V> p;
   const int first_lane = l.sub * a.tile.lanes;
-  if constexpr (!ANY) {
+  if constexpr (WAY == kRopeWhole) {
     const int away = a.n_freq / V;
     p.lane[0] = p.lane[1] = first_lane + (l.at < away ? l.at + away : l.at - away);
     p.crossed = false;
@@ -269,33 +291,72 @@ __device__ __forceinline__ RopePartner<V> rope_partner(const RopeArgs& a, const 
   return p;
 }
 
-// The partners' values as they are stored.
-template <typename T, int V, bool ANY>
-__device__ __forceinline__ typename Raw<T, V>::type partners(const typename Raw<T, V>::type& r,
-                                                             const RopePartner<V>& p) {
-  constexpr int N = V * sizeof(T) / 4;
-  if constexpr (N == 1) {
-    return __builtin_bit_cast(
-        typename Raw<T, V>::type,
-        __builtin_amdgcn_ds_bpermute(4 * p.lane[0], __builtin_bit_cast(int, r)));
-  } else {
-    typedef int words __attribute__((ext_vector_type(N)));
-    const words w = __builtin_bit_cast(words, r);
-    words o;
-#pragma unroll
-    for (int i = 0; i < N; ++i)
-      o[i] = __builtin_amdgcn_ds_bpermute(4 * p.lane[i / (N / 2)],
-                                          ANY && p.crossed ? w[(i + N / 2) % N] : w[i]);
-    return __builtin_bit_cast(typename Raw<T, V>::type, o);
-  }
+// The place of value e's partner in its vector (its own where it passes).
+__device__ __forceinline__ int partner_of(const RopeArgs& a, int e) {
+  return e < a.n_freq ? e + a.n_freq : e < 2 * a.n_freq ? e - a.n_freq : e;
 }
-template <int V, bool ANY>
-__device__ __forceinline__ void partners(const float (&w)[V], const RopePartner<V>& p,
-                                         float (&o)[V]) {
+
+// The partners of U passes' accesses, widened one pass at a time.  `rows`: where
+// a.gather, kRopeRow * U bytes of the wave's own.
+constexpr int kRopeRow = kWave * 16;  // rope_lds_of
+template <typename T, int V, int U, int WAY>
+struct RopePartners {
+  RopePartner<V> p;
+  const T* rows;
+  const RopeArgs& a;
+  const RopeLane& l;
+  __device__ __forceinline__ RopePartners(const RopeArgs& args, const RopeLane& lane,
+                                          const typename Raw<T, V>::type (&r)[U], char* lds)
+      : p(rope_partner<V, WAY>(args, lane)), rows(reinterpret_cast<T*>(lds)), a(args), l(lane) {
+    if constexpr (WAY != kRopeGather) return;
+    wave_lds_fence();
+    if (l.live) {
 #pragma unroll
-  for (int i = 0; i < V; ++i)
-    o[i] = __int_as_float(__builtin_amdgcn_ds_bpermute(
-        4 * p.lane[i / (V / 2)], __float_as_int(ANY && p.crossed ? w[(i + V / 2) % V] : w[i])));
+      for (int u = 0; u < U; ++u)
+        *reinterpret_cast<typename Raw<T, V>::type*>(
+            reinterpret_cast<T*>(lds + u * kRopeRow) + l.sub * a.dim + l.at * V) = r[u];
+    }
+    wave_lds_fence();
+  }
+  __device__ __forceinline__ void get(const typename Raw<T, V>::type& r, int u,
+                                      float (&o)[V]) const {
+    if constexpr (WAY == kRopeGather) {
+      const T* row = rows + u * (kRopeRow / sizeof(T)) + (l.live ? l.sub : 0) * a.dim;
+#pragma unroll
+      for (int i = 0; i < V; ++i) o[i] = static_cast<float>(row[partner_of(a, l.at * V + i)]);
+      return;
+    }
+    constexpr int N = V * sizeof(T) / 4;
+    typename Raw<T, V>::type q;
+    if constexpr (N == 1) {
+      q = __builtin_bit_cast(
+          typename Raw<T, V>::type,
+          __builtin_amdgcn_ds_bpermute(4 * p.lane[0], __builtin_bit_cast(int, r)));
+    } else {
+      typedef int words __attribute__((ext_vector_type(N)));
+      const words w = __builtin_bit_cast(words, r);
+      words x;
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        x[i] = __builtin_amdgcn_ds_bpermute(4 * p.lane[i / (N / 2)],
+                                            WAY == kRopeHalves && p.crossed ? w[(i + N / 2) % N] : w[i]);
+      q = __builtin_bit_cast(typename Raw<T, V>::type, x);
+    }
+#pragma unroll
+    for (int i = 0; i < V; ++i) o[i] = raw_at<T, V>(q, i);
+  }
+};
+
+// One weight, widened (1 without weights).
+template <typename T>
+__device__ __forceinline__ float load_weight(const RopeArgs& a, const RopeSide& side, int i) {
+  if (side.w == nullptr) return 1.0f;
+  if (a.w_f32) {
+    const float* w = static_cast<const float*>(side.w);
+    return load_any<float, 1, false>(w + i, VBH_SPAN(w, a.dim));
+  }
+  const T* w = static_cast<const T*>(side.w);
+  return static_cast<float>(load_any<T, 1, false>(w + i, VBH_SPAN(w, a.dim)));
 }
 
 template <typename W, int V>
@@ -317,34 +378,63 @@ __device__ __forceinline__ void load_weights(const RopeArgs& a, const RopeSide& 
   else widen_weights<T, V>(a, side, l, w);
 }
 
+// The weights of the partners of a lane's values (half pairing).
+template <typename T, int V, int WAY>
+__device__ __forceinline__ void partner_weights(const RopeArgs& a, const RopeSide& side,
+                                                const RopeLane& l, const RopePartner<V>& p,
+                                                const float (&w)[V], float (&o)[V]) {
+  if constexpr (WAY == kRopeGather) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) o[i] = load_weight<T>(a, side, partner_of(a, l.at * V + i));
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < V; ++i)
+    o[i] = __int_as_float(__builtin_amdgcn_ds_bpermute(
+        4 * p.lane[i / (V / 2)],
+        __float_as_int(WAY == kRopeHalves && p.crossed ? w[(i + V / 2) % V] : w[i])));
+}
+
 // How a lane's V values turn: y_i = x_i c[i] + x_partner s[i], passing[i] where
-// they do not (there are such values only with ANY).
+// they do not (not with kRopeWhole).
 template <int V>
 struct Turn {
   float c[V], s[V];
   bool passing[V];
 };
 
-template <int V, bool ADJ, bool ANY>
+template <int V, bool ADJ, int WAY>
 __device__ __forceinline__ void make_turn(const RopeArgs& a, const RopeLane& l,
                                           const float2* table, Turn<V>& t) {
   if constexpr (ADJ) {
 #pragma unroll
     for (int i = 0; i < V; i += 2) {
       const int p = (l.at * V + i) >> 1;
-      const bool pass = ANY && p >= a.n_freq;
-      const float2 cs = table[ANY ? min(p, a.n_freq - 1) : p];
+      const bool pass = WAY != kRopeWhole && p >= a.n_freq;
+      const float2 cs = table[WAY != kRopeWhole ? min(p, a.n_freq - 1) : p];
       t.passing[i] = t.passing[i + 1] = pass;
       t.c[i] = t.c[i + 1] = pass ? 1.0f : cs.x;
       t.s[i] = pass ? 0.0f : -cs.y;
       t.s[i + 1] = pass ? 0.0f : cs.y;
     }
   } else {
-    constexpr int H = ANY ? V / 2 : V;  // values that turn alike
+    if constexpr (WAY == kRopeGather) {
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const int e = l.at * V + i;
+        const bool pass = e >= 2 * a.n_freq, first = e < a.n_freq;
+        const float2 cs = table[pass ? 0 : first ? e : e - a.n_freq];
+        t.passing[i] = pass;
+        t.c[i] = pass ? 1.0f : cs.x;
+        t.s[i] = pass ? 0.0f : first ? -cs.y : cs.y;
+      }
+      return;
+    }
+    constexpr int H = WAY == kRopeWhole ? V : V / 2;  // values that turn alike
 #pragma unroll
     for (int h = 0; h < V / H; ++h) {
       const int at = l.at * V + h * H;
-      const bool pass = ANY && at >= 2 * a.n_freq, first = at < a.n_freq;
+      const bool pass = WAY != kRopeWhole && at >= 2 * a.n_freq, first = at < a.n_freq;
       const float2* from = table + (pass ? 0 : first ? at : at - a.n_freq);
 #pragma unroll
       for (int i = h * H; i < (h + 1) * H; ++i) {
@@ -398,7 +488,7 @@ __device__ __forceinline__ void wave_sums(float (&v)[N], int log2) {
 // Sums of N values over the lanes of each vector, in every lane of it.  `scratch`:
 // N * kRopeScratch floats of the wave's own, used where the lanes are no power of
 // two: there each lane leaves its value and adds up its vector's.
-constexpr int kRopeScratch = 128;
+constexpr int kRopeScratch = 128;  // rope_lds_of
 template <int N>
 __device__ __forceinline__ void vector_sums(const RopeArgs& a, const RopeLane& l, float (&v)[N],
                                             float* scratch) {
@@ -461,7 +551,7 @@ struct RopeOut {
     for (int i = 0; i < V; ++i) r[i] = static_cast<T>(o[i]);
     const int off = there ? at * static_cast<int>(sizeof(T)) : INT_MAX;
     constexpr int N = V * sizeof(T) / 4;
-    constexpr int kAux = MEM == kRopeStream ? 2 : 0;  // nt
+        constexpr int kAux = MEM == kRopeStream ? kCacheNtSc1 : kCacheSc1;
     typedef int words __attribute__((ext_vector_type(N)));
     if constexpr (N == 4)
       __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(words, r), rsrc, off, 0, kAux);
@@ -517,18 +607,6 @@ __device__ __forceinline__ RopePair rope_pair(const RopeArgs& a, const RopeLane&
   r.has_a = l.live && slot < slots;
   r.has_b = r.has_a && r.b < a.dim;
   return r;
-}
-
-// One weight, widened (1 without weights).
-template <typename T>
-__device__ __forceinline__ float load_weight(const RopeArgs& a, const RopeSide& side, int i) {
-  if (side.w == nullptr) return 1.0f;
-  if (a.w_f32) {
-    const float* w = static_cast<const float*>(side.w);
-    return load_any<float, 1, false>(w + i, VBH_SPAN(w, a.dim));
-  }
-  const T* w = static_cast<const T*>(side.w);
-  return static_cast<float>(load_any<T, 1, false>(w + i, VBH_SPAN(w, a.dim)));
 }
 
 template <typename T>

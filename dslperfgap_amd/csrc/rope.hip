@@ -14,21 +14,18 @@
 
 namespace vbh {
 
-#ifndef ZPAD
-#define ZPAD 5 * all(t.accesses) > 4 * all(padded)
-#endif
-#ifndef ZFB
-#define ZFB 6
-#endif
 namespace {
 
 // A wave's share: U passes over one side of token t, from head `head0` on.
-template <typename T, int V, int U, bool NORM, bool ADJ, bool ANY, int MEM>
+template <typename T, int V, int U, bool NORM, bool ADJ, int WAY, int MEM>
 __device__ __forceinline__ void rope_share(const RopeArgs& a, const RopeSide& side,
-                                           const RopeToken& t, int head0, float2* table,
-                                           float* scratch) {
+                                           const RopeToken& t, int head0, float* lds) {
   const RopeLane l = rope_lane(a);
   const Span sx = VBH_SPAN(static_cast<const T*>(side.x), rope_extent(a, side.xs, side.heads));
+  const RopeLds parts = rope_lds_of(a, NORM ? kRopePasses : 0, kRopePasses);
+  float2* table = reinterpret_cast<float2*>(lds);
+  float* scratch = lds + parts.table;
+  char* rows = reinterpret_cast<char*>(scratch + parts.scratch);
   const RopeAngles angles(a);
   const double pos = angles.position(a, t);
   float w[V];
@@ -46,13 +43,13 @@ __device__ __forceinline__ void rope_share(const RopeArgs& a, const RopeSide& si
   }
   angles.make(a, t, pos, table);
   wave_lds_fence();
-  const RopePartner<V> partner = rope_partner<V, ANY>(a, l);
+  const RopePartners<T, V, U, WAY> partners(a, l, x, rows);
   Turn<V> turn;
-  make_turn<V, ADJ, ANY>(a, l, table, turn);
+  make_turn<V, ADJ, WAY>(a, l, table, turn);
   float size[U];
   if constexpr (NORM) {
     float theirs[V];
-    if constexpr (!ADJ) partners<V, ANY>(w, partner, theirs);
+    if constexpr (!ADJ) partner_weights<T, V, WAY>(a, side, l, partners.p, w, theirs);
 #pragma unroll
     for (int i = 0; i < V; ++i) {
       turn.c[i] *= w[i];
@@ -69,28 +66,30 @@ __device__ __forceinline__ void rope_share(const RopeArgs& a, const RopeSide& si
   const int to = (head0 + l.sub) * a.dim + l.at * V, step = a.tile.per_pass * a.dim;
 #pragma unroll
   for (int u = 0; u < U; ++u) {
-    typename Raw<T, V>::type other = x[u];
-    if constexpr (!ADJ) other = partners<T, V, ANY>(x[u], partner);
-    float o[V];
+    float other[V], o[V];
+    if constexpr (!ADJ) partners.get(x[u], u, other);
 #pragma unroll
     for (int i = 0; i < V; ++i) {
       const float xi = raw_at<T, V>(x[u], i);
-      const float xp = raw_at<T, V>(other, ADJ ? i ^ 1 : i);
+      const float xp = ADJ ? raw_at<T, V>(x[u], i ^ 1) : other[i];
       float y = fmaf(xi, turn.c[i], xp * turn.s[i]);
       // a value that passes takes nothing from another, which may be infinite
-      if (ANY && turn.passing[i]) y = xi * turn.c[i];
+      if (WAY != kRopeWhole && turn.passing[i]) y = xi * turn.c[i];
       o[i] = NORM ? y * size[u] : y;
     }
     out.store(to + u * step, ok[u], o);
   }
 }
 
-// 5 waves to a SIMD: up to 96 registers, which 4 passes of 16-bit values use.
-template <typename T, int V, bool NORM, bool ADJ, bool ANY, int MEM>
-__global__ __launch_bounds__(kRopeBlock, ZFB) void rope_rows(const RopeArgs) {
+// 6 waves to a SIMD, 80 registers: norm and rotation of 16384 tokens of 40 bf16 heads of
+// 128 take 53.2 us so, 53.9 at 5 waves, 57.0 at 7 and 74 at 8, where registers spill;
+// of 96, adjacent pairs 45.0 and 50.7 at 5.
+template <typename T, int V, bool NORM, bool ADJ, int WAY, int MEM>
+__global__ __launch_bounds__(kRopeBlock, 6) void rope_rows(const RopeArgs) {
   const RopeArgs& a = launch_args();
   extern __shared__ __align__(16) float rope_lds[];
   const int wave = wave_index();
+  float* lds = rope_lds + wave * rope_lds_of(a, NORM ? kRopePasses : 0, kRopePasses).all();
   const uint32_t chunks = static_cast<uint32_t>(a.q.chunks + a.k.chunks);
   const uint32_t unit = blockIdx.x * static_cast<uint32_t>(kRopeWaves) + wave;
   const uint32_t turn_of = unit / chunks;
@@ -98,20 +97,14 @@ __global__ __launch_bounds__(kRopeBlock, ZFB) void rope_rows(const RopeArgs) {
   if (token >= a.tokens) return;
   const int chunk = static_cast<int>(unit - turn_of * chunks);
   const RopeToken t = rope_token(a, token);
-  const bool is_q = chunk < a.q.chunks;
-  const RopeSide& side = a.side(!is_q);
-  const int head0 =
-      (is_q ? chunk : chunk - a.q.chunks) * side.per_wave * a.tile.per_pass;
-  const int table_floats = rope_table_floats(a.n_freq);
-  const int scratch_floats = NORM && a.tile.lanes_log2 < 0 ? kRopePasses * kRopeScratch : 0;
-  float* mine = rope_lds + wave * (table_floats + scratch_floats);
-  float2* table = reinterpret_cast<float2*>(mine);
-  float* scratch = mine + table_floats;
+  const bool is_k = chunk >= a.q.chunks;
+  const RopeSide& side = a.side(is_k);
+  const int head0 = (is_k ? chunk - a.q.chunks : chunk) * side.per_wave * a.tile.per_pass;
   switch (side.per_wave) {
-    case 1: return rope_share<T, V, 1, NORM, ADJ, ANY, MEM>(a, side, t, head0, table, scratch);
-    case 2: return rope_share<T, V, 2, NORM, ADJ, ANY, MEM>(a, side, t, head0, table, scratch);
-    case 3: return rope_share<T, V, 3, NORM, ADJ, ANY, MEM>(a, side, t, head0, table, scratch);
-    default: return rope_share<T, V, 4, NORM, ADJ, ANY, MEM>(a, side, t, head0, table, scratch);
+    case 1: return rope_share<T, V, 1, NORM, ADJ, WAY, MEM>(a, side, t, head0, lds);
+    case 2: return rope_share<T, V, 2, NORM, ADJ, WAY, MEM>(a, side, t, head0, lds);
+    case 3: return rope_share<T, V, 3, NORM, ADJ, WAY, MEM>(a, side, t, head0, lds);
+    default: return rope_share<T, V, 4, NORM, ADJ, WAY, MEM>(a, side, t, head0, lds);
   }
 }
 
@@ -183,20 +176,16 @@ constexpr int64_t kRopeMaxGrid = ((int64_t(1) << 32) - 1) / kRopeBlock;
 
 void rope_shape(RopeArgs& a, int dt, bool adjacent, bool norm, int64_t few, int most) {
   RopeTile& t = a.tile;
-  // the widest access that fits vectors and, in half accesses that are whole words,
-  // the way to the partners
-  t.v = dt == kF32 ? 4 : 8;
-  auto fits = [&](int v) {
-    const int step = dt == kF32 || v > 2 ? v / 2 : v;
-    return a.dim % v == 0 && (adjacent || a.n_freq % step == 0);
-  };
-  while (t.v > 1 && !fits(t.v)) t.v /= 2;
+  t.v = dt == kF32 ? 4 : 8;  // the widest access that vectors are a whole number of
+  while (t.v > 1 && a.dim % t.v != 0) t.v /= 2;
   t.accesses = a.dim / t.v;
   if (t.v == 1 || t.accesses > kWave) {  // pair by pair
     t.v = 1;
     t.accesses = std::min((a.dim + 1) / 2, kWave);
     most = 1;
   }
+  // half accesses that are whole words find their partners in one lane each
+  a.gather = !adjacent && t.v > 1 && a.n_freq % (dt == kF32 || t.v > 2 ? t.v / 2 : t.v) != 0;
   int padded = 1;
   while (padded < t.accesses) padded *= 2;
   auto passes = [&](const RopeSide& side, int lanes) {
@@ -205,9 +194,10 @@ void rope_shape(RopeArgs& a, int dt, bool adjacent, bool norm, int64_t few, int 
   auto all = [&](int lanes) { return passes(a.q, lanes) + passes(a.k, lanes); };
   // Vectors of no power of two of accesses: side by side without a gap, or a power of
   // two of lanes apart, which leaves lanes idle but sums in registers.  MI355X, 16384
-  // tokens of 32 + 8 bf16 heads, passes and us, side by side / apart: heads of 96,
-  // 9 / 10 passes, norm SIDE96 / APART96; heads of 80, 8 / 10 passes, norm SIDE80 / APART80
-  t.lanes = t.v == 1 || (norm && ZPAD) ||
+  // tokens of 32 + 8 bf16 heads, us side by side / apart: heads of 96 (9 / 10 passes)
+  // forward 53.4 / 49.5, backward 87.0 / 77.6; heads of 80 (8 / 10 passes) 52.2 / 51.7 and
+  // 70.3 / 74.5; heads of 72 (7 / 10) 55.1 / 55.0 and 75.2 / 80.1
+  t.lanes = t.v == 1 || (norm && 5 * all(t.accesses) > 4 * all(padded)) ||
                     all(t.accesses) == all(padded)
                 ? padded
                 : t.accesses;
@@ -236,7 +226,7 @@ hipError_t launch_rope(const RopeArgs& args, int dt, bool adjacent, bool norm, h
   rope_shape(a, dt, adjacent, norm, kRopeFewPasses, kRopePasses);
   const RopeTile& t = a.tile;
   const int chunks = a.q.chunks + a.k.chunks;
-  const bool any = 2 * a.n_freq < a.dim || (!adjacent && a.n_freq % t.v != 0);
+  const bool whole = 2 * a.n_freq == a.dim && (adjacent || a.n_freq % t.v == 0);
   const int64_t bytes =
       a.tokens * (a.q.heads + a.k.heads) * a.dim * (dt == kF32 ? 4 : 2);
   hipError_t err = hipErrorInvalidValue;
@@ -265,14 +255,16 @@ hipError_t launch_rope(const RopeArgs& args, int dt, bool adjacent, bool norm, h
           return;
         }
         const size_t floats =
-            size_t(kRopeWaves) * (rope_table_floats(a.n_freq) +
-                                  (N && t.lanes_log2 < 0 ? kRopePasses * kRopeScratch : 0));
+            size_t(kRopeWaves) * rope_lds_of(a, N ? kRopePasses : 0, kRopePasses).all();
         auto rows = [&](auto mc) {
           constexpr int M = decltype(mc)::value;
-          if (t.v == VN && !any) go(rope_rows<T, VN, N, A, false, M>, floats);
-          else if (t.v == VN) go(rope_rows<T, VN, N, A, true, M>, floats);
-          else if (VN == 8 && t.v == 4) go(rope_rows<T, 4, N, A, true, M>, floats);
-          else go(rope_rows<T, 2, N, A, true, M>, floats);
+          if (t.v == VN && whole) return go(rope_rows<T, VN, N, A, kRopeWhole, M>, floats);
+          dispatch_bool(a.gather != 0, [&](auto gc) {
+            constexpr int W = decltype(gc)::value && !A ? kRopeGather : kRopeHalves;
+            if (t.v == VN) go(rope_rows<T, VN, N, A, W, M>, floats);
+            else if (VN == 8 && t.v == 4) go(rope_rows<T, 4, N, A, W, M>, floats);
+            else go(rope_rows<T, 2, N, A, W, M>, floats);
+          });
         };
         dispatch_rope_mem(rope_mem(bytes, bytes), rows);
       });

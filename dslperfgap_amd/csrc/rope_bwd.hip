@@ -17,13 +17,7 @@ namespace vbh {
 
 namespace {
 
-#ifndef ZGU
-#define ZGU 2
-#endif
-#ifndef ZGW
-#define ZGW 4
-#endif
-constexpr int kGradPasses = ZGU;  // passes of a wave's share, at most
+constexpr int kGradPasses = 2;  // passes of a wave's share, at most
 
 // Workgroups that have queries' waves and that have keys' (one may have both), and
 // the first of the latter.
@@ -77,13 +71,16 @@ __device__ __forceinline__ void write_part(const RopeArgs& a, const float* sums,
 }
 
 // The wave's share of its tokens, U passes each; dw: the lane's sums.
-template <typename T, int V, int U, bool ADJ, bool ANY, int MEM>
+template <typename T, int V, int U, bool ADJ, int WAY, int MEM>
 __device__ __forceinline__ void grad_share(const RopeArgs& a, const RopeSide& side,
                                            const RopeLane& l, int chunk, int first,
-                                           float2* table, float* scratch, float (&dw)[V]) {
+                                           float* lds, float (&dw)[V]) {
+  const RopeLds parts = rope_lds_of(a, 2 * kGradPasses, kGradPasses);
+  float2* table = reinterpret_cast<float2*>(lds);
+  float* scratch = lds + parts.table;
+  char* rows = reinterpret_cast<char*>(scratch + parts.scratch);
   const Span sx = VBH_SPAN(static_cast<const T*>(side.x), rope_extent(a, side.xs, side.heads));
   const Span sg = VBH_SPAN(static_cast<const T*>(side.g), rope_extent(a, side.gs, side.heads));
-  const RopePartner<V> partner = rope_partner<V, ANY>(a, l);
   const float inv_dim = 1.0f / static_cast<float>(a.dim);
   const int head0 = chunk * U * a.tile.per_pass;
   float w[V];
@@ -121,7 +118,8 @@ __device__ __forceinline__ void grad_share(const RopeArgs& a, const RopeSide& si
     angles.make(a, t, pos, table);
     wave_lds_fence();
     Turn<V> turn;
-    make_turn<V, ADJ, ANY>(a, l, table, turn);
+    make_turn<V, ADJ, WAY>(a, l, table, turn);
+    const RopePartners<T, V, U, WAY> partners(a, l, g, rows);
     const RopeOut<T, V, MEM> out(a, side, t.t);
     auto finish = [&](int u, const float (&dn)[V], float s0, float s1) {
       // lanes without a vector add nothing to the sums
@@ -137,16 +135,16 @@ __device__ __forceinline__ void grad_share(const RopeArgs& a, const RopeSide& si
       out.store(to + u * y_step, ok[u], o);
     };
     auto begin = [&](int u, float (&dn)[V], float& s0, float& s1) {
-      R other = g[u];
-      if constexpr (!ADJ) other = partners<T, V, ANY>(g[u], partner);
+      float other[V];
+      if constexpr (!ADJ) partners.get(g[u], u, other);
       s0 = squares<T, V>(x[u]);
       s1 = 0.0f;
 #pragma unroll
       for (int i = 0; i < V; ++i) {
         const float gi = raw_at<T, V>(g[u], i);
-        const float gp = raw_at<T, V>(other, ADJ ? i ^ 1 : i);
+        const float gp = ADJ ? raw_at<T, V>(g[u], i ^ 1) : other[i];
         float n = fmaf(gi, turn.c[i], gp * turn.s[i]);
-        if (ANY && turn.passing[i]) n = gi;
+        if (WAY != kRopeWhole && turn.passing[i]) n = gi;
         dn[i] = n;
         s1 = fmaf(n * w[i], raw_at<T, V>(x[u], i), s1);
       }
@@ -160,8 +158,8 @@ __device__ __forceinline__ void grad_share(const RopeArgs& a, const RopeSide& si
   }
 }
 
-template <typename T, int V, bool ADJ, bool ANY, int MEM>
-__global__ __launch_bounds__(kRopeBlock, ZGW) void qk_norm_rope_grads(const RopeArgs,
+template <typename T, int V, bool ADJ, int WAY, int MEM>
+__global__ __launch_bounds__(kRopeBlock, 4) void qk_norm_rope_grads(const RopeArgs,
                                                                     float* parts) {
   const RopeArgs& a = launch_args();
   extern __shared__ __align__(16) float rope_lds[];
@@ -169,20 +167,15 @@ __global__ __launch_bounds__(kRopeBlock, ZGW) void qk_norm_rope_grads(const Rope
   const RopeWalk walk = rope_walk(a, wave);
   const RopeLane l = rope_lane(a);
   const RopeSide& side = a.side(!walk.is_q);
-  const int table_floats = rope_table_floats(a.n_freq);
-  const int scratch_floats = a.tile.lanes_log2 < 0 ? 2 * kGradPasses * kRopeScratch : 0;
-  float* mine = rope_lds + wave * (table_floats + scratch_floats);
-  float2* table = reinterpret_cast<float2*>(mine);
-  float* scratch = mine + table_floats;
+  float* lds = rope_lds + wave * rope_lds_of(a, 2 * kGradPasses, kGradPasses).all();
   float dw[V];
 #pragma unroll
   for (int i = 0; i < V; ++i) dw[i] = 0.0f;
   if (walk.live) {
     if (side.per_wave == 1)
-      grad_share<T, V, 1, ADJ, ANY, MEM>(a, side, l, walk.chunk, walk.token, table, scratch, dw);
+      grad_share<T, V, 1, ADJ, WAY, MEM>(a, side, l, walk.chunk, walk.token, lds, dw);
     else
-      grad_share<T, V, kGradPasses, ADJ, ANY, MEM>(a, side, l, walk.chunk, walk.token, table,
-                                                    scratch, dw);
+      grad_share<T, V, kGradPasses, ADJ, WAY, MEM>(a, side, l, walk.chunk, walk.token, lds, dw);
   }
   if (parts == nullptr) return;
   __syncthreads();
@@ -298,17 +291,33 @@ __global__ __launch_bounds__(kSumWaves* kWave) void qk_weight_grads(const float*
   const int rows = is_q ? q_rows : k_rows;
   const float* from = parts + static_cast<int64_t>(is_q ? 0 : q_rows) * dim;
   float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll 4
-  for (int r = wave * 16 + lane % 16; r < rows; r += kSumLines) {
-    const float* row = from + static_cast<int64_t>(r) * dim;
-    if (dim % 4 == 0 && d < dim) {
-      const typename Raw<float, 4>::type x = load_any<float, 4, false>(row + d, sp);
+  for (int r = wave * 16 + lane % 16; r < rows; r += 4 * kSumLines) {
+    // four rows' loads in flight; rows behind the last are the first of them again
+    const float* row[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) v[i] += x[i];
-    } else {
+    for (int j = 0; j < 4; ++j) {
+      const int rr = r + j * kSumLines;
+      row[j] = from + static_cast<int64_t>(rr < rows ? rr : r) * dim + d;
+    }
+    float x[4][4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (d + i < dim) v[i] += load_any<float, 1, false>(row + d + i, sp);
+    for (int j = 0; j < 4; ++j) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[j][i] = 0.0f;
+      if (dim % 4 == 0 && d < dim) {
+        const typename Raw<float, 4>::type y = load_any<float, 4, false>(row[j], sp);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[j][i] = y[i];
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (d + i < dim) x[j][i] = load_any<float, 1, false>(row[j] + i, sp);
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] += r + j * kSumLines < rows ? x[j][i] : 0.0f;
     }
   }
   wave_sums<4>(v, 4);
@@ -361,7 +370,7 @@ hipError_t launch_qk_norm_rope_bwd(const RopeArgs& args, int dt, bool adjacent, 
   grad_shape(a, dt, adjacent);
   const RopeTile& t = a.tile;
   const RopeRows rows = rope_rows_of(a);
-  const bool any = 2 * a.n_freq < a.dim || (!adjacent && a.n_freq % t.v != 0);
+  const bool whole = 2 * a.n_freq == a.dim && (adjacent || a.n_freq % t.v == 0);
   const bool sums = dq_weight != nullptr || dk_weight != nullptr;
   const int64_t bytes =
       a.tokens * (a.q.heads + a.k.heads) * a.dim * (dt == kF32 ? 4 : 2);
@@ -387,14 +396,16 @@ hipError_t launch_qk_norm_rope_bwd(const RopeArgs& args, int dt, bool adjacent, 
           return;
         }
         const size_t floats =
-            size_t(kRopeWaves) * (rope_table_floats(a.n_freq) +
-                                  (t.lanes_log2 < 0 ? 2 * kGradPasses * kRopeScratch : 0));
+            size_t(kRopeWaves) * rope_lds_of(a, 2 * kGradPasses, kGradPasses).all();
         auto grads = [&](auto mc) {
           constexpr int M = decltype(mc)::value;
-          if (t.v == VN && !any) go(qk_norm_rope_grads<T, VN, A, false, M>, floats);
-          else if (t.v == VN) go(qk_norm_rope_grads<T, VN, A, true, M>, floats);
-          else if (VN == 8 && t.v == 4) go(qk_norm_rope_grads<T, 4, A, true, M>, floats);
-          else go(qk_norm_rope_grads<T, 2, A, true, M>, floats);
+          if (t.v == VN && whole) return go(qk_norm_rope_grads<T, VN, A, kRopeWhole, M>, floats);
+          dispatch_bool(a.gather != 0, [&](auto gc) {
+            constexpr int W = decltype(gc)::value && !A ? kRopeGather : kRopeHalves;
+            if (t.v == VN) go(qk_norm_rope_grads<T, VN, A, W, M>, floats);
+            else if (VN == 8 && t.v == 4) go(qk_norm_rope_grads<T, 4, A, W, M>, floats);
+            else go(qk_norm_rope_grads<T, 2, A, W, M>, floats);
+          });
         };
         dispatch_rope_mem(rope_mem(2 * bytes, bytes), grads);
       });

@@ -354,6 +354,7 @@ struct RopeArgs {
   float eps = 0.0f;
   // set by the launcher
   RopeTile tile;
+  int gather = 0;                     // partners through the LDS (rope.h)
   int64_t first = 0;                  // token that the launch begins with
 };
 hipError_t launch_rope(const RopeArgs& a, int dt, bool adjacent, bool norm, hipStream_t s);

@@ -97,7 +97,8 @@ def _check(lead=(2, 37), hq=4, hk=2, dim=64, n=None, dtype=F32, wdtype=None, pai
 # nothing (80, 96, 192), value by value along a wave (250, 510, 1023), partial rotation
 SIZES = [(2, 1), (3, 1), (8, 4), (16, 8), (20, 10), (33, 16), (64, 32), (65, 32), (72, 36),
          (80, 40), (80, 10), (96, 48), (100, 50), (128, 64), (128, 32), (128, 3), (192, 96),
-         (250, 125), (256, 128), (510, 255), (512, 256), (1023, 511), (1024, 512), (1024, 100)]
+         (250, 125), (256, 128),
+         (50, 25), (66, 33), (24, 6), (120, 15), (104, 52), (36, 7), (42, 10), (126, 63), (510, 255), (512, 256), (1023, 511), (1024, 512), (1024, 100)]
 
 
 @pytest.mark.parametrize("pairing", ["half", "adjacent"])
