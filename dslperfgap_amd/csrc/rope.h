@@ -75,7 +75,7 @@ struct RopeLds {
 };
 __host__ __device__ inline RopeLds rope_lds_of(const RopeArgs& a, int sums, int passes) {
   RopeLds r;
-  r.table = (2 * a.n_freq + 3) & ~3;
+  r.table = (2 * a.n_freq + 15) & ~15;  // table_place stays in runs of 8 pairs
   r.scratch = a.tile.lanes_log2 < 0 ? sums * 128 : 0;
   r.rows = a.gather ? passes * (kWave * 16 / 4) : 0;
   return r;
@@ -200,6 +200,34 @@ __device__ __forceinline__ int64_t token_offset(const RopeToken& t, const int64_
   return t.b * st[0] + t.s * st[1];
 }
 
+// Place of pair p in a wave's table of float2, p and p + 1 side by side for even p.
+// Lanes read whole runs of pairs, 64 bytes apart at 8 each; the exchange of 16-byte
+// words within 64 bytes, another in each 256, lets 16 of them read at once without
+// bank conflicts.
+__device__ __forceinline__ int table_place(int p) {
+  const int word = p >> 1;
+  return ((word ^ ((word >> 4) & 3)) << 1) | (p & 1);
+}
+// N pairs from p on (even where N is).
+template <int N>
+__device__ __forceinline__ void read_turns(const float2* table, int p, float (&c)[N],
+                                           float (&s)[N]) {
+  if constexpr (N == 1) {
+    const float2 v = table[table_place(p)];
+    c[0] = v.x;
+    s[0] = v.y;
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; i += 2) {
+      const float4 v = *reinterpret_cast<const float4*>(table + table_place(p + i));
+      c[i] = v.x;
+      s[i] = v.y;
+      c[i + 1] = v.z;
+      s[i + 1] = v.w;
+    }
+  }
+}
+
 // (cos, sin) * scale of pairs lane, lane + 64, ... of a token, one lane each, into
 // the wave's table.  What the first of them needs of memory is loaded by itself, so
 // that a wave that walks over tokens may ask for it ahead of its other loads, which
@@ -223,7 +251,7 @@ struct RopeAngles {
     float2 cs = cos_sin_turns(f - __builtin_rint(f));
     cs.x *= a.scale;
     cs.y *= a.sin_scale;
-    table[p] = cs;
+    table[table_place(p)] = cs;
   }
   __device__ __forceinline__ void make(const RopeArgs& a, const RopeToken& t, double pos,
                                        float2* table) const {
@@ -407,41 +435,43 @@ template <int V, bool ADJ, int WAY>
 __device__ __forceinline__ void make_turn(const RopeArgs& a, const RopeLane& l,
                                           const float2* table, Turn<V>& t) {
   if constexpr (ADJ) {
+    constexpr int N = V / 2;
+    const int p0 = l.at * N;
+    float c[N], si[N];
+    // a run whose first pair passes reads another; n_freq may end inside a run, whose
+    // rest lies in the table's last places, unwritten and unused
+    read_turns<N>(table, WAY != kRopeWhole && p0 >= a.n_freq ? 0 : p0, c, si);
 #pragma unroll
-    for (int i = 0; i < V; i += 2) {
-      const int p = (l.at * V + i) >> 1;
-      const bool pass = WAY != kRopeWhole && p >= a.n_freq;
-      const float2 cs = table[WAY != kRopeWhole ? min(p, a.n_freq - 1) : p];
-      t.passing[i] = t.passing[i + 1] = pass;
-      t.c[i] = t.c[i + 1] = pass ? 1.0f : cs.x;
-      t.s[i] = pass ? 0.0f : -cs.y;
-      t.s[i + 1] = pass ? 0.0f : cs.y;
+    for (int i = 0; i < N; ++i) {
+      const bool pass = WAY != kRopeWhole && p0 + i >= a.n_freq;
+      t.passing[2 * i] = t.passing[2 * i + 1] = pass;
+      t.c[2 * i] = t.c[2 * i + 1] = pass ? 1.0f : c[i];
+      t.s[2 * i] = pass ? 0.0f : -si[i];
+      t.s[2 * i + 1] = pass ? 0.0f : si[i];
+    }
+  } else if constexpr (WAY == kRopeGather) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const int e = l.at * V + i;
+      const bool pass = e >= 2 * a.n_freq, first = e < a.n_freq;
+      const float2 cs = table[table_place(pass ? 0 : first ? e : e - a.n_freq)];
+      t.passing[i] = pass;
+      t.c[i] = pass ? 1.0f : cs.x;
+      t.s[i] = pass ? 0.0f : first ? -cs.y : cs.y;
     }
   } else {
-    if constexpr (WAY == kRopeGather) {
-#pragma unroll
-      for (int i = 0; i < V; ++i) {
-        const int e = l.at * V + i;
-        const bool pass = e >= 2 * a.n_freq, first = e < a.n_freq;
-        const float2 cs = table[pass ? 0 : first ? e : e - a.n_freq];
-        t.passing[i] = pass;
-        t.c[i] = pass ? 1.0f : cs.x;
-        t.s[i] = pass ? 0.0f : first ? -cs.y : cs.y;
-      }
-      return;
-    }
     constexpr int H = WAY == kRopeWhole ? V : V / 2;  // values that turn alike
 #pragma unroll
     for (int h = 0; h < V / H; ++h) {
       const int at = l.at * V + h * H;
       const bool pass = WAY != kRopeWhole && at >= 2 * a.n_freq, first = at < a.n_freq;
-      const float2* from = table + (pass ? 0 : first ? at : at - a.n_freq);
+      float c[H], si[H];
+      read_turns<H>(table, pass ? 0 : first ? at : at - a.n_freq, c, si);
 #pragma unroll
-      for (int i = h * H; i < (h + 1) * H; ++i) {
-        const float2 cs = from[i - h * H];
-        t.passing[i] = pass;
-        t.c[i] = pass ? 1.0f : cs.x;
-        t.s[i] = pass ? 0.0f : first ? -cs.y : cs.y;
+      for (int i = 0; i < H; ++i) {
+        t.passing[h * H + i] = pass;
+        t.c[h * H + i] = pass ? 1.0f : c[i];
+        t.s[h * H + i] = pass ? 0.0f : first ? -si[i] : si[i];
       }
     }
   }

@@ -113,7 +113,8 @@ template <typename T, int K, bool NORM, bool ADJ>
 __global__ __launch_bounds__(kRopeBlock) void rope_values(const RopeArgs a) {
   extern __shared__ __align__(16) float rope_lds[];
   const int wave = wave_index();
-  float2* table = reinterpret_cast<float2*>(rope_lds) + wave * a.n_freq;
+  float2* table =
+      reinterpret_cast<float2*>(rope_lds + wave * rope_lds_of(a, 0, 0).table);
   const uint32_t chunks = static_cast<uint32_t>(a.q.chunks + a.k.chunks);
   const uint32_t unit = blockIdx.x * static_cast<uint32_t>(kRopeWaves) + wave;
   const uint32_t turn_of = unit / chunks;
@@ -158,7 +159,7 @@ __global__ __launch_bounds__(kRopeBlock) void rope_values(const RopeArgs a) {
     }
     float ya = na, yb = nb;
     if (r.p >= 0) {
-      const float2 cs = table[r.p];
+      const float2 cs = table[table_place(r.p)];
       ya = fmaf(na, cs.x, -nb * cs.y);
       yb = fmaf(nb, cs.x, na * cs.y);
     }
@@ -174,15 +175,17 @@ constexpr int64_t kRopeMaxGrid = ((int64_t(1) << 32) - 1) / kRopeBlock;
 
 }  // namespace
 
-void rope_shape(RopeArgs& a, int dt, bool adjacent, bool norm, int64_t few, int most) {
+void rope_shape(RopeArgs& a, int dt, bool adjacent, bool norm, int64_t many, int least,
+                int most, bool even) {
   RopeTile& t = a.tile;
-  t.v = dt == kF32 ? 4 : 8;  // the widest access that vectors are a whole number of
+  const int elt = dt == kF32 ? 4 : 2;
+  t.v = 16 / elt;  // the widest access that vectors are a whole number of
   while (t.v > 1 && a.dim % t.v != 0) t.v /= 2;
   t.accesses = a.dim / t.v;
   if (t.v == 1 || t.accesses > kWave) {  // pair by pair
     t.v = 1;
     t.accesses = std::min((a.dim + 1) / 2, kWave);
-    most = 1;
+    least = most = 1;
   }
   // half accesses that are whole words find their partners in one lane each
   a.gather = !adjacent && t.v > 1 && a.n_freq % (dt == kF32 || t.v > 2 ? t.v / 2 : t.v) != 0;
@@ -204,12 +207,17 @@ void rope_shape(RopeArgs& a, int dt, bool adjacent, bool norm, int64_t few, int 
   t.lanes_log2 = (t.lanes & (t.lanes - 1)) == 0 ? __builtin_ctz(t.lanes) : -1;
   t.per_pass = kWave / t.lanes;
   const int pq = passes(a.q, t.lanes), pk = passes(a.k, t.lanes);
-  if (a.tokens * (pq + pk) < few) most = 1;
+  const int64_t total = a.tokens * (pq + pk);
+  if (a.n_freq <= kWave && t.lanes_log2 >= 0 && t.lanes == t.accesses && t.v * elt == 16)
+    most = std::min(most, 4);
+  most = total < many
+             ? 1
+             : static_cast<int>(std::min<int64_t>(most, std::max<int64_t>(total / many, least)));
   auto share = [&](RopeSide& side, int n) {
-    // the fewest passes with a wave's own work (angles and the like) taken for two;
-    // the larger share of two alike
+    // the fewest passes with a wave's own work (angles and the like) taken for two; the
+    // larger share of two alike
     int best = 1 << 30;
-    for (int u = 1; u <= most; ++u) {
+    for (int u = 1; u <= most; u += even && u > 1 ? 2 : 1) {
       const int chunks = (n + u - 1) / u;
       if (chunks * (u + 2) > best) continue;
       best = chunks * (u + 2);
@@ -223,7 +231,7 @@ void rope_shape(RopeArgs& a, int dt, bool adjacent, bool norm, int64_t few, int 
 
 hipError_t launch_rope(const RopeArgs& args, int dt, bool adjacent, bool norm, hipStream_t s) {
   RopeArgs a = args;
-  rope_shape(a, dt, adjacent, norm, kRopeFewPasses, kRopePasses);
+  rope_shape(a, dt, adjacent, norm, kRopeFewPasses, kRopePasses, kRopePasses, false);
   const RopeTile& t = a.tile;
   const int chunks = a.q.chunks + a.k.chunks;
   const bool whole = 2 * a.n_freq == a.dim && (adjacent || a.n_freq % t.v == 0);
@@ -249,7 +257,7 @@ hipError_t launch_rope(const RopeArgs& args, int dt, bool adjacent, bool norm, h
       dispatch_bool(adjacent, [&](auto ac) {
         constexpr bool A = decltype(ac)::value;
         if (t.v == 1) {
-          const size_t floats = size_t(2) * kRopeWaves * a.n_freq;
+          const size_t floats = size_t(kRopeWaves) * rope_lds_of(a, 0, 0).table;
           if ((a.dim + 1) / 2 <= kWave) go(rope_values<T, 1, N, A>, floats);
           else go(rope_values<T, kRopePairs, N, A>, floats);
           return;

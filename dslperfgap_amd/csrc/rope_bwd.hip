@@ -17,7 +17,7 @@ namespace vbh {
 
 namespace {
 
-constexpr int kGradPasses = 2;  // passes of a wave's share, at most
+constexpr int kGradPasses = 2;  // that a wave has in registers at a time
 
 // Workgroups that have queries' waves and that have keys' (one may have both), and
 // the first of the latter.
@@ -70,8 +70,9 @@ __device__ __forceinline__ void write_part(const RopeArgs& a, const float* sums,
   }
 }
 
-// The wave's share of its tokens, U passes each; dw: the lane's sums.
-template <typename T, int V, int U, bool ADJ, int WAY, int MEM>
+// The wave's share of its tokens, U passes at a time (MORE: more than once); dw: the
+// lane's sums.
+template <typename T, int V, int U, bool MORE, bool ADJ, int WAY, int MEM>
 __device__ __forceinline__ void grad_share(const RopeArgs& a, const RopeSide& side,
                                            const RopeLane& l, int chunk, int first,
                                            float* lds, float (&dw)[V]) {
@@ -82,7 +83,7 @@ __device__ __forceinline__ void grad_share(const RopeArgs& a, const RopeSide& si
   const Span sx = VBH_SPAN(static_cast<const T*>(side.x), rope_extent(a, side.xs, side.heads));
   const Span sg = VBH_SPAN(static_cast<const T*>(side.g), rope_extent(a, side.gs, side.heads));
   const float inv_dim = 1.0f / static_cast<float>(a.dim);
-  const int head0 = chunk * U * a.tile.per_pass;
+  const int head0 = chunk * (MORE ? side.per_wave : U) * a.tile.per_pass;
   float w[V];
   load_weights<T, V>(a, side, l, w);
   const T* x0 = static_cast<const T*>(side.x);
@@ -91,70 +92,69 @@ __device__ __forceinline__ void grad_share(const RopeArgs& a, const RopeSide& si
   const int64_t lane_g = (head0 + l.sub) * side.gs[2] + l.at * V;
   const int64_t x_step = a.tile.per_pass * side.xs[2], g_step = a.tile.per_pass * side.gs[2];
   const int to = (head0 + l.sub) * a.dim + l.at * V, y_step = a.tile.per_pass * a.dim;
-  bool ok[U];
-#pragma unroll
-  for (int u = 0; u < U; ++u)
-    ok[u] = l.live && head0 + u * a.tile.per_pass + l.sub < side.heads;
-
-  typedef typename Raw<T, V>::type R;
-  auto load = [&](const RopeToken& t, R(&g)[U], R(&x)[U]) {
-    const T* from_x = x0 + token_offset(t, side.xs) + lane_x;
-    const T* from_g = g0 + token_offset(t, side.gs) + lane_g;
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      // lanes without a vector read their values of the first: no branch keeps the
-      // loads apart
-      g[u] = load_any<T, V, MEM != kRopeCached>(ok[u] ? from_g + u * g_step : g0 + l.at * V, sg);
-      x[u] = load_any<T, V, MEM != kRopeCached>(ok[u] ? from_x + u * x_step : x0 + l.at * V, sx);
-    }
-  };
   const RopeAngles angles(a);
+
   for (int64_t token = first; token < a.tokens; token += side.walkers) {
     const RopeToken t = rope_token(a, token);
     const double pos = angles.position(a, t);
-    R x[U], g[U];
-    load(t, g, x);
-    wave_lds_fence();
-    angles.make(a, t, pos, table);
-    wave_lds_fence();
-    Turn<V> turn;
-    make_turn<V, ADJ, WAY>(a, l, table, turn);
-    const RopePartners<T, V, U, WAY> partners(a, l, g, rows);
+    const T* from_x = x0 + token_offset(t, side.xs) + lane_x;
+    const T* from_g = g0 + token_offset(t, side.gs) + lane_g;
     const RopeOut<T, V, MEM> out(a, side, t.t);
-    auto finish = [&](int u, const float (&dn)[V], float s0, float s1) {
-      // lanes without a vector add nothing to the sums
-      const float r = ok[u] ? inverse_root(fmaf(s0, inv_dim, a.eps)) : 0.0f;
-      const float mean = s1 * r * inv_dim * r;
-      float o[V];
+    Turn<V> turn;
+    // the share's passes, U at a time
+    for (int pass = 0; pass < (MORE ? side.per_wave : U); pass += U) {
+      typename Raw<T, V>::type x[U], g[U];
+      bool ok[U];
 #pragma unroll
-      for (int i = 0; i < V; ++i) {
-        const float unit = raw_at<T, V>(x[u], i) * r;
-        dw[i] = fmaf(dn[i], unit, dw[i]);
-        o[i] = fmaf(dn[i] * r, w[i], -unit * mean);
+      for (int u = 0; u < U; ++u) {
+        // lanes without a vector read their values of the first: no branch keeps the
+        // loads apart
+        ok[u] = l.live && head0 + (pass + u) * a.tile.per_pass + l.sub < side.heads;
+        g[u] = load_any<T, V, MEM != kRopeCached>(
+            ok[u] ? from_g + (pass + u) * g_step : g0 + l.at * V, sg);
+        x[u] = load_any<T, V, MEM != kRopeCached>(
+            ok[u] ? from_x + (pass + u) * x_step : x0 + l.at * V, sx);
       }
-      out.store(to + u * y_step, ok[u], o);
-    };
-    auto begin = [&](int u, float (&dn)[V], float& s0, float& s1) {
-      float other[V];
-      if constexpr (!ADJ) partners.get(g[u], u, other);
-      s0 = squares<T, V>(x[u]);
-      s1 = 0.0f;
-#pragma unroll
-      for (int i = 0; i < V; ++i) {
-        const float gi = raw_at<T, V>(g[u], i);
-        const float gp = ADJ ? raw_at<T, V>(g[u], i ^ 1) : other[i];
-        float n = fmaf(gi, turn.c[i], gp * turn.s[i]);
-        if (WAY != kRopeWhole && turn.passing[i]) n = gi;
-        dn[i] = n;
-        s1 = fmaf(n * w[i], raw_at<T, V>(x[u], i), s1);
+      if (pass == 0) {
+        wave_lds_fence();
+        angles.make(a, t, pos, table);
+        wave_lds_fence();
+        make_turn<V, ADJ, WAY>(a, l, table, turn);
       }
-    };
-    float dn[U][V], sums[2 * U];
+      const RopePartners<T, V, U, WAY> partners(a, l, g, rows);
+      float dn[U][V], sums[2 * U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) begin(u, dn[u], sums[2 * u], sums[2 * u + 1]);
-    vector_sums<2 * U>(a, l, sums, scratch);
+      for (int u = 0; u < U; ++u) {
+        float other[V], dot = 0.0f;
+        if constexpr (!ADJ) partners.get(g[u], u, other);
 #pragma unroll
-    for (int u = 0; u < U; ++u) finish(u, dn[u], sums[2 * u], sums[2 * u + 1]);
+        for (int i = 0; i < V; ++i) {
+          const float gi = raw_at<T, V>(g[u], i);
+          const float gp = ADJ ? raw_at<T, V>(g[u], i ^ 1) : other[i];
+          float n = fmaf(gi, turn.c[i], gp * turn.s[i]);
+          if (WAY != kRopeWhole && turn.passing[i]) n = gi;
+          dn[u][i] = n;
+          dot = fmaf(n * w[i], raw_at<T, V>(x[u], i), dot);
+        }
+        sums[2 * u] = squares<T, V>(x[u]);
+        sums[2 * u + 1] = dot;
+      }
+      vector_sums<2 * U>(a, l, sums, scratch);
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        // lanes without a vector add nothing to the sums
+        const float r = ok[u] ? inverse_root(fmaf(sums[2 * u], inv_dim, a.eps)) : 0.0f;
+        const float mean = sums[2 * u + 1] * r * inv_dim * r;
+        float o[V];
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          const float unit = raw_at<T, V>(x[u], i) * r;
+          dw[i] = fmaf(dn[u][i], unit, dw[i]);
+          o[i] = fmaf(dn[u][i] * r, w[i], -unit * mean);
+        }
+        out.store(to + (pass + u) * y_step, ok[u], o);
+      }
+    }
   }
 }
 
@@ -173,9 +173,13 @@ __global__ __launch_bounds__(kRopeBlock, 4) void qk_norm_rope_grads(const RopeAr
   for (int i = 0; i < V; ++i) dw[i] = 0.0f;
   if (walk.live) {
     if (side.per_wave == 1)
-      grad_share<T, V, 1, ADJ, WAY, MEM>(a, side, l, walk.chunk, walk.token, lds, dw);
+      grad_share<T, V, 1, false, ADJ, WAY, MEM>(a, side, l, walk.chunk, walk.token, lds, dw);
+    else if (side.per_wave == kGradPasses)
+      grad_share<T, V, kGradPasses, false, ADJ, WAY, MEM>(a, side, l, walk.chunk, walk.token,
+                                                          lds, dw);
     else
-      grad_share<T, V, kGradPasses, ADJ, WAY, MEM>(a, side, l, walk.chunk, walk.token, lds, dw);
+      grad_share<T, V, kGradPasses, true, ADJ, WAY, MEM>(a, side, l, walk.chunk, walk.token,
+                                                         lds, dw);
   }
   if (parts == nullptr) return;
   __syncthreads();
@@ -194,7 +198,8 @@ __global__ __launch_bounds__(kRopeBlock) void qk_norm_rope_value_grads(const Rop
                                                                        float* parts) {
   extern __shared__ __align__(16) float rope_lds[];
   const int wave = wave_index();
-  float2* table = reinterpret_cast<float2*>(rope_lds) + wave * a.n_freq;
+  float2* table =
+      reinterpret_cast<float2*>(rope_lds + wave * rope_lds_of(a, 0, 0).table);
   const RopeLane l = rope_lane(a);
   const float inv_dim = 1.0f / static_cast<float>(a.dim);
   float dw[2 * K];
@@ -228,7 +233,7 @@ __global__ __launch_bounds__(kRopeBlock) void qk_norm_rope_value_grads(const Rop
       na[k] = load_value<T>(g + r.a, has_a, sg);
       nb[k] = load_value<T>(g + r.b, has_b, sg);
       if (has_a && r.p >= 0) {
-        const float2 cs = table[r.p];
+        const float2 cs = table[table_place(r.p)];
         const float ga = na[k], gb = nb[k];
         na[k] = fmaf(ga, cs.x, -gb * cs.y);
         nb[k] = fmaf(gb, cs.x, ga * cs.y);
@@ -334,15 +339,20 @@ __global__ __launch_bounds__(kSumWaves* kWave) void qk_weight_grads(const float*
   store_any<W, 1, false>(out + to, &sum, so);
 }
 
-// Waves of a launch: as many as the card holds at once; below some times as many
-// passes a wave takes one at a time.
+// Waves of a launch: as many as the card holds at once; passes beyond which a wave takes
+// more than one of a token's, whose angles it then makes once.  Up to 4 of them where a
+// token's angles take one round of the lanes and vectors lie over a power of two of them
+// without a gap, 8 otherwise.  MI355X, 16384 tokens of 40 bf16 heads, us at 2 / 4 / 8: of
+// 128 87.4 / 87.1 / 87.6 (65536 tokens 371 / 367 / 378), 192 94 / 85 / 79, 256 104 / 92 / 91,
+// 100 113 / 109 / 99, 50 97 / 97 / 85, 96 75.6 / 73.9 / 71.8.
 constexpr int64_t kGradWaves = 4096;
-constexpr int64_t kGradFewPasses = 4 * kGradWaves;
+constexpr int64_t kGradMany = 4 * kGradWaves;
+constexpr int kGradShare = 8;
 
 // rope_shape, and the walkers of each side: waves in proportion to its work, no more
 // than it has tokens, and none that would only share the last turn of the others.
 void grad_shape(RopeArgs& a, int dt, bool adjacent) {
-  rope_shape(a, dt, adjacent, true, kGradFewPasses, kGradPasses);
+  rope_shape(a, dt, adjacent, true, kGradMany, kGradPasses, kGradShare, true);
   auto work = [&](const RopeSide& s) { return int64_t(s.chunks) * (s.per_wave + 2); };
   const int64_t all = work(a.q) + work(a.k);
   for (RopeSide* s : {&a.q, &a.k}) {
@@ -390,7 +400,7 @@ hipError_t launch_qk_norm_rope_bwd(const RopeArgs& args, int dt, bool adjacent, 
       dispatch_bool(adjacent, [&](auto ac) {
         constexpr bool A = decltype(ac)::value;
         if (t.v == 1) {
-          const size_t floats = size_t(2) * kRopeWaves * a.n_freq;
+          const size_t floats = size_t(kRopeWaves) * rope_lds_of(a, 0, 0).table;
           if ((a.dim + 1) / 2 <= kWave) go(qk_norm_rope_value_grads<T, 1, A>, floats);
           else go(qk_norm_rope_value_grads<T, kRopePairs, A>, floats);
           return;

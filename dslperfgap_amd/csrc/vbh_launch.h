@@ -358,9 +358,12 @@ struct RopeArgs {
   int64_t first = 0;                  // token that the launch begins with
 };
 hipError_t launch_rope(const RopeArgs& a, int dt, bool adjacent, bool norm, hipStream_t s);
-// Fills a.tile and the sides' per_wave and chunks; norm: vectors are summed over;
-// few: launches below this many passes give a wave one, most: a wave's at most.
-void rope_shape(RopeArgs& a, int dt, bool adjacent, bool norm, int64_t few, int most);
+// Fills a.tile and the sides' per_wave and chunks.  norm: vectors are summed over.  In
+// launches of fewer passes than `many` a wave takes one of a token's, in others up to
+// `least`, or as many as leave `many` shares, at most `most`; even: one or an even
+// number.
+void rope_shape(RopeArgs& a, int dt, bool adjacent, bool norm, int64_t many, int least, int most,
+                bool even);
 // The norm's backward.  With the weights' gradients wanted (dq_weight, dk_weight
 // not null) `parts` holds rope_bwd_part_floats(a, dt, adjacent) floats.
 int64_t rope_bwd_part_floats(const RopeArgs& a, int dt, bool adjacent);
