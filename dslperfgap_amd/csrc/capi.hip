@@ -1588,8 +1588,8 @@ static int rope_args(const vbh_rope_desc* d, const char* what, bool norm, bool g
   a->w_f32 = d->w_dtype == kF32;
   a->scale = a->sin_scale = d->scale;
   a->eps = d->eps;
-  a->q.heads = static_cast<int>(d->q_heads);
-  a->k.heads = static_cast<int>(d->k_heads);
+  a->q().heads = static_cast<int>(d->q_heads);
+  a->k().heads = static_cast<int>(d->k_heads);
   // strides; tokens lie one stride apart where both dims of every operand allow it,
   // so that no kernel divides by seq
   bool flat = d->batch == 1 || d->seq == 1;
@@ -1607,11 +1607,11 @@ static int rope_args(const vbh_rope_desc* d, const char* what, bool norm, bool g
     if (extent >= kRopeMaxExtent) ok = false;
     if (from[0] != mul_sat(d->seq, from[1])) collapses = false;
   };
-  take(d->q_stride, d->q_heads, a->q.xs);
-  take(d->k_stride, d->k_heads, a->k.xs);
+  take(d->q_stride, d->q_heads, a->q().xs);
+  take(d->k_stride, d->k_heads, a->k().xs);
   if (grads) {
-    take(d->dq_stride, d->q_heads, a->q.gs);
-    take(d->dk_stride, d->k_heads, a->k.gs);
+    take(d->dq_stride, d->q_heads, a->q().gs);
+    take(d->dk_stride, d->k_heads, a->k().gs);
   }
   const int64_t pos[3] = {d->pos_stride[1], d->pos_stride[2], d->pos_stride[0]};
   int64_t got[3];
@@ -1626,7 +1626,7 @@ static int rope_args(const vbh_rope_desc* d, const char* what, bool norm, bool g
                                       (d->axes - 1) * got[2] + 1;
   if ((flat || collapses) && a->tokens > 0) {
     if (d->seq == 1) {  // the batch is the only token dim
-      for (int64_t* st : {a->q.xs, a->k.xs, a->q.gs, a->k.gs}) st[1] = st[0];
+      for (int64_t* st : {a->q().xs, a->k().xs, a->q().gs, a->k().gs}) st[1] = st[0];
       a->pos_stride[2] = a->pos_stride[1];
     }
     a->seq = static_cast<int>(a->tokens);
@@ -1650,18 +1650,18 @@ static int rope_run(const vbh_rope_desc* d, const char* what, bool norm, bool ba
                     const void* inv_freq, void* q_out, void* k_out, void* stream) {
   RopeArgs a;
   if (int rc = rope_args(d, what, norm, false, &a)) return rc;
-  if (a.tokens == 0 || a.q.heads + a.k.heads == 0) return 0;  // empty outputs
-  if (!rope_side_ok(a.q.heads, {q, q_out}) || !rope_side_ok(a.k.heads, {k, k_out}) ||
+  if (a.tokens == 0 || a.q().heads + a.k().heads == 0) return 0;  // empty outputs
+  if (!rope_side_ok(a.q().heads, {q, q_out}) || !rope_side_ok(a.k().heads, {k, k_out}) ||
       !positions || !inv_freq)
     return fail(VBH_E_INVALID, "%s: null pointer", what);
   if (!aligned16(q_out) || !aligned16(k_out))
     return fail(VBH_E_INVALID, "%s: outputs must be 16-byte aligned", what);
-  a.q.x = q;
-  a.k.x = k;
-  a.q.y = q_out;
-  a.k.y = k_out;
-  a.q.w = qw;
-  a.k.w = kw;
+  a.q().x = q;
+  a.k().x = k;
+  a.q().y = q_out;
+  a.k().y = k_out;
+  a.q().w = qw;
+  a.k().w = kw;
   a.pos = positions;
   a.freq = inv_freq;
   if (back) a.sin_scale = -a.scale;
@@ -1706,9 +1706,9 @@ int vbh_qk_norm_rope_bwd(const vbh_rope_desc* desc, const void* dq_out, const vo
   if (int rc = rope_args(desc, what, true, true, &a)) return rc;
   if (workspace_bytes < 0) return fail(VBH_E_INVALID, "%s: negative workspace size", what);
   const bool adjacent = desc->pairing == VBH_ROPE_ADJACENT;
-  const bool empty = a.tokens == 0 || a.q.heads + a.k.heads == 0;
-  if (!empty && (!rope_side_ok(a.q.heads, {q, dq_out, dq}) ||
-                 !rope_side_ok(a.k.heads, {k, dk_out, dk}) || !positions || !inv_freq))
+  const bool empty = a.tokens == 0 || a.q().heads + a.k().heads == 0;
+  if (!empty && (!rope_side_ok(a.q().heads, {q, dq_out, dq}) ||
+                 !rope_side_ok(a.k().heads, {k, dk_out, dk}) || !positions || !inv_freq))
     return fail(VBH_E_INVALID, "%s: null pointer", what);
   if (!aligned16(dq) || !aligned16(dk))
     return fail(VBH_E_INVALID, "%s: outputs must be 16-byte aligned", what);
@@ -1718,14 +1718,14 @@ int vbh_qk_norm_rope_bwd(const vbh_rope_desc* desc, const void* dq_out, const vo
       (!workspace || workspace_bytes < need || !aligned16(workspace)))
     return fail(VBH_E_INVALID, "%s: the weights' gradients need an aligned workspace of %lld bytes",
                 what, static_cast<long long>(need));
-  a.q.x = q;
-  a.k.x = k;
-  a.q.g = dq_out;
-  a.k.g = dk_out;
-  a.q.y = dq;
-  a.k.y = dk;
-  a.q.w = q_weight;
-  a.k.w = k_weight;
+  a.q().x = q;
+  a.k().x = k;
+  a.q().g = dq_out;
+  a.k().g = dk_out;
+  a.q().y = dq;
+  a.k().y = dk;
+  a.q().w = q_weight;
+  a.k().w = k_weight;
   a.pos = positions;
   a.freq = inv_freq;
   a.sin_scale = -a.scale;

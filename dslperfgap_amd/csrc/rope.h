@@ -4,9 +4,10 @@
 // token's queries or of its keys, so that the angles are made once (one sincos per
 // lane for 64 pairs, through the LDS) for up to 8 passes over vectors.  In a pass
 // the wave holds `per_pass` vectors side by side, each lane V consecutive values:
-// the accesses of a pass run over memory without gaps wherever the heads do.  (Both members of every pair in one lane, as two pieces of half the vector
-// each, costs no exchange, but pieces of less than a 128-byte line cost more: on
-// MI355X 38 us against 27 for 16384 tokens of 40 bf16 heads of 64.)
+// the accesses of a pass run over memory without gaps wherever the heads do.  (Both
+// members of every pair in one lane, as two pieces of half the vector each, costs no
+// exchange, but pieces of less than a 128-byte line cost more: on MI355X 38 us against
+// 27 for 16384 tokens of 40 bf16 heads of 64.)
 //   adjacent pairing: a lane's values pair among themselves
 //   half pairing:     the partners lie in other lanes of the vector's, n_freq / V
 //                     away, whose 16 bytes come over the LDS crossbar as they are
@@ -44,8 +45,7 @@ enum RopeMem : int { kRopeCached = 0, kRopeOnce = 1, kRopeStream = 2 };
 
 // What a launch reads and writes, against the 256 MiB cache in front of the memory.
 // MI355X, 16384 tokens of 40 bf16 heads (168 MB in, as much out; three sets of inputs
-// in turn), us by loads / stores, nt: nontemporal:
-// (without the write-through)
+// in turn), us by loads / stores, nt: nontemporal, all without the write-through:
 //   forward, 168 MB in and out   nt / nt 55.6, nt / plain 51.8, plain / plain 61.1
 //   the same, 336 MB             nt / nt 108.4, nt / plain 116
 //   the same with the norm, 84 MB nt / plain 29.5, plain / plain 33.2
@@ -66,6 +66,8 @@ void dispatch_rope_mem(RopeMem m, Fn&& fn) {
   else fn(std::integral_constant<int, kRopeStream>{});
 }
 
+constexpr int kRopeScratch = 128;  // floats per sum: 64 lanes, lines of 4
+
 // A wave's part of the LDS, in floats (whole 16-byte vectors): its table of angles, the
 // scratch of `sums` sums where vectors are no power of two of lanes, and where a.gather
 // the vectors of `passes` passes.
@@ -76,7 +78,7 @@ struct RopeLds {
 __host__ __device__ inline RopeLds rope_lds_of(const RopeArgs& a, int sums, int passes) {
   RopeLds r;
   r.table = (2 * a.n_freq + 15) & ~15;  // table_place stays in runs of 8 pairs
-  r.scratch = a.tile.lanes_log2 < 0 ? sums * 128 : 0;
+  r.scratch = a.tile.lanes_log2 < 0 ? sums * kRopeScratch : 0;
   r.rows = a.gather ? passes * (kWave * 16 / 4) : 0;
   return r;
 }
@@ -518,7 +520,6 @@ __device__ __forceinline__ void wave_sums(float (&v)[N], int log2) {
 // Sums of N values over the lanes of each vector, in every lane of it.  `scratch`:
 // N * kRopeScratch floats of the wave's own, used where the lanes are no power of
 // two: there each lane leaves its value and adds up its vector's.
-constexpr int kRopeScratch = 128;  // rope_lds_of
 template <int N>
 __device__ __forceinline__ void vector_sums(const RopeArgs& a, const RopeLane& l, float (&v)[N],
                                             float* scratch) {

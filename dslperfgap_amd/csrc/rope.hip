@@ -90,16 +90,16 @@ __global__ __launch_bounds__(kRopeBlock, 6) void rope_rows(const RopeArgs) {
   extern __shared__ __align__(16) float rope_lds[];
   const int wave = wave_index();
   float* lds = rope_lds + wave * rope_lds_of(a, NORM ? kRopePasses : 0, kRopePasses).all();
-  const uint32_t chunks = static_cast<uint32_t>(a.q.chunks + a.k.chunks);
+  const uint32_t chunks = static_cast<uint32_t>(a.q().chunks + a.k().chunks);
   const uint32_t unit = blockIdx.x * static_cast<uint32_t>(kRopeWaves) + wave;
   const uint32_t turn_of = unit / chunks;
   const int64_t token = a.first + turn_of;
   if (token >= a.tokens) return;
   const int chunk = static_cast<int>(unit - turn_of * chunks);
   const RopeToken t = rope_token(a, token);
-  const bool is_k = chunk >= a.q.chunks;
+  const bool is_k = chunk >= a.q().chunks;
   const RopeSide& side = a.side(is_k);
-  const int head0 = (is_k ? chunk - a.q.chunks : chunk) * side.per_wave * a.tile.per_pass;
+  const int head0 = (is_k ? chunk - a.q().chunks : chunk) * side.per_wave * a.tile.per_pass;
   switch (side.per_wave) {
     case 1: return rope_share<T, V, 1, NORM, ADJ, WAY, MEM>(a, side, t, head0, lds);
     case 2: return rope_share<T, V, 2, NORM, ADJ, WAY, MEM>(a, side, t, head0, lds);
@@ -115,7 +115,7 @@ __global__ __launch_bounds__(kRopeBlock) void rope_values(const RopeArgs a) {
   const int wave = wave_index();
   float2* table =
       reinterpret_cast<float2*>(rope_lds + wave * rope_lds_of(a, 0, 0).table);
-  const uint32_t chunks = static_cast<uint32_t>(a.q.chunks + a.k.chunks);
+  const uint32_t chunks = static_cast<uint32_t>(a.q().chunks + a.k().chunks);
   const uint32_t unit = blockIdx.x * static_cast<uint32_t>(kRopeWaves) + wave;
   const uint32_t turn_of = unit / chunks;
   const int64_t token = a.first + turn_of;
@@ -123,9 +123,9 @@ __global__ __launch_bounds__(kRopeBlock) void rope_values(const RopeArgs a) {
   const int chunk = static_cast<int>(unit - turn_of * chunks);
   const RopeToken t = rope_token(a, token);
   const RopeLane l = rope_lane(a);
-  const bool is_q = chunk < a.q.chunks;
+  const bool is_q = chunk < a.q().chunks;
   const RopeSide& side = a.side(!is_q);
-  const int head = (is_q ? chunk : chunk - a.q.chunks) * a.tile.per_pass + l.sub;
+  const int head = (is_q ? chunk : chunk - a.q().chunks) * a.tile.per_pass + l.sub;
   const bool ok = l.live && head < side.heads;
   const Span sx = VBH_SPAN(static_cast<const T*>(side.x), rope_extent(a, side.xs, side.heads));
   const T* x = static_cast<const T*>(side.x) + token_offset(t, side.xs) + head * side.xs[2];
@@ -194,7 +194,7 @@ void rope_shape(RopeArgs& a, int dt, bool adjacent, bool norm, int64_t many, int
   auto passes = [&](const RopeSide& side, int lanes) {
     return (side.heads + kWave / lanes - 1) / (kWave / lanes);
   };
-  auto all = [&](int lanes) { return passes(a.q, lanes) + passes(a.k, lanes); };
+  auto all = [&](int lanes) { return passes(a.q(), lanes) + passes(a.k(), lanes); };
   // Vectors of no power of two of accesses: side by side without a gap, or a power of
   // two of lanes apart, which leaves lanes idle but sums in registers.  MI355X, 16384
   // tokens of 32 + 8 bf16 heads, us side by side / apart: heads of 96 (9 / 10 passes)
@@ -206,7 +206,7 @@ void rope_shape(RopeArgs& a, int dt, bool adjacent, bool norm, int64_t many, int
                 : t.accesses;
   t.lanes_log2 = (t.lanes & (t.lanes - 1)) == 0 ? __builtin_ctz(t.lanes) : -1;
   t.per_pass = kWave / t.lanes;
-  const int pq = passes(a.q, t.lanes), pk = passes(a.k, t.lanes);
+  const int pq = passes(a.q(), t.lanes), pk = passes(a.k(), t.lanes);
   const int64_t total = a.tokens * (pq + pk);
   if (a.n_freq <= kWave && t.lanes_log2 >= 0 && t.lanes == t.accesses && t.v * elt == 16)
     most = std::min(most, 4);
@@ -225,18 +225,18 @@ void rope_shape(RopeArgs& a, int dt, bool adjacent, bool norm, int64_t many, int
       side.chunks = chunks;
     }
   };
-  share(a.q, pq);
-  share(a.k, pk);
+  share(a.q(), pq);
+  share(a.k(), pk);
 }
 
 hipError_t launch_rope(const RopeArgs& args, int dt, bool adjacent, bool norm, hipStream_t s) {
   RopeArgs a = args;
   rope_shape(a, dt, adjacent, norm, kRopeFewPasses, kRopePasses, kRopePasses, false);
   const RopeTile& t = a.tile;
-  const int chunks = a.q.chunks + a.k.chunks;
+  const int chunks = a.q().chunks + a.k().chunks;
   const bool whole = 2 * a.n_freq == a.dim && (adjacent || a.n_freq % t.v == 0);
   const int64_t bytes =
-      a.tokens * (a.q.heads + a.k.heads) * a.dim * (dt == kF32 ? 4 : 2);
+      a.tokens * (a.q().heads + a.k().heads) * a.dim * (dt == kF32 ? 4 : 2);
   hipError_t err = hipErrorInvalidValue;
   auto go = [&](auto kernel, size_t floats) {
     // as many launches as keep each under 2^32 work-items

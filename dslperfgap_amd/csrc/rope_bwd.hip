@@ -25,7 +25,7 @@ struct RopeRows {
   int q, k, k_from;
 };
 __host__ __device__ inline RopeRows rope_rows_of(const RopeArgs& a) {
-  const int q = a.q.chunks * a.q.walkers, k = a.k.chunks * a.k.walkers;
+  const int q = a.q().chunks * a.q().walkers, k = a.k().chunks * a.k().walkers;
   RopeRows r;
   r.q = (q + kRopeWaves - 1) / kRopeWaves;
   r.k_from = q / kRopeWaves;
@@ -41,10 +41,10 @@ struct RopeWalk {
 };
 __device__ __forceinline__ RopeWalk rope_walk(const RopeArgs& a, int wave) {
   const int w = static_cast<int>(blockIdx.x) * kRopeWaves + wave;
-  const int q = a.q.chunks * a.q.walkers, k = a.k.chunks * a.k.walkers;
+  const int q = a.q().chunks * a.q().walkers, k = a.k().chunks * a.k().walkers;
   const bool is_q = w < q;
   const uint32_t i = static_cast<uint32_t>(is_q ? w : w - q);
-  const uint32_t chunks = static_cast<uint32_t>(max(is_q ? a.q.chunks : a.k.chunks, 1));
+  const uint32_t chunks = static_cast<uint32_t>(max(is_q ? a.q().chunks : a.k().chunks, 1));
   const uint32_t token = i / chunks;
   return RopeWalk{is_q, w < q + k, static_cast<int>(i - token * chunks),
                   static_cast<int>(token)};
@@ -57,7 +57,7 @@ __device__ __forceinline__ void write_part(const RopeArgs& a, const float* sums,
   const RopeRows rows = rope_rows_of(a);
   const Span sp = VBH_SPAN(parts, static_cast<int64_t>(rows.q + rows.k) * a.dim);
   const int block = static_cast<int>(blockIdx.x);
-  const int cut = min(max(a.q.chunks * a.q.walkers - block * kRopeWaves, 0), kRopeWaves);
+  const int cut = min(max(a.q().chunks * a.q().walkers - block * kRopeWaves, 0), kRopeWaves);
   for (int d = static_cast<int>(threadIdx.x); d < a.dim; d += kRopeBlock) {
     float q = 0.0f, k = 0.0f;
     for (int v = 0; v < cut * each; ++v) q += sums[v * a.dim + d];
@@ -115,6 +115,12 @@ __device__ __forceinline__ void grad_share(const RopeArgs& a, const RopeSide& si
         x[u] = load_any<T, V, MEM != kRopeCached>(
             ok[u] ? from_x + (pass + u) * x_step : x0 + l.at * V, sx);
       }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        // and, with no gradient and r = 0 below, add nothing to the weights' sums
+        // (not a number only where the first vector makes them so)
+        if (!ok[u]) g[u] = typename Raw<T, V>::type{};
+      }
       if (pass == 0) {
         wave_lds_fence();
         angles.make(a, t, pos, table);
@@ -142,7 +148,6 @@ __device__ __forceinline__ void grad_share(const RopeArgs& a, const RopeSide& si
       vector_sums<2 * U>(a, l, sums, scratch);
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        // lanes without a vector add nothing to the sums
         const float r = ok[u] ? inverse_root(fmaf(sums[2 * u], inv_dim, a.eps)) : 0.0f;
         const float mean = sums[2 * u + 1] * r * inv_dim * r;
         float o[V];
@@ -354,8 +359,8 @@ constexpr int kGradShare = 8;
 void grad_shape(RopeArgs& a, int dt, bool adjacent) {
   rope_shape(a, dt, adjacent, true, kGradMany, kGradPasses, kGradShare, true);
   auto work = [&](const RopeSide& s) { return int64_t(s.chunks) * (s.per_wave + 2); };
-  const int64_t all = work(a.q) + work(a.k);
-  for (RopeSide* s : {&a.q, &a.k}) {
+  const int64_t all = work(a.q()) + work(a.k());
+  for (RopeSide* s : {&a.q(), &a.k()}) {
     s->walkers = 0;
     if (s->chunks == 0 || a.tokens == 0) continue;
     const int64_t most =
@@ -383,8 +388,8 @@ hipError_t launch_qk_norm_rope_bwd(const RopeArgs& args, int dt, bool adjacent, 
   const bool whole = 2 * a.n_freq == a.dim && (adjacent || a.n_freq % t.v == 0);
   const bool sums = dq_weight != nullptr || dk_weight != nullptr;
   const int64_t bytes =
-      a.tokens * (a.q.heads + a.k.heads) * a.dim * (dt == kF32 ? 4 : 2);
-  const int waves = a.q.chunks * a.q.walkers + a.k.chunks * a.k.walkers;
+      a.tokens * (a.q().heads + a.k().heads) * a.dim * (dt == kF32 ? 4 : 2);
+  const int waves = a.q().chunks * a.q().walkers + a.k().chunks * a.k().walkers;
   hipError_t err = hipSuccess;
   if (waves > 0) {
     const size_t row_sums = sums ? size_t(kRopeWaves) * t.per_pass * a.dim : 0;

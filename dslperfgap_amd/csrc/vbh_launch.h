@@ -338,8 +338,12 @@ struct RopeTile {
   int per_pass = 64;  // vectors that a wave holds side by side
 };
 struct RopeArgs {
-  RopeSide q, k;  // side 0, side 1 (side())
-  __host__ __device__ const RopeSide& side(bool is_k) const { return (&q)[is_k ? 1 : 0]; }
+  RopeSide sides[2];  // queries, keys
+  __host__ __device__ RopeSide& q() { return sides[0]; }
+  __host__ __device__ RopeSide& k() { return sides[1]; }
+  __host__ __device__ const RopeSide& q() const { return sides[0]; }
+  __host__ __device__ const RopeSide& k() const { return sides[1]; }
+  __host__ __device__ const RopeSide& side(bool is_k) const { return sides[is_k ? 1 : 0]; }
   const void* pos = nullptr;
   const void* freq = nullptr;
   int64_t pos_stride[3] = {0, 0, 0};  // axis, batch, token

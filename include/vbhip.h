@@ -256,7 +256,7 @@ int64_t vbh_reduce_workspace_bytes(int64_t outer, int64_t n, int64_t inner, int 
  * The angle is formed in 64 bits and reduced before it is rounded to 32.
  * Strides are in elements and may be zero (inputs) or those of any view whose
  * vectors are contiguous; outputs are contiguous [batch, seq, heads, head_dim],
- * 16-byte aligned. */
+ * 16-byte aligned and apart from the inputs. */
 #define VBH_ROPE_MAX_AXES 4
 #define VBH_ROPE_MAX_DIM 1024
 

@@ -104,7 +104,9 @@ def backward(dy, x, theta, pairing, scale, weight, eps):
     mean(dn w u): r within 13 steps, the sum of m 22 more, the products 2 each, so that
     80 steps of r (G |w| + |u| mean(G |w| |u|)) hold all.  The weight's gradient adds N
     terms of G |u|, each within 8 + 13 + 2 steps, in chains of fewer than 400 + N / 256
-    additions."""
+    additions: a lane adds N / 256 at most where both sides' passes together are no more
+    than 5 times this side's heads (4096 waves, a side's in proportion to its passes + 2
+    per share), the sums of its workgroup and of the rows fewer than 400."""
     dy, x = dy.double(), x.double()
     w = torch.ones(x.shape[-1], dtype=torch.float64) if weight is None else weight.double()
     dn = turn(dy, theta, pairing, scale, back=True)

@@ -1,0 +1,61 @@
+"""Calls that reach every kernel of the query / key operators at sizes whose last vectors,
+lanes, shares and workgroups are not full.  run() returns the outputs; as a program it
+saves them, and the debug library's failed bounds checks, to the file it is given."""
+import sys
+from pathlib import Path
+
+import torch
+
+sys.path.insert(0, str(Path(__file__).resolve().parents[1]))
+
+from dslperfgap_amd import _lib  # noqa: E402
+from dslperfgap_amd.viperbench.qk_norm_rope.hip_impl import (  # noqa: E402
+    qk_norm_rope_bwd, qk_norm_rope_fwd)
+from dslperfgap_amd.viperbench.rope.hip_impl import rope_bwd, rope_fwd  # noqa: E402
+
+DEV = "cuda:0"
+SIZES = [(64, 32), (64, 20), (72, 36), (80, 40), (96, 48), (100, 50), (50, 25), (33, 16),
+         (192, 96), (256, 128), (1023, 511), (1024, 512)]
+# tokens, query heads, key heads: single passes; shares of several, several tokens a wave
+COUNTS = [(1, 1, 1), (37, 5, 2), (8193, 9, 3)]
+
+
+def run() -> dict:
+    out = {}
+    for dtype in (torch.float32, torch.bfloat16):
+        for dim, n in SIZES:
+            for tokens, hq, hk in COUNTS:
+                if tokens > 1000 and dim > 256:
+                    continue
+                g = torch.Generator(DEV).manual_seed(dim + tokens)
+
+                def heads(h):
+                    return torch.randn(tokens, h, dim, generator=g, device=DEV).to(dtype)
+
+                q, k, gq, gk = heads(hq), heads(hk), heads(hq), heads(hk)
+                w = torch.rand(dim, generator=g, device=DEV) + 0.5
+                pos = torch.arange(tokens, device=DEV)
+                freq = 10000.0 ** -(torch.arange(n, device=DEV) / n)
+                for pairing in ("half", "adjacent"):
+                    key = f"{dtype} {dim} {n} {tokens} {pairing} "
+                    got = [*rope_fwd(q, k, pos, freq, pairing=pairing),
+                           *rope_bwd(gq, gk, pos, freq, pairing=pairing),
+                           *qk_norm_rope_fwd(q, k, w, w, pos, freq, pairing=pairing),
+                           *qk_norm_rope_bwd(gq, gk, q, k, w, w, pos, freq, pairing=pairing)]
+                    for i, t in enumerate(got):
+                        # the whole output as bits, summed: exact, and small to keep
+                        bits = t.contiguous().view(torch.int16 if t.dtype == torch.bfloat16
+                                                   else torch.int32)
+                        out[key + str(i)] = bits.long().sum().cpu()
+    torch.cuda.synchronize()
+    return out
+
+
+if __name__ == "__main__":
+    # child process: VBHIP_LIB names the debug library
+    _lib.lib()
+    _lib.debug_bounds(clear=True)
+    outs = run()
+    failed, where = _lib.debug_bounds(clear=True)
+    torch.save({"outs": outs, "failed": failed, "where": where}, sys.argv[1])
+    print(f"[bounds] {len(outs)} outputs, {failed} failed checks", flush=True)
