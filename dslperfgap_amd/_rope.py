@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+import numbers
 
 import torch
 
@@ -95,6 +96,14 @@ def make_plan(what, q, k, positions, inv_freq, sections, section_order, pairing,
                          f"{section_order!r}")
     if pairing not in PAIRINGS:
         raise ValueError(f"{what}: pairing must be one of {sorted(PAIRINGS)}, got {pairing!r}")
+    # plans are kept by these values: numbers, nothing that may change behind its key
+    for value, name in ((scale, "scale"), (eps, "eps")):
+        if not isinstance(value, numbers.Real):
+            raise TypeError(f"{what}: {name} must be a number, got {type(value).__name__}")
+    scale, eps = float(scale), float(eps)
+    if sections is not None and not (isinstance(sections, tuple) and
+                                     all(isinstance(s, numbers.Integral) for s in sections)):
+        raise TypeError(f"{what}: sections must be a tuple or list of integers, got {sections!r}")
     parts = (n,) if sections is None else tuple(int(s) for s in sections)
     if not 1 <= len(parts) <= _lib.ROPE_MAX_AXES:
         raise ValueError(f"{what}: sections must name 1..{_lib.ROPE_MAX_AXES} axes, got "
@@ -193,7 +202,7 @@ def rotate(what, q, k, positions, inv_freq, sections, section_order, pairing, sc
             return rotate(what, qc, kc, positions, inv_freq, sections, section_order, pairing,
                           scale)
         p = _PLANS.put(key, make_plan(what, q, k, positions, inv_freq, sections, section_order,
-                                      pairing, float(scale), 0.0, None, None))
+                                      pairing, scale, 0.0, None, None))
     dev = q.get_device()
     if (dev < 0 or k.get_device() != dev or positions.get_device() != dev or
             inv_freq.get_device() != dev):
@@ -224,7 +233,7 @@ def norm_rotate(q, k, q_weight, k_weight, positions, inv_freq, eps, sections, se
             return norm_rotate(qc, kc, qw, kw, positions, inv_freq, eps, sections,
                                section_order, pairing, scale)
         p = _PLANS.put(key, make_plan(what, q, k, positions, inv_freq, sections, section_order,
-                                      pairing, float(scale), float(eps), (qw, kw), None))
+                                      pairing, scale, eps, (qw, kw), None))
     dev = _on(q.get_device(), what, q, k, qw, kw, positions, inv_freq)
     fn, desc, q_shape, q_strides, k_shape, k_strides, _, _ = p
     q_out = q.new_empty_strided(q_shape, q_strides)
@@ -255,7 +264,7 @@ def norm_rotate_grads(dq_out, dk_out, q, k, q_weight, k_weight, positions, inv_f
             return norm_rotate_grads(*dense, q_weight, k_weight, positions, inv_freq, eps,
                                      sections, section_order, pairing, scale)
         p = _PLANS.put(key, make_plan(what, q, k, positions, inv_freq, sections, section_order,
-                                      pairing, float(scale), float(eps), (qw, kw),
+                                      pairing, scale, eps, (qw, kw),
                                       (dq_out, dk_out)))
     dev = _on(q.get_device(), what, q, k, dq_out, dk_out, qw, kw, positions, inv_freq)
     fn, desc, q_shape, q_strides, k_shape, k_strides, n, _ = p

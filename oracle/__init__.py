@@ -19,6 +19,10 @@ ce_loops
     Pure-Python per-(row, column block) loops following the reference's Triton
     program (ViperBench/cross_entropy/triton_impl.py:33-75, 98-120), for tiny
     inputs; pins the vectorized CE restatement.
+rope
+    The rotation of queries and keys and the per-head norm ahead of it, forward
+    and backward in float64, with error bounds for 32-bit evaluation.  The
+    reference has no such operator.
 
 Pinning (what checks each function; see tests/test_oracle_pins.py):
   layer_norm      numpy fp64 closed form; mean-0 / variance invariants; all-equal
@@ -43,6 +47,8 @@ Pinning (what checks each function; see tests/test_oracle_pins.py):
   max_reduction / argmax  hand-computed known answers (ties -> first index,
                   NaN is the largest value, all -inf rows -> 0, +inf ties);
                   numpy first-occurrence argmax over every dim
+  rope            complex multiplication; torch.autograd and differences of the
+                  forward for the gradients (tests/test_rope_api.py)
 The reference itself ships no golden vectors or fixtures for this path, and its
 Python was not imported or run: every function above is pinned by the checks
 listed, none is "parity unpinned".
