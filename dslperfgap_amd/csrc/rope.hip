@@ -82,7 +82,7 @@ __device__ __forceinline__ void rope_share(const RopeArgs& a, const RopeSide& si
 }
 
 // 6 waves to a SIMD, 80 registers: norm and rotation of 16384 tokens of 40 bf16 heads of
-// 128 take 53.2 us so, 53.9 at 5 waves, 57.0 at 7 and 74 at 8, where registers spill;
+// 128 take 53.2 us so (54.9 in a later run), 53.9 at 5 waves, 57.0 at 7 and 74 at 8, where registers spill;
 // of 96, adjacent pairs 45.0 and 50.7 at 5.
 template <typename T, int V, bool NORM, bool ADJ, int WAY, int MEM>
 __global__ __launch_bounds__(kRopeBlock, 6) void rope_rows(const RopeArgs) {
