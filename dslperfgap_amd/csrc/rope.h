@@ -12,9 +12,11 @@
 //   half pairing:     the partners lie in other lanes of the vector's, n_freq / V
 //                     away, whose 16 bytes come over the LDS crossbar as they are
 //                     stored; both lanes then widen both vectors (RopePartner)
-// Per value y_i = (x_i C_i + x_partner S_i) r: the cosines and sines, their signs,
+// Per value y_i = (x_i r) C_i + (x_partner r) S_i: the cosines and sines, their signs,
 // the scale and the weights meet in C and S once per wave, so that the norm adds
-// one product per value and its sum of squares.
+// its sum of squares and one product per value, two in half pairing.  (One product
+// with r at the end would do, but x_i C_i may pass the range of 32 bits where y_i
+// does not.)
 //
 // Vectors that no lane access of 2 values or more fits (odd sizes, more than 64
 // lanes) go pair by pair: a lane holds both members of a pair (rope_values,

@@ -70,12 +70,15 @@ __device__ __forceinline__ void rope_share(const RopeArgs& a, const RopeSide& si
     if constexpr (!ADJ) partners.get(x[u], u, other);
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-      const float xi = raw_at<T, V>(x[u], i);
-      const float xp = ADJ ? raw_at<T, V>(x[u], i ^ 1) : other[i];
-      float y = fmaf(xi, turn.c[i], xp * turn.s[i]);
+      float xi = raw_at<T, V>(x[u], i);
+      float xp = ADJ ? raw_at<T, V>(x[u], i ^ 1) : other[i];
+      if constexpr (NORM) {  // first: a product with C or S may pass the range of 32 bits
+        xi *= size[u];
+        xp *= size[u];
+      }
+      const float y = fmaf(xi, turn.c[i], xp * turn.s[i]);
       // a value that passes takes nothing from another, which may be infinite
-      if (WAY != kRopeWhole && turn.passing[i]) y = xi * turn.c[i];
-      o[i] = NORM ? y * size[u] : y;
+      o[i] = WAY != kRopeWhole && turn.passing[i] ? xi * turn.c[i] : y;
     }
     out.store(to + u * step, ok[u], o);
   }
