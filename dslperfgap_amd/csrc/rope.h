@@ -97,6 +97,12 @@ __device__ __forceinline__ float inverse_root(float m) {
   return __builtin_amdgcn_rsqf(tiny ? m * 0x1p96f : m) * (tiny ? 0x1p48f : 1.0f);
 }
 
+// Infinite or not a number.
+__device__ __forceinline__ bool past_range(float x) { return !(fabsf(x) <= 0x1.fffffep127f); }
+
+// True in every lane where it is in one of the wave's.
+__device__ __forceinline__ bool wave_any(bool b) { return __ballot(b) != 0; }
+
 // What one wave wrote to its part of the LDS is there for all of its lanes (the
 // wave's LDS accesses stay in order; this keeps the compiler to it).
 __device__ __forceinline__ void wave_lds_fence() {

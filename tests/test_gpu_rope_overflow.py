@@ -5,7 +5,7 @@ lowest value, against rms_norm and rope_fwd one after the other."""
 import pytest
 import torch
 
-from dslperfgap_amd.viperbench.qk_norm_rope.hip_impl import qk_norm_rope_fwd
+from dslperfgap_amd.viperbench.qk_norm_rope.hip_impl import qk_norm_rope_bwd, qk_norm_rope_fwd
 from dslperfgap_amd.viperbench.rms_norm.hip_impl import rms_norm
 from dslperfgap_amd.viperbench.rope.hip_impl import rope_fwd
 from oracle import rope as ref
@@ -73,3 +73,62 @@ def test_rows_of_the_lowest_value(dim, n, pairing, dtype):
     for out in qk_norm_rope_fwd(xd, xd, wd, wd, pd, fd, EPS, pairing=pairing):
         assert not bool(out.cpu()[low].any())
         _held(out.cpu()[~low], want[~low], bound[~low], dtype, "forward")
+
+
+@pytest.mark.parametrize("pairing,dtype", HOW, ids=str)
+@pytest.mark.parametrize("dim,n", SIZES)
+def test_large_vectors_with_large_gradients(dim, n, pairing, dtype):
+    """sum(dn w x) passes 1e39, mean(dn w u) is 1e22 at most."""
+    print(f"[gpu] large gradients, heads of {dim}, {pairing}, {dtype}", flush=True)
+    x, dy, pos, freq, theta, g = _case(dim, n, dtype)
+    x, dy = (x.float() * 3e17).to(dtype), (dy.float() * 1e21).to(dtype)
+    w = (1 + 0.3 * torch.rand(dim, generator=g)).to(dtype)
+    got = qk_norm_rope_bwd(*[t.to(DEV) for t in (dy, dy, x, x, w, w, pos, freq)], EPS,
+                           pairing=pairing)
+    dx, dw, bx, bw = ref.backward(dy, x, theta, pairing, 1.0, w, EPS)
+    for i in (0, 1):
+        _held(got[i], dx, bx, dtype, "backward")
+        _held(got[2 + i], dw, bw, dtype, "weight")
+
+
+@pytest.mark.parametrize("pairing,dtype", HOW, ids=str)
+@pytest.mark.parametrize("dim,n", SIZES)
+def test_gradients_of_rows_of_the_lowest_value(dim, n, pairing, dtype):
+    """They are zeros, and add nothing to the weights'; the others keep theirs."""
+    print(f"[gpu] gradients at lowest values, heads of {dim}, {pairing}, {dtype}", flush=True)
+    x, dy, w, pos, freq, theta, low = _with_lowest_rows(dim, n, dtype)
+    got = qk_norm_rope_bwd(*[t.to(DEV) for t in (dy, dy, x, x, w, w, pos, freq)], EPS,
+                           pairing=pairing)
+    dx, _, bx, _ = ref.backward(dy, x, theta, pairing, 1.0, w, EPS)
+    for t in (dy, x):
+        t[low] = 0
+    _, dw, _, bw = ref.backward(dy, x, theta, pairing, 1.0, w, EPS)
+    for i in (0, 1):
+        assert not bool(got[i].cpu()[low].any())
+        _held(got[i].cpu()[~low], dx[~low], bx[~low], dtype, "backward")
+        _held(got[2 + i], dw, bw, dtype, "weight")
+
+
+# a wave takes one pass of a token, two, and eight, of several tokens
+@pytest.mark.parametrize("tokens,hq,hk,dim", [(700, 6, 2, 128), (4200, 32, 8, 128),
+                                              (14000, 16, 4, 192)])
+@pytest.mark.parametrize("pairing", ["half", "adjacent"])
+def test_lowest_rows_leave_the_others_as_they_are(tokens, hq, hk, dim, pairing):
+    """The others' gradients are bit for bit those of a call in which such rows are zeros."""
+    print(f"[gpu] {tokens} tokens of {hq} + {hk} heads of {dim}, {pairing}", flush=True)
+    g = torch.Generator(DEV).manual_seed(dim)
+    q, k, gq, gk = (torch.randn(tokens, h, dim, generator=g, device=DEV).to(BF16)
+                    for h in (hq, hk, hq, hk))
+    w = (1 + 0.3 * torch.randn(dim, generator=g, device=DEV)).to(BF16)
+    pos, freq = torch.arange(tokens, device=DEV), ref.inv_freq(dim // 2).to(DEV)
+    low = [torch.rand(t.shape[:2], generator=g, device=DEV) < 0.01 for t in (q, k)]
+    outs = []
+    for fill in (torch.finfo(BF16).min, 0.0):
+        x = [t.clone() for t in (q, k)]
+        for t, rows in zip(x, low):
+            t[rows] = fill
+        outs.append(qk_norm_rope_bwd(gq, gk, *x, w, w, pos, freq, EPS, pairing=pairing))
+    for i, rows in enumerate(low):
+        assert int(rows.sum()) > 0 and not bool(outs[0][i][rows].any())
+        assert torch.equal(outs[0][i][~rows], outs[1][i][~rows])
+        assert torch.equal(outs[0][2 + i], outs[1][2 + i])
