@@ -2,8 +2,9 @@
 the checks of their arguments and the descriptors of their launches, cached by what
 decides them.
 
-Every argument rule is checked where a plan is made, without a GPU; a call with
-tensors the plan knows goes straight to the entry point.
+Options are plain numbers when a plan is looked up by them (values that only equal such
+are refused first); every other rule is checked where a plan is made, without a GPU, and a
+call with tensors the plan knows goes straight to the entry point.
 """
 from __future__ import annotations
 
@@ -70,12 +71,28 @@ def _position_strides(positions, lead, axes, what):
     raise ValueError(f"{what}: positions must have shape {want}, got {list(positions.shape)}")
 
 
+def _number(what, value, name):
+    """An option as a float."""
+    if not isinstance(value, numbers.Real):
+        raise TypeError(f"{what}: {name} must be a number, got {type(value).__name__}")
+    return float(value)
+
+
+def _sections(what, sections):
+    """Sections as a tuple of ints."""
+    if not (isinstance(sections, (tuple, list)) and
+            all(isinstance(s, numbers.Integral) for s in sections)):
+        raise TypeError(f"{what}: sections must be a tuple or list of integers, got {sections!r}")
+    return tuple(map(int, sections))
+
+
 def make_plan(what, q, k, positions, inv_freq, sections, section_order, pairing, scale, eps,
               weights, grads):
     """The plan of a call whose vectors and weights the kernels read as they are: (entry
     point, descriptor's address, shape and strides of the queries' output, of the keys',
-    workspace bytes, descriptor), or the error its arguments deserve.  `weights`: None (no
-    norm) or (q_weight, k_weight); `grads`: None or (dq_out, dk_out)."""
+    workspace bytes, descriptor), or the error its arguments deserve.  `sections`: None or a
+    tuple of ints; `weights`: None (no norm) or (q_weight, k_weight); `grads`: None or
+    (dq_out, dk_out)."""
     # the vectors that run through the rotation, under the name the caller knows
     names = ("dq_out", "dk_out") if what == "rope_bwd" else ("q", "k")
     _check_pair(q, k, what, names)
@@ -96,15 +113,7 @@ def make_plan(what, q, k, positions, inv_freq, sections, section_order, pairing,
                          f"{section_order!r}")
     if pairing not in PAIRINGS:
         raise ValueError(f"{what}: pairing must be one of {sorted(PAIRINGS)}, got {pairing!r}")
-    # plans are kept by these values: numbers, nothing that may change behind its key
-    for value, name in ((scale, "scale"), (eps, "eps")):
-        if not isinstance(value, numbers.Real):
-            raise TypeError(f"{what}: {name} must be a number, got {type(value).__name__}")
-    scale, eps = float(scale), float(eps)
-    if sections is not None and not (isinstance(sections, tuple) and
-                                     all(isinstance(s, numbers.Integral) for s in sections)):
-        raise TypeError(f"{what}: sections must be a tuple or list of integers, got {sections!r}")
-    parts = (n,) if sections is None else tuple(int(s) for s in sections)
+    parts = (n,) if sections is None else sections
     if not 1 <= len(parts) <= _lib.ROPE_MAX_AXES:
         raise ValueError(f"{what}: sections must name 1..{_lib.ROPE_MAX_AXES} axes, got "
                          f"{list(parts)}")
@@ -190,8 +199,10 @@ def _run(fn, what, dev, *args):
 
 def rotate(what, q, k, positions, inv_freq, sections, section_order, pairing, scale):
     """rope_fwd, and rope_bwd with q and k the incoming gradients."""
-    if type(sections) is list:
-        sections = tuple(sections)
+    if sections is not None:
+        sections = _sections(what, sections)
+    if type(scale) is not float:
+        scale = _number(what, scale, "scale")
     key = (what, q.shape, q.stride(), q.dtype, k.shape, k.stride(), k.dtype, positions.shape,
            positions.stride(), positions.dtype, inv_freq.shape, inv_freq.stride(), inv_freq.dtype,
            sections, section_order, pairing, scale)
@@ -218,14 +229,18 @@ def rotate(what, q, k, positions, inv_freq, sections, section_order, pairing, sc
 def norm_rotate(q, k, q_weight, k_weight, positions, inv_freq, eps, sections, section_order,
                 pairing, scale):
     what = "qk_norm_rope_fwd"
-    if type(sections) is list:
-        sections = tuple(sections)
+    if sections is not None:
+        sections = _sections(what, sections)
+    if type(scale) is not float:
+        scale = _number(what, scale, "scale")
+    if type(eps) is not float:
+        eps = _number(what, eps, "eps")
     qw, kw = _weights(q_weight, k_weight, q.dtype, what)
     key = (what, q.shape, q.stride(), q.dtype, k.shape, k.stride(), k.dtype, positions.shape,
            positions.stride(), positions.dtype, inv_freq.shape, inv_freq.stride(), inv_freq.dtype,
-           sections, section_order, pairing, scale, eps, None if qw is None else qw.shape,
-           None if kw is None else kw.shape, (kw if qw is None else qw) is None or
-           (kw if qw is None else qw).dtype)
+           sections, section_order, pairing, scale, eps,
+           None if qw is None else qw.shape, None if kw is None else kw.shape,
+           (kw if qw is None else qw) is None or (kw if qw is None else qw).dtype)
     p = _PLANS.get(key)
     if p is None:
         qc, kc = _contiguous(q), _contiguous(k)
@@ -247,15 +262,20 @@ def norm_rotate(q, k, q_weight, k_weight, positions, inv_freq, eps, sections, se
 def norm_rotate_grads(dq_out, dk_out, q, k, q_weight, k_weight, positions, inv_freq, eps,
                       sections, section_order, pairing, scale):
     what = "qk_norm_rope_bwd"
-    if type(sections) is list:
-        sections = tuple(sections)
+    if sections is not None:
+        sections = _sections(what, sections)
+    if type(scale) is not float:
+        scale = _number(what, scale, "scale")
+    if type(eps) is not float:
+        eps = _number(what, eps, "eps")
     qw, kw = _weights(q_weight, k_weight, q.dtype, what)
     key = (what, q.shape, q.stride(), q.dtype, k.shape, k.stride(), k.dtype, positions.shape,
            positions.stride(), positions.dtype, inv_freq.shape, inv_freq.stride(), inv_freq.dtype,
-           sections, section_order, pairing, scale, eps, None if qw is None else qw.shape,
-           None if kw is None else kw.shape, (kw if qw is None else qw) is None or
-           (kw if qw is None else qw).dtype, dq_out.shape, dq_out.stride(), dq_out.dtype,
-           dk_out.shape, dk_out.stride(), dk_out.dtype)
+           sections, section_order, pairing, scale, eps,
+           None if qw is None else qw.shape, None if kw is None else kw.shape,
+           (kw if qw is None else qw) is None or (kw if qw is None else qw).dtype,
+           dq_out.shape, dq_out.stride(), dq_out.dtype, dk_out.shape, dk_out.stride(),
+           dk_out.dtype)
     p = _PLANS.get(key)
     if p is None:
         args = (dq_out, dk_out, q, k)
