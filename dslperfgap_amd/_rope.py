@@ -205,7 +205,7 @@ def rotate(what, q, k, positions, inv_freq, sections, section_order, pairing, sc
         scale = _number(what, scale, "scale")
     key = (what, q.shape, q.stride(), q.dtype, k.shape, k.stride(), k.dtype, positions.shape,
            positions.stride(), positions.dtype, inv_freq.shape, inv_freq.stride(), inv_freq.dtype,
-           sections, section_order, pairing, scale)
+           sections, section_order, pairing, scale or str(scale))  # -0.0 == 0.0
     p = _PLANS.get(key)
     if p is None:
         qc, kc = _contiguous(q), _contiguous(k)
@@ -238,7 +238,7 @@ def norm_rotate(q, k, q_weight, k_weight, positions, inv_freq, eps, sections, se
     qw, kw = _weights(q_weight, k_weight, q.dtype, what)
     key = (what, q.shape, q.stride(), q.dtype, k.shape, k.stride(), k.dtype, positions.shape,
            positions.stride(), positions.dtype, inv_freq.shape, inv_freq.stride(), inv_freq.dtype,
-           sections, section_order, pairing, scale, eps,
+           sections, section_order, pairing, scale or str(scale), eps,
            None if qw is None else qw.shape, None if kw is None else kw.shape,
            (kw if qw is None else qw) is None or (kw if qw is None else qw).dtype)
     p = _PLANS.get(key)
@@ -271,7 +271,7 @@ def norm_rotate_grads(dq_out, dk_out, q, k, q_weight, k_weight, positions, inv_f
     qw, kw = _weights(q_weight, k_weight, q.dtype, what)
     key = (what, q.shape, q.stride(), q.dtype, k.shape, k.stride(), k.dtype, positions.shape,
            positions.stride(), positions.dtype, inv_freq.shape, inv_freq.stride(), inv_freq.dtype,
-           sections, section_order, pairing, scale, eps,
+           sections, section_order, pairing, scale or str(scale), eps,
            None if qw is None else qw.shape, None if kw is None else kw.shape,
            (kw if qw is None else qw) is None or (kw if qw is None else qw).dtype,
            dq_out.shape, dq_out.stride(), dq_out.dtype, dk_out.shape, dk_out.stride(),

@@ -47,3 +47,14 @@ def test_values_that_equal_right_ones_are_refused_as_before_them(right, wrong, n
             with pytest.raises(TypeError, match=f"{name} must be"):
                 call()
         _planned(pos=pos, **right)
+
+
+def test_scales_of_either_zero_have_plans_of_their_own():
+    """-0 * x and 0 * x differ in the sign of zero."""
+    _rope._PLANS.cache_clear()
+    signs = []
+    for scale in (0.0, -0.0, 0, False):
+        with pytest.raises(ValueError, match="GPU tensors"):
+            rope_fwd(Q, K, POS, FREQ, scale=scale)
+        signs.append(len(_rope._PLANS))
+    assert signs == [1, 2, 2, 2]
