@@ -132,11 +132,11 @@ def make_plan(what, q, k, positions, inv_freq, sections, section_order, pairing,
     d.axes, d.section_order, d.pairing = len(parts), ORDERS[section_order], PAIRINGS[pairing]
     d.dtype, d.w_dtype = _bridge.FLOAT_CODES[q.dtype], _lib.F32
     d.pos_dtype, d.f64_freq = POSITION_CODES[positions.dtype], inv_freq.dtype == torch.float64
-    if not math.isfinite(scale):
-        raise ValueError(f"{what}: scale must be finite, got {scale}")
-    if not (math.isfinite(eps) and eps >= 0.0):
-        raise ValueError(f"{what}: eps must be finite and not negative, got {eps}")
-    d.scale, d.eps = scale, eps
+    d.scale, d.eps = scale, eps  # rounded to 32 bits
+    if not math.isfinite(d.scale):
+        raise ValueError(f"{what}: scale must be finite in 32 bits, got {scale}")
+    if not (math.isfinite(d.eps) and eps >= 0.0):
+        raise ValueError(f"{what}: eps must be finite in 32 bits and not negative, got {eps}")
     if weights is not None:
         for w, name in zip(weights, ("q_weight", "k_weight")):
             if w is None:

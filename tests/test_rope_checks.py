@@ -58,3 +58,18 @@ def test_scales_of_either_zero_have_plans_of_their_own():
             rope_fwd(Q, K, POS, FREQ, scale=scale)
         signs.append(len(_rope._PLANS))
     assert signs == [1, 2, 2, 2]
+
+
+@pytest.mark.parametrize("how,match", [
+    ({"scale": 1e300}, "scale must be finite in 32 bits"),
+    ({"scale": -3.5e38}, "scale must be finite in 32 bits"),
+    ({"eps": 1e300}, "eps must be finite in 32 bits"),
+], ids=str)
+def test_numbers_beyond_32_bits_are_refused_and_leave_no_plan(how, match):
+    _rope._PLANS.cache_clear()
+    for call in _calls(**how):
+        with pytest.raises(ValueError, match=match):
+            call()
+    assert not _rope._PLANS
+    _planned(scale=3.4028234e38)
+    _planned(eps=3.4028234e38)
