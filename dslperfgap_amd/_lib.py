@@ -50,6 +50,7 @@ _f32 = ctypes.c_float
 
 # limits and codes of the rotation (VBH_ROPE_*)
 ROPE_MAX_AXES, ROPE_MAX_DIM = 4, 1024
+ROPE_MAX_HEADS, ROPE_MAX_TOKENS, ROPE_MAX_VALUES = 1 << 16, (1 << 31) - 1, 1 << 46
 ROPE_HALF, ROPE_ADJACENT = 0, 1
 ROPE_BLOCKS, ROPE_CYCLE = 0, 1
 

@@ -106,6 +106,15 @@ def make_plan(what, q, k, positions, inv_freq, sections, section_order, pairing,
     n = inv_freq.shape[0]
     if not 1 <= dim <= _lib.ROPE_MAX_DIM:
         raise ValueError(f"{what}: head_dim must be 1..{_lib.ROPE_MAX_DIM}, got {dim}")
+    heads, tokens = (q.shape[-2], k.shape[-2]), math.prod(lead)
+    if max(heads) > _lib.ROPE_MAX_HEADS:
+        raise ValueError(f"{what}: {names[0]} and {names[1]} may have at most "
+                         f"{_lib.ROPE_MAX_HEADS} heads, got {heads[0]} and {heads[1]}")
+    if tokens > _lib.ROPE_MAX_TOKENS:
+        raise ValueError(f"{what}: fewer than 2^31 tokens are taken, got {tokens}")
+    if tokens * sum(heads) * dim > _lib.ROPE_MAX_VALUES:
+        raise ValueError(f"{what}: {names[0]} and {names[1]} may have at most 2^46 values, got "
+                         f"{tokens * sum(heads) * dim}")
     if not 1 <= n <= dim // 2:
         raise ValueError(f"{what}: inv_freq of {n} does not fit a head_dim of {dim}")
     if section_order not in ORDERS:

@@ -877,11 +877,9 @@ int register_bounds_record(const char* file, BoundsRecordFn fn) {
 }
 #endif
 
-// Limits of the rotation's operands: heads of each side, and the elements from an
-// operand's first to its last (so that byte offsets fit 64 bits with room).
-constexpr int kRopeMaxHeads = 1 << 16;
+// Elements from a rotation operand's first to its last are fewer, so that byte offsets
+// fit 64 bits with room.
 constexpr int64_t kRopeMaxExtent = int64_t(1) << 58;
-constexpr int64_t kRopeMaxValues = int64_t(1) << 46;  // of q and k, beyond any memory
 
 }  // namespace vbh
 
@@ -1544,9 +1542,9 @@ static int rope_args(const vbh_rope_desc* d, const char* what, bool norm, bool g
   if (d->n_freq < 1 || d->n_freq > d->head_dim / 2)
     return fail(VBH_E_INVALID, "%s: %lld frequencies for a head_dim of %lld", what,
                 static_cast<long long>(d->n_freq), static_cast<long long>(d->head_dim));
-  if (d->q_heads > kRopeMaxHeads || d->k_heads > kRopeMaxHeads)
-    return fail(VBH_E_RANGE, "%s: more than %d heads", what, kRopeMaxHeads);
-  if (mul_sat(d->batch, d->seq) > kMaxCols)
+  if (d->q_heads > VBH_ROPE_MAX_HEADS || d->k_heads > VBH_ROPE_MAX_HEADS)
+    return fail(VBH_E_RANGE, "%s: more than %d heads", what, VBH_ROPE_MAX_HEADS);
+  if (mul_sat(d->batch, d->seq) > VBH_ROPE_MAX_TOKENS)
     return fail(VBH_E_RANGE, "%s: 2^31 tokens or more", what);
   if (d->axes < 1 || d->axes > VBH_ROPE_MAX_AXES)
     return fail(VBH_E_INVALID, "%s: %d position axes, 1..%d are taken", what, d->axes,
@@ -1632,7 +1630,7 @@ static int rope_args(const vbh_rope_desc* d, const char* what, bool norm, bool g
     a->seq = static_cast<int>(a->tokens);
     a->batch = 1;
   }
-  if (mul_sat(a->tokens, (d->q_heads + d->k_heads) * d->head_dim) > kRopeMaxValues)
+  if (mul_sat(a->tokens, (d->q_heads + d->k_heads) * d->head_dim) > VBH_ROPE_MAX_VALUES)
     return fail(VBH_E_RANGE, "%s: more than 2^46 values", what);
   return 0;
 }

@@ -6,7 +6,8 @@
 * ``q`` is ``[tokens, q_heads, head_dim]`` or ``[batch, tokens, q_heads, head_dim]``,
   ``k`` the same with its own number of heads; float32, float16 or bfloat16, in any
   strides (a slice of a packed projection, a transposed ``[batch, heads, tokens,
-  head_dim]``).  The outputs are new contiguous tensors of the same shape.
+  head_dim]``).  The outputs are new contiguous tensors of the same shape.  Limits:
+  ``head_dim`` 1024, 65536 heads of each, fewer than 2^31 tokens, 2^46 values in all.
 * The first ``2 n`` values of a head turn, ``n = len(inv_freq)`` (float32 or float64, on
   the GPU); the others pass.  Pair ``p`` turns by ``position * inv_freq[p]``, formed in 64
   bits, so that far positions keep their angles; ``scale`` multiplies what turns.

@@ -259,6 +259,11 @@ int64_t vbh_reduce_workspace_bytes(int64_t outer, int64_t n, int64_t inner, int 
  * 16-byte aligned and apart from the inputs. */
 #define VBH_ROPE_MAX_AXES 4
 #define VBH_ROPE_MAX_DIM 1024
+/* Beyond these, or with strides that are negative or span 2^58 elements or more:
+ * VBH_E_RANGE. */
+#define VBH_ROPE_MAX_HEADS 65536               /* of each of q and k                 */
+#define VBH_ROPE_MAX_TOKENS 2147483647         /* batch * seq                        */
+#define VBH_ROPE_MAX_VALUES (INT64_C(1) << 46) /* of q and k together                */
 
 /* pairing: pair p is values (p, n_freq + p), or (2 p, 2 p + 1) */
 #define VBH_ROPE_HALF 0

@@ -1,11 +1,13 @@
 """What the query / key operators refuse does not depend on the calls before, and is refused
 before anything is allocated."""
 import decimal
+import re
+from pathlib import Path
 
 import pytest
 import torch
 
-from dslperfgap_amd import _rope
+from dslperfgap_amd import _lib, _rope
 from dslperfgap_amd.viperbench.qk_norm_rope.hip_impl import qk_norm_rope_bwd, qk_norm_rope_fwd
 from dslperfgap_amd.viperbench.rope.hip_impl import rope_bwd, rope_fwd
 
@@ -73,3 +75,40 @@ def test_numbers_beyond_32_bits_are_refused_and_leave_no_plan(how, match):
     assert not _rope._PLANS
     _planned(scale=3.4028234e38)
     _planned(eps=3.4028234e38)
+
+
+def _sizes(lead, hq, hk, dim=16):
+    """Operands of any size in one vector of memory."""
+    one = torch.zeros(dim)
+    return {"q": one.expand(*lead, hq, dim), "k": one.expand(*lead, hk, dim),
+            "pos": torch.zeros(1, dtype=torch.int32).expand(lead)}
+
+
+@pytest.mark.parametrize("sizes,match", [
+    (((5,), 65537, 1), "at most 65536 heads"), (((5,), 1, 65537), "at most 65536 heads"),
+    (((1 << 31,), 1, 1), "fewer than 2\\^31 tokens"),
+    (((1 << 16, 1 << 15), 1, 1), "fewer than 2\\^31 tokens"),
+    (((1 << 30,), 1 << 12, 1), "at most 2\\^46 values"),
+], ids=str)
+def test_sizes_beyond_the_kernels_are_refused_and_leave_no_plan(sizes, match):
+    _rope._PLANS.cache_clear()
+    for call in _calls(**_sizes(*sizes)):
+        with pytest.raises(ValueError, match=match):
+            call()
+    assert not _rope._PLANS
+
+
+@pytest.mark.parametrize("sizes", [((5,), 65536, 65536), (((1 << 31) - 1,), 1, 1),
+                                   ((1 << 15, 1 << 15), 4095, 1)], ids=str)
+def test_the_largest_sizes_are_taken(sizes):
+    _planned(**_sizes(*sizes))
+
+
+def test_the_limits_are_the_headers():
+    header = (Path(__file__).parents[1] / "include" / "vbhip.h").read_text()
+    limits = dict(re.findall(r"#define VBH_(ROPE_MAX_\w+) +(\(.*?\) << \d+\)|\d+)", header))
+    assert len(limits) == 5
+    for name, text in limits.items():
+        value = text.replace("INT64_C(1)", "1")
+        a, _, b = value.strip("()").partition(" << ")
+        assert getattr(_lib, name) == int(a) << int(b or 0), name
