@@ -1,1 +1,1 @@
-"""ViperBench/rms_norm: HIP backend (hip_impl)."""
+"""qk_norm_rope: HIP backend (hip_impl)."""

@@ -1,1 +1,1 @@
-"""ViperBench/rms_norm: HIP backend (hip_impl)."""
+"""rope: HIP backend (hip_impl)."""

@@ -1,6 +1,7 @@
 """What the query / key operators refuse does not depend on the calls before, and is refused
 before anything is allocated."""
 import decimal
+import importlib
 import re
 from pathlib import Path
 
@@ -112,3 +113,10 @@ def test_the_limits_are_the_headers():
         value = text.replace("INT64_C(1)", "1")
         a, _, b = value.strip("()").partition(" << ")
         assert getattr(_lib, name) == int(a) << int(b or 0), name
+
+
+@pytest.mark.parametrize("name", ["rope", "qk_norm_rope"])
+def test_packages_say_what_they_hold(name):
+    """Neither is an operator of ViperBench."""
+    doc = importlib.import_module(f"dslperfgap_amd.viperbench.{name}").__doc__
+    assert doc.startswith(name + ":") and "ViperBench" not in doc
