@@ -2,7 +2,8 @@
 //
 // A token has q_heads + k_heads vectors of D values.  A wave takes a share of one
 // token's queries or of its keys, so that the angles are made once (one sincos per
-// lane for 64 pairs, through the LDS) for up to 8 passes over vectors.  In a pass
+// lane for 64 pairs, through the LDS) for up to kRopePasses passes over vectors (the norm's
+// backward: up to kGradShare, kGradPasses of them at a time).  In a pass
 // the wave holds `per_pass` vectors side by side, each lane V consecutive values:
 // the accesses of a pass run over memory without gaps wherever the heads do.  (Both
 // members of every pair in one lane, as two pieces of half the vector each, costs no
@@ -36,7 +37,7 @@ constexpr int kCacheSc1 = 1 << 4;  // cache-policy operand: device scope
 constexpr int kRopeWaves = 4;  // waves per workgroup
 constexpr int kRopeBlock = kRopeWaves * kWave;
 constexpr int kRopePairs = 8;  // pairs of a lane that goes pair by pair
-constexpr int kRopePasses = 4; // passes of a wave's share, at most
+constexpr int kRopePasses = 4; // passes of a wave's share in rope_rows, at most
 
 // How a launch treats memory (rope_mem): kRopeCached, kRopeOnce: nontemporal loads,
 // kRopeStream: nontemporal loads and stores.  All write through the L2 at device scope,
@@ -46,15 +47,14 @@ constexpr int kRopePasses = 4; // passes of a wave's share, at most
 enum RopeMem : int { kRopeCached = 0, kRopeOnce = 1, kRopeStream = 2 };
 
 // What a launch reads and writes, against the 256 MiB cache in front of the memory.
-// MI355X, 16384 tokens of 40 bf16 heads (168 MB in, as much out; three sets of inputs
-// in turn), us by loads / stores, nt: nontemporal, all without the write-through:
-//   forward, 168 MB in and out   nt / nt 55.6, nt / plain 51.8, plain / plain 61.1
-//   the same, 336 MB             nt / nt 108.4, nt / plain 116
-//   the same with the norm, 84 MB nt / plain 29.5, plain / plain 33.2
-//   the same, 42 MB              nt / nt 16.8, nt / plain 16.7, plain / plain 15.1
-//   backward, 336 MB in, 168 out nt / nt 97.0, nt / plain 91.3, plain / plain 105
-//   the same, 168 MB in, 84 out  nt / nt 52.6, nt / plain 50.2, plain / plain 51.2
-//   the same, 84 MB in, 42 out   nt / nt 31.0, nt / plain 31.6, plain / plain 30.6
+// MI355X, tokens of 40 bf16 heads of 128, half pairing, three sets of inputs in turn, us as
+// kRopeCached / kRopeOnce / kRopeStream (backward: twice as much read as written):
+//   tokens, MB written    rotation              norm and rotation     backward
+//   2048, 21               9.2 /  9.2 /  9.5     9.8 / 10.2 / 10.3    20.7 / 22.0 / 22.2
+//   4096, 42              14.8 / 16.1 / 17.2    15.8 / 17.7 / 18.6    31.7 / 31.9 / 33.0
+//   8192, 84              28.1 / 28.0 / 30.1    30.6 / 30.2 / 31.8    50.7 / 49.1 / 52.4
+//   16384, 168            59.9 / 50.4 / 54.8    60.8 / 54.3 / 57.5   102.5 / 85.9 / 93.6
+//   32768, 336           117.4 /106.6 /104.8   114.0 /110.6 /109.4   197.1 /188.4 /180.3
 constexpr int64_t kRopeCachedBytes = int64_t(128) << 20;  // read and written
 constexpr int64_t kRopeOnceBytes = int64_t(224) << 20;    // written
 inline RopeMem rope_mem(int64_t read, int64_t written) {
@@ -376,8 +376,8 @@ struct RopePartners {
       words x;
 #pragma unroll
       for (int i = 0; i < N; ++i)
-        x[i] = __builtin_amdgcn_ds_bpermute(4 * p.lane[i / (N / 2)],
-                                            WAY == kRopeHalves && p.crossed ? w[(i + N / 2) % N] : w[i]);
+        x[i] = __builtin_amdgcn_ds_bpermute(
+            4 * p.lane[i / (N / 2)], WAY == kRopeHalves && p.crossed ? w[(i + N / 2) % N] : w[i]);
       q = __builtin_bit_cast(typename Raw<T, V>::type, x);
     }
 #pragma unroll
@@ -590,7 +590,7 @@ struct RopeOut {
     for (int i = 0; i < V; ++i) r[i] = static_cast<T>(o[i]);
     const int off = there ? at * static_cast<int>(sizeof(T)) : INT_MAX;
     constexpr int N = V * sizeof(T) / 4;
-        constexpr int kAux = MEM == kRopeStream ? kCacheNtSc1 : kCacheSc1;
+    constexpr int kAux = MEM == kRopeStream ? kCacheNtSc1 : kCacheSc1;
     typedef int words __attribute__((ext_vector_type(N)));
     if constexpr (N == 4)
       __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(words, r), rsrc, off, 0, kAux);

@@ -84,9 +84,10 @@ __device__ __forceinline__ void rope_share(const RopeArgs& a, const RopeSide& si
   }
 }
 
-// 6 waves to a SIMD, 80 registers: norm and rotation of 16384 tokens of 40 bf16 heads of
-// 128 take 53.2 us so (54.9 in a later run), 53.9 at 5 waves, 57.0 at 7 and 74 at 8, where registers spill;
-// of 96, adjacent pairs 45.0 and 50.7 at 5.
+// 6 waves to a SIMD, 80 registers.  MI355X, norm and rotation of 16384 tokens of 40 bf16
+// heads, us at 5 / 6 / 7 / 8 waves, in turn: heads of 128, half pairing 53.7 / 54.0 / 54.6 /
+// 69.2 (registers spill at 8), adjacent 54.6 / 51.5 / 51.5 / 50.9; of 96 49.8 / 49.9 / 49.6 /
+// 62.7 and 50.9 / 44.7 / 44.7 / 42.9.  Without the norm all four take the same within 1%.
 template <typename T, int V, bool NORM, bool ADJ, int WAY, int MEM>
 __global__ __launch_bounds__(kRopeBlock, 6) void rope_rows(const RopeArgs) {
   const RopeArgs& a = launch_args();

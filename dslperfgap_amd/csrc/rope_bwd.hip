@@ -377,13 +377,17 @@ __global__ __launch_bounds__(kSumWaves* kWave) void qk_weight_grads(const float*
   store_any<W, 1, false>(out + to, &sum, so);
 }
 
-// Waves of a launch: as many as the card holds at once, 4 to a SIMD (with single passes
-// only, 6 or 8 fit, and 8192 tokens of 40 bf16 heads of 128 take 57.6 and 87.9 us against
-// 48.3); passes beyond which a wave takes more than one of a token's, whose angles it then
-// makes once.  Up to 4 of them where a token's angles take one round of the lanes and
-// vectors lie over a power of two of them without a gap, 8 otherwise.  MI355X, 16384
-// tokens of 40 bf16 heads, us at 2 / 4 / 8: of 128 87.4 / 87.1 / 87.6 (65536 tokens
-// 371 / 367 / 378), 192 94 / 85 / 79, 256 104 / 92 / 91 (both 8192 tokens),
+// Waves of a launch, whatever the kernel: as many as the card holds at once of the 16-bit
+// ones with 16-byte accesses, 4 to a SIMD (with single passes only, 6 or 8 fit, and 8192
+// tokens of 40 bf16 heads of 128 take 57.6 and 87.9 us against 48.3).  5 to 8 would fit of
+// those that hold 59 to 92 registers (accesses of 2 values, one pair to a lane, fp32 with
+// adjacent pairs); of that of eight pairs to a lane 2 or 3 do (136 to 168 registers in
+// fp32, 184 to 200 in 16 bits), and the others wait for a second round.  No counts of
+// their own were tried.  kGradMany: passes beyond which a wave takes more than one of a
+// token's, whose angles it then makes once.  Up to 4 of them where a token's angles take one
+// round of the lanes and vectors lie over a power of two of them without a gap, 8 otherwise.
+// MI355X, 16384 tokens of 40 bf16 heads, us at 2 / 4 / 8: of 128 87.4 / 87.1 / 87.6 (65536
+// tokens 371 / 367 / 378), 192 94 / 85 / 79, 256 104 / 92 / 91 (both 8192 tokens),
 // 100 113 / 109 / 99, 50 97 / 97 / 85, 96 75.6 / 73.9 / 71.8.
 constexpr int64_t kGradWaves = 4096;
 constexpr int64_t kGradMany = 4 * kGradWaves;

@@ -5,7 +5,9 @@ one pass, HIP backend.
 (q_out, k_out)``: each vector of ``head_dim`` values becomes ``x / sqrt(mean(x^2) + eps) *
 weight`` (as ``rms_norm``) and is turned as by ``rope_fwd`` (viperbench/rope, which
 describes ``positions``, ``inv_freq``, ``sections``, ``section_order``, ``pairing``,
-``scale`` and the layouts); fp32 throughout, rounded once.
+``scale`` and the layouts); fp32 throughout, rounded once.  A vector of finite values whose
+squares add up beyond the range of fp32 becomes zeros, as in ``rms_norm``, and so do its
+gradients.
 
 ``qk_norm_rope_bwd(dq_out, dk_out, q, k, q_weight, k_weight, positions, inv_freq, ...) ->
 (dq, dk, dq_weight, dk_weight)`` from the forward's inputs and the gradients of its
