@@ -158,8 +158,9 @@ __global__ __launch_bounds__(kRopeBlock) void rope_values(const RopeArgs a) {
     if (!r.has_a) continue;
     float na = xa[k], nb = xb[k];
     if constexpr (NORM) {
-      na *= size * load_weight<T>(a, side, r.a);
-      nb *= size * (r.has_b ? load_weight<T>(a, side, r.b) : 1.0f);
+      // the vector first: size * weight may leave the range of 32 bits
+      na = na * size * load_weight<T>(a, side, r.a);
+      nb = nb * size * (r.has_b ? load_weight<T>(a, side, r.b) : 1.0f);
     }
     float ya = na, yb = nb;
     if (r.p >= 0) {

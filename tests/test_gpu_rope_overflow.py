@@ -132,3 +132,19 @@ def test_lowest_rows_leave_the_others_as_they_are(tokens, hq, hk, dim, pairing):
         assert int(rows.sum()) > 0 and not bool(outs[0][i][rows].any())
         assert torch.equal(outs[0][i][~rows], outs[1][i][~rows])
         assert torch.equal(outs[0][2 + i], outs[1][2 + i])
+
+
+@pytest.mark.parametrize("pairing,dtype", HOW, ids=str)
+@pytest.mark.parametrize("dim,n", SIZES)
+@pytest.mark.parametrize("size,weight", [(1e-18, 1e22), (1e18, 1e-22)])
+def test_sizes_and_weights_of_which_one_is_large_and_one_small(dim, n, pairing, dtype, size,
+                                                               weight):
+    """1 / sqrt(mean) times the weight is 1e40 or 1e-40, the outputs are 1e22 or 1e-22."""
+    print(f"[gpu] vectors of {size}, weights of {weight}, heads of {dim}, {pairing}, {dtype}",
+          flush=True)
+    x, _, pos, freq, theta, g = _case(dim, n, dtype)
+    x = (x.float() * size).to(dtype)
+    w = (weight * (1 + torch.rand(dim, generator=g))).to(dtype)
+    got = qk_norm_rope_fwd(*[t.to(DEV) for t in (x, x, w, w, pos, freq)], 0.0, pairing=pairing)
+    for out in got:
+        _held(out, *ref.forward(x, theta, pairing, 1.0, w, 0.0), dtype, "forward")
