@@ -70,12 +70,20 @@ __device__ __forceinline__ void write_part(const RopeArgs& a, const float* sums,
   }
 }
 
+// Whether a vector's gradients need sum(dn w u), which has to wait for r, since `dot`,
+// sum(dn w x), leaves the range of 32 bits: it is infinite (or not a number), or the vector
+// so small that terms of dot may be lost below 2^-149.  Those move mean(dn w u) by less than
+// 2^-149 r and du - u mean(dn w u) by that times |u| <= 32: below 2^-24 of a du of 2^-100
+// and more while r <= 2^20, where any eps of 2^-40 and more keeps it.
+__device__ __forceinline__ bool needs_unit_sum(float dot, float r) {
+  return past_range(dot) || r > 0x1p20f;
+}
+
 // The wave's share of its tokens, U passes at a time (MORE: more than once); dw: the
-// lane's sums.  True if a vector's sum(dn w x) passes the range of 32 bits, which that of
-// dn w u need not, but the latter has to wait for r: AGAIN goes over the share once more
-// and stores such vectors' gradients, by the latter sum.  (Apart from the first time, whose
-// registers it leaves alone: 16384 tokens of 40 bf16 heads of 128, half pairing, 86.2 us,
-// as without a second sum; with it in place 93.)
+// lane's sums.  True if a vector needs_unit_sum: AGAIN goes over the share once more and
+// stores such vectors' gradients.  (Apart from the first time, whose registers it leaves
+// alone: 16384 tokens of 40 bf16 heads of 128, half pairing, 86.2 us, as without a second
+// sum; with it in place 93.)
 template <typename T, int V, int U, bool MORE, bool AGAIN, bool ADJ, int WAY, int MEM>
 __device__ __forceinline__ bool grad_share(const RopeArgs& a, const RopeSide& side,
                                            const RopeLane& l, int chunk, int first,
@@ -97,7 +105,7 @@ __device__ __forceinline__ bool grad_share(const RopeArgs& a, const RopeSide& si
   const int64_t x_step = a.tile.per_pass * side.xs[2], g_step = a.tile.per_pass * side.gs[2];
   const int to = (head0 + l.sub) * a.dim + l.at * V, y_step = a.tile.per_pass * a.dim;
   const RopeAngles angles(a);
-  bool over = false;
+  bool again = false;
 
   for (int64_t token = first; token < a.tokens; token += side.walkers) {
     const RopeToken t = rope_token(a, token);
@@ -154,29 +162,30 @@ __device__ __forceinline__ bool grad_share(const RopeArgs& a, const RopeSide& si
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         const float r = ok[u] ? inverse_root(fmaf(sums[2 * u], inv_dim, a.eps)) : 0.0f;
-        float mean = sums[2 * u + 1] * r * inv_dim * r;
-        const bool past = ok[u] && past_range(sums[2 * u + 1]);
-        over = over || past;
+        float mean = sums[2 * u + 1] * r * inv_dim;
+        const bool needs = ok[u] && needs_unit_sum(sums[2 * u + 1], r);
+        again = again || needs;
         if constexpr (AGAIN) {
           float dot[1] = {0.0f};
 #pragma unroll
           for (int i = 0; i < V; ++i)
             dot[0] = fmaf(dn[u][i] * w[i], raw_at<T, V>(x[u], i) * r, dot[0]);
           vector_sums<1>(a, l, dot, scratch);
-          mean = dot[0] * inv_dim * r;
+          mean = dot[0] * inv_dim;
         }
         float o[V];
 #pragma unroll
         for (int i = 0; i < V; ++i) {
           const float unit = raw_at<T, V>(x[u], i) * r;
           if constexpr (!AGAIN) dw[i] = fmaf(dn[u][i], unit, dw[i]);
-          o[i] = fmaf(dn[u][i] * r, w[i], -unit * mean);
+          // r last: dn r, like dn w x, may leave the range of 32 bits
+          o[i] = r * fmaf(dn[u][i], w[i], -unit * mean);
         }
-        out.store(to + (pass + u) * y_step, AGAIN ? past : ok[u], o);
+        out.store(to + (pass + u) * y_step, AGAIN ? needs : ok[u], o);
       }
     }
   }
-  return over;
+  return again;
 }
 
 template <typename T, int V, bool ADJ, int WAY, int MEM>
@@ -193,17 +202,17 @@ __global__ __launch_bounds__(kRopeBlock, 4) void qk_norm_rope_grads(const RopeAr
 #pragma unroll
   for (int i = 0; i < V; ++i) dw[i] = 0.0f;
   if (walk.live) {
-    bool over;
+    bool again;
     if (side.per_wave == 1)
-      over = grad_share<T, V, 1, false, false, ADJ, WAY, MEM>(a, side, l, walk.chunk, walk.token,
+      again = grad_share<T, V, 1, false, false, ADJ, WAY, MEM>(a, side, l, walk.chunk, walk.token,
                                                               lds, dw);
     else if (side.per_wave == kGradPasses)
-      over = grad_share<T, V, kGradPasses, false, false, ADJ, WAY, MEM>(a, side, l, walk.chunk,
+      again = grad_share<T, V, kGradPasses, false, false, ADJ, WAY, MEM>(a, side, l, walk.chunk,
                                                                         walk.token, lds, dw);
     else
-      over = grad_share<T, V, kGradPasses, true, false, ADJ, WAY, MEM>(a, side, l, walk.chunk,
+      again = grad_share<T, V, kGradPasses, true, false, ADJ, WAY, MEM>(a, side, l, walk.chunk,
                                                                        walk.token, lds, dw);
-    if (__builtin_expect(wave_any(over), 0))
+    if (__builtin_expect(wave_any(again), 0))
       grad_share<T, V, 1, true, true, ADJ, WAY, MEM>(a, side, l, walk.chunk, walk.token, lds, dw);
   }
   if (parts == nullptr) return;
@@ -270,7 +279,8 @@ __global__ __launch_bounds__(kRopeBlock) void qk_norm_rope_value_grads(const Rop
     vector_sums<2>(a, l, sums, nullptr);
     const float size = inverse_root(fmaf(sums[0], inv_dim, a.eps));
     float mean = sums[1] * size * inv_dim;
-    if (__builtin_expect(wave_any(ok && past_range(sums[1])), 0)) {  // as in grad_share
+    const bool needs = ok && needs_unit_sum(sums[1], size);
+    if (__builtin_expect(wave_any(needs), 0)) {
       float dot[1] = {0.0f};
 #pragma unroll
       for (int k = 0; k < K; ++k) {
@@ -281,7 +291,7 @@ __global__ __launch_bounds__(kRopeBlock) void qk_norm_rope_value_grads(const Rop
           dot[0] = fmaf(nb[k] * load_weight<T>(a, side, r.b), xb[k] * size, dot[0]);
       }
       vector_sums<1>(a, l, dot, nullptr);
-      if (past_range(sums[1])) mean = dot[0] * inv_dim;
+      if (needs) mean = dot[0] * inv_dim;
     }
 #pragma unroll
     for (int k = 0; k < K; ++k) {

@@ -148,3 +148,25 @@ def test_sizes_and_weights_of_which_one_is_large_and_one_small(dim, n, pairing, 
     got = qk_norm_rope_fwd(*[t.to(DEV) for t in (x, x, w, w, pos, freq)], 0.0, pairing=pairing)
     for out in got:
         _held(out, *ref.forward(x, theta, pairing, 1.0, w, 0.0), dtype, "forward")
+
+
+@pytest.mark.parametrize("pairing,dtype", HOW, ids=str)
+@pytest.mark.parametrize("dim,n", SIZES)
+@pytest.mark.parametrize("size,gradient,weight", [
+    (1e-18, 1e-26, 1.0),   # sum(dn w x) is 1e-42, mean(dn w u) 1e-26
+    (1e-18, 1e-29, 1.0),   # its terms are 1e-47, less than the smallest number
+    (1e-18, 1e22, 1e-22),  # dn / sqrt(mean) is 1e40, the gradients are 1e18
+    (1e18, 1e-22, 1e20),   # dn / sqrt(mean) is 1e-40, the gradients are 1e-20
+])
+def test_gradients_of_large_and_small_parts(dim, n, pairing, dtype, size, gradient, weight):
+    print(f"[gpu] vectors of {size}, gradients of {gradient}, weights of {weight}, heads of "
+          f"{dim}, {pairing}, {dtype}", flush=True)
+    x, dy, pos, freq, theta, g = _case(dim, n, dtype)
+    x, dy = (x.float() * size).to(dtype), (dy.float() * gradient).to(dtype)
+    w = (weight * (1 + torch.rand(dim, generator=g))).to(dtype)
+    got = qk_norm_rope_bwd(*[t.to(DEV) for t in (dy, dy, x, x, w, w, pos, freq)], 0.0,
+                           pairing=pairing)
+    dx, dw, bx, bw = ref.backward(dy, x, theta, pairing, 1.0, w, 0.0)
+    for i in (0, 1):
+        _held(got[i], dx, bx, dtype, "backward")
+        _held(got[2 + i], dw, bw, dtype, "weight")
