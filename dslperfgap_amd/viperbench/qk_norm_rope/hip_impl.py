@@ -7,7 +7,8 @@ weight`` (as ``rms_norm``) and is turned as by ``rope_fwd`` (viperbench/rope, wh
 describes ``positions``, ``inv_freq``, ``sections``, ``section_order``, ``pairing``,
 ``scale`` and the layouts); fp32 throughout, rounded once.  A vector of finite values whose
 squares add up beyond the range of fp32 becomes zeros, as in ``rms_norm``, and so do its
-gradients.
+gradients; with ``eps`` 0 one whose squares are all 0 in fp32 (values below 2^-75) has no
+finite output.
 
 ``qk_norm_rope_bwd(dq_out, dk_out, q, k, q_weight, k_weight, positions, inv_freq, ...) ->
 (dq, dk, dq_weight, dk_weight)`` from the forward's inputs and the gradients of its
