@@ -72,6 +72,9 @@ SIGNATURES = {
     "vbh_last_error": (ctypes.c_char_p, []),
     "vbh_layer_norm_fwd": (_i32, [_vp, _vp, _vp, _vp, _i64, _i64, _f32, _i32, _i32, _vp]),
     "vbh_rms_norm_fwd": (_i32, [_vp, _vp, _vp, _i64, _i64, _f32, _i32, _i32, _vp]),
+    "vbh_layer_norm_bwd": (_i32, [_vp] * 6 + [_i64, _i64, _f32, _i32, _i32, _vp, _i64, _vp]),
+    "vbh_rms_norm_bwd": (_i32, [_vp] * 5 + [_i64, _i64, _f32, _i32, _i32, _vp, _i64, _vp]),
+    "vbh_norm_bwd_workspace_bytes": (_i64, [_i64, _i64, _i32, _i32]),
     "vbh_softmax_fwd": (_i32, [_vp, _vp, _i64, _i64, _i32, _i32, _i32, _vp]),
     "vbh_softmax_fwd_ws": (_i32, [_vp, _vp, _i64, _i64, _i32, _i32, _i32, _vp, _i64, _vp]),
     "vbh_softmax_workspace_bytes": (_i64, [_i64, _i64, _i32]),
@@ -120,7 +123,8 @@ SIGNATURES = {
 
 # entry points _vbhfast binds (every launching one)
 FAST_ENTRY_POINTS = (
-    "vbh_layer_norm_fwd", "vbh_rms_norm_fwd", "vbh_softmax_fwd", "vbh_softmax_fwd_ws",
+    "vbh_layer_norm_fwd", "vbh_rms_norm_fwd", "vbh_layer_norm_bwd", "vbh_rms_norm_bwd",
+    "vbh_softmax_fwd", "vbh_softmax_fwd_ws",
     "vbh_softmax_dim_fwd",
     "vbh_logsumexp_fwd", "vbh_logsumexp_fwd_ws", "vbh_cross_entropy_fwd",
     "vbh_cross_entropy_fwd_ws", "vbh_cross_entropy_fwd_noalloc", "vbh_cross_entropy_bwd",

@@ -967,6 +967,66 @@ int vbh_rms_norm_fwd(const void* x, const void* w, void* y, int64_t rows, int64_
                     "rms_norm launch");
 }
 
+// The gradients of both norms (`db` and `ln` with LayerNorm only).
+static int norm_bwd(const char* what, bool ln, const void* dy, const void* x, const void* w,
+                    void* dx, void* dw, void* db, int64_t rows, int64_t cols, float eps,
+                    int dtype, int w_dtype, void* workspace, int64_t workspace_bytes,
+                    void* stream) {
+  if (!is_float(dtype)) return fail(VBH_E_DTYPE, "%s: unsupported dtype %d", what, dtype);
+  if (w_dtype != dtype && w_dtype != kF32)
+    return fail(VBH_E_DTYPE, "%s: weight dtype %d must equal x dtype %d or be fp32", what,
+                w_dtype, dtype);
+  if (rows < 0 || cols < 0 || workspace_bytes < 0)
+    return fail(VBH_E_INVALID, "%s: negative size", what);
+  if (cols > kMaxCols) return fail(VBH_E_RANGE, "%s: cols %lld too large", what,
+                                   static_cast<long long>(cols));
+  if (rows > kMaxWorkItems / kMaxBlock || mul_sat(rows, cols) > VBH_NORM_BWD_MAX_VALUES)
+    return fail(VBH_E_RANGE, "%s: %lld x %lld values are more than one launch takes", what,
+                static_cast<long long>(rows), static_cast<long long>(cols));
+  if (cols == 0) return 0;
+  if (rows > 0 && (!dy || !x || !w || !dx)) return fail(VBH_E_INVALID, "%s: null pointer", what);
+  const bool sums = dw != nullptr || db != nullptr;
+  if (rows == 0 && !sums) return 0;
+  const int64_t need = vbh_norm_bwd_workspace_bytes(rows, cols, dtype, ln);
+  if (norm_bwd_needs_workspace(rows, cols, dtype, sums) &&
+      (!workspace || workspace_bytes < need || !aligned16(workspace)))
+    return fail(VBH_E_INVALID, "%s: needs an aligned workspace of %lld bytes", what,
+                static_cast<long long>(need));
+  NormGradArgs a;
+  a.x = x;
+  a.dy = dy;
+  a.w = w;
+  a.dx = dx;
+  a.rows = rows;
+  a.cols = static_cast<int>(cols);
+  a.eps = eps;
+  return hip_status(launch_norm_bwd(a, ln, dtype, w_dtype, dw, db, static_cast<float*>(workspace),
+                                    static_cast<hipStream_t>(stream)),
+                    what);
+}
+
+int64_t vbh_norm_bwd_workspace_bytes(int64_t rows, int64_t cols, int dtype, int layer_norm) {
+  if (!is_float(dtype) || rows < 0 || cols <= 0 || cols > kMaxCols ||
+      mul_sat(rows, cols) > VBH_NORM_BWD_MAX_VALUES)
+    return 0;
+  return static_cast<int64_t>(sizeof(float)) *
+         norm_bwd_workspace_floats(rows, cols, dtype, layer_norm != 0);
+}
+
+int vbh_layer_norm_bwd(const void* dy, const void* x, const void* w, void* dx, void* dw, void* db,
+                       int64_t rows, int64_t cols, float eps, int dtype, int w_dtype,
+                       void* workspace, int64_t workspace_bytes, void* stream) {
+  return norm_bwd("layer_norm_bwd", true, dy, x, w, dx, dw, db, rows, cols, eps, dtype, w_dtype,
+                  workspace, workspace_bytes, stream);
+}
+
+int vbh_rms_norm_bwd(const void* dy, const void* x, const void* w, void* dx, void* dw,
+                     int64_t rows, int64_t cols, float eps, int dtype, int w_dtype,
+                     void* workspace, int64_t workspace_bytes, void* stream) {
+  return norm_bwd("rms_norm_bwd", false, dy, x, w, dx, dw, nullptr, rows, cols, eps, dtype,
+                  w_dtype, workspace, workspace_bytes, stream);
+}
+
 static bool softmax_pair_ok(int idt, int odt) {
   if (!is_float(idt) || !is_float(odt)) return false;
   return idt == odt || (odt == kF32 && idt != kF32);

@@ -374,6 +374,29 @@ int64_t rope_bwd_part_floats(const RopeArgs& a, int dt, bool adjacent);
 hipError_t launch_qk_norm_rope_bwd(const RopeArgs& a, int dt, bool adjacent, void* dq_weight,
                                    void* dk_weight, float* parts, hipStream_t s);
 
+// Gradients of LayerNorm and RMSNorm (norm_bwd.hip).  x, dy, dx: [rows, cols]
+// contiguous, w: [cols].
+struct NormGradArgs {
+  const void* x = nullptr;
+  const void* dy = nullptr;
+  const void* w = nullptr;
+  void* dx = nullptr;
+  int64_t rows = 0;
+  int cols = 0;
+  float eps = 0.0f;
+  // set by the launcher
+  int tpr = 64;                       // lanes per row
+  float* parts = nullptr;             // [part_rows][pitch]: dw's rows, then db's
+  int64_t part_rows = 0, pitch = 0;
+};
+// Floats of the launcher's workspace (16-byte aligned), and whether the launch needs it
+// (`sums`: with the weights' gradients).
+int64_t norm_bwd_workspace_floats(int64_t rows, int64_t cols, int dt, bool ln);
+bool norm_bwd_needs_workspace(int64_t rows, int64_t cols, int dt, bool sums);
+// dw, db: [cols] of type `wdt`, each null where not wanted (db with ln only).
+hipError_t launch_norm_bwd(NormGradArgs a, bool ln, int dt, int wdt, void* dw, void* db,
+                           float* workspace, hipStream_t stream);
+
 // Reduction over the middle axis.  With c.segs > 1, `parts` holds
 // outer * inner * segs fp32 results, and as many int32 rows for max / argmax.
 hipError_t launch_reduce_cols(const void* x, void* vals, int64_t* idx, void* parts,

@@ -101,6 +101,12 @@ ENTRY(vbh_layer_norm_fwd, "ppppqqfiip",
       fn_vbh_layer_norm_fwd(P(0), P(1), P(2), P(3), Q(4), Q(5), F(6), I(7), I(8), P(9)))
 ENTRY(vbh_rms_norm_fwd, "pppqqfiip",
       fn_vbh_rms_norm_fwd(P(0), P(1), P(2), Q(3), Q(4), F(5), I(6), I(7), P(8)))
+ENTRY(vbh_layer_norm_bwd, "ppppppqqfiipqp",
+      fn_vbh_layer_norm_bwd(P(0), P(1), P(2), P(3), P(4), P(5), Q(6), Q(7), F(8), I(9), I(10),
+                            P(11), Q(12), P(13)))
+ENTRY(vbh_rms_norm_bwd, "pppppqqfiipqp",
+      fn_vbh_rms_norm_bwd(P(0), P(1), P(2), P(3), P(4), Q(5), Q(6), F(7), I(8), I(9), P(10),
+                          Q(11), P(12)))
 ENTRY(vbh_softmax_fwd, "ppqqiiip",
       fn_vbh_softmax_fwd(P(0), P(1), Q(2), Q(3), I(4), I(5), I(6), P(7)))
 ENTRY(vbh_softmax_fwd_ws, "ppqqiiipqp",
@@ -158,7 +164,7 @@ static const struct {
     SLOT(vbh_reduce_fwd),
     SLOT(vbh_reduce_fwd_ws),     SLOT(vbh_stream_copy),      SLOT(vbh_stream_read),
     SLOT(vbh_rope_fwd),          SLOT(vbh_rope_bwd),         SLOT(vbh_qk_norm_rope_fwd),
-    SLOT(vbh_qk_norm_rope_bwd),
+    SLOT(vbh_qk_norm_rope_bwd),  SLOT(vbh_layer_norm_bwd),   SLOT(vbh_rms_norm_bwd),
 };
 #define N_SLOTS (sizeof(slots) / sizeof(slots[0]))
 
@@ -197,7 +203,7 @@ static PyMethodDef methods[] = {
     METHOD(vbh_cross_entropy_bwd), METHOD(vbh_reduce_fwd),
     METHOD(vbh_reduce_fwd_ws),     METHOD(vbh_stream_copy),       METHOD(vbh_stream_read),
     METHOD(vbh_rope_fwd),          METHOD(vbh_rope_bwd),          METHOD(vbh_qk_norm_rope_fwd),
-    METHOD(vbh_qk_norm_rope_bwd),
+    METHOD(vbh_qk_norm_rope_bwd),  METHOD(vbh_layer_norm_bwd),    METHOD(vbh_rms_norm_bwd),
     {NULL, NULL, 0, NULL},
 };
 

@@ -6,6 +6,10 @@ trailing ``weight.shape`` dims, same shape and dtype as ``x``.
 
 One read of x and one write of y per call (libvbhip ``vbh_layer_norm_fwd``);
 launched on torch's current stream, no host synchronisation.
+
+``layer_norm_bwd(dy, x, weight, bias, eps=1e-5) -> (dx, dweight, dbias)``, its gradients
+from the forward's inputs and the gradient of its output: two reads and one write of the
+rows (``vbh_layer_norm_bwd``).  No reference counterpart (its layer_norm is forward only).
 """
 import os
 import sys
@@ -16,7 +20,7 @@ if _ROOT not in sys.path:  # loadable by file path, as ViperBench's harness load
 
 import torch  # noqa: E402
 
-from dslperfgap_amd import _bridge, _lib  # noqa: E402
+from dslperfgap_amd import _bridge, _lib, _norm_bwd  # noqa: E402
 
 
 def layer_norm(x, weight, bias, eps=1e-5):
@@ -86,3 +90,32 @@ def _plan(x, weight, bias):
         return False
     cols = weight.shape[0]
     return (x.numel() // cols if cols else 0, cols, code, _lib.entry("vbh_layer_norm_fwd"))
+
+
+def layer_norm_bwd(dy, x, weight, bias, eps=1e-5):
+    """The gradients of layer_norm's x, weight and bias from that of its output (x's shape
+    and dtype).  ``bias`` is only asked whether there is one: its gradient is None without.
+    The weights' gradients are summed in fp32 in a fixed order and have the weights' dtype.
+    """
+    if eps != 1e-5:
+        raise ValueError(f"Only eps=1e-5 is supported (got {eps}). "
+                         "The Triton kernel hardcodes eps=1e-5.")
+    what = "layer_norm_bwd"
+    norm_shape = tuple(weight.shape)
+    k = len(norm_shape)
+    if x.dim() < k or tuple(x.shape[x.dim() - k:]) != norm_shape:
+        raise RuntimeError(f"{what}: normalized_shape {list(norm_shape)} does not match "
+                           f"the trailing dims of input {list(x.shape)}")
+    if bias is not None:
+        if bias.shape != weight.shape:
+            raise RuntimeError(f"{what}: bias shape {list(bias.shape)} != {list(norm_shape)}")
+        if bias.dtype != weight.dtype:
+            raise TypeError(f"{what}: weight and bias dtypes differ")
+    if weight.dtype != x.dtype and weight.dtype != torch.float32:
+        raise TypeError(f"{what}: weight dtype {weight.dtype} must be {x.dtype} or float32")
+    dev, dx, dw, args = _norm_bwd.prepare(what, dy, x, weight, bias, eps, True)
+    db = None if bias is None else _bridge.empty(weight, weight.shape)
+    dy, x, weight, rest = args
+    _bridge.launch("vbh_layer_norm_bwd", dev, dy.data_ptr(), x.data_ptr(), weight.data_ptr(),
+                   dx.data_ptr(), dw.data_ptr(), _bridge.ptr(db), *rest)
+    return dx, dw, db

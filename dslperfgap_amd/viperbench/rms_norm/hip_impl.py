@@ -6,6 +6,10 @@ the last ``len(normalized_shape)`` dims:
 ``((x.float() / sqrt(mean(x.float()**2) + eps)) * weight.float()).to(x.dtype)``.
 
 One read of x and one write of y per call (libvbhip ``vbh_rms_norm_fwd``).
+
+``rms_norm_bwd(dy, x, normalized_shape, weight, eps=1e-5) -> (dx, dweight)``, its gradients
+from the forward's inputs and the gradient of its output: two reads and one write of the
+rows (``vbh_rms_norm_bwd``).  No reference counterpart (its rms_norm is forward only).
 """
 import os
 import sys
@@ -16,7 +20,7 @@ if _ROOT not in sys.path:
 
 import torch  # noqa: E402
 
-from dslperfgap_amd import _bridge, _lib  # noqa: E402
+from dslperfgap_amd import _bridge, _lib, _norm_bwd  # noqa: E402
 
 
 def rms_norm(x, normalized_shape, weight, eps=1e-5):
@@ -75,3 +79,27 @@ def _plan(shape, dtype, wshape, wdtype):
     cols = int(shape[-1])
     return (_bridge.numel_prod(shape) // cols, cols, code, _bridge.FLOAT_CODES[wdtype],
             _lib.entry("vbh_rms_norm_fwd"))
+
+
+def rms_norm_bwd(dy, x, normalized_shape, weight, eps=1e-5):
+    """The gradients of rms_norm's x and weight from that of its output (x's shape and
+    dtype).  The weight's gradient is summed in fp32 in a fixed order and has the weight's
+    shape and dtype."""
+    what = "rms_norm_bwd"
+    k = len(tuple(normalized_shape))
+    if k > x.dim():
+        raise RuntimeError(f"{what}: normalized_shape {tuple(normalized_shape)} has more dims "
+                           f"than input {list(x.shape)}")
+    cols = _bridge.numel_prod(x.shape[x.dim() - k:])
+    if weight.numel() != cols:
+        raise RuntimeError(f"{what}: weight has {weight.numel()} elements, the normalized "
+                           f"dims hold {cols}")
+    if not (float(eps) >= 0.0 and float(eps) < float("inf")):
+        raise ValueError(f"{what}: eps must be finite and not negative, got {eps}")
+    wide = weight.dtype in (x.dtype, torch.float32)
+    dev, dx, dw, args = _norm_bwd.prepare(what, dy, x, weight if wide else weight.float(), None,
+                                          eps, False)
+    dy, x, w, rest = args
+    _bridge.launch("vbh_rms_norm_bwd", dev, dy.data_ptr(), x.data_ptr(), w.data_ptr(),
+                   dx.data_ptr(), dw.data_ptr(), *rest)
+    return dx, dw if wide else dw.to(weight.dtype)

@@ -75,6 +75,29 @@ int vbh_rms_norm_fwd(const void* x, const void* w, void* y,
                      int64_t rows, int64_t cols, float eps,
                      int dtype, int w_dtype, void* stream);
 
+/* Gradients of vbh_layer_norm_fwd and vbh_rms_norm_fwd.  With u = (x - mean) r,
+ * r = 1 / sqrt(var + eps) (RMSNorm: mean 0, the mean of squares), g = dy w:
+ *   dx = r (g - mean(g) - u mean(g u))  (RMSNorm: without mean(g)),
+ *   dw = sum over rows of dy u,  db = sum over rows of dy.
+ * u is formed again from x: the forward keeps nothing.  dy, x, dx: [rows, cols] of
+ * `dtype`; w, dw, db: [cols] of `w_dtype` (`dtype` or F32); dw, db may be null (not
+ * wanted).  fp32 throughout, rounded once; the sums over rows in a fixed order,
+ * through a workspace of vbh_norm_bwd_workspace_bytes bytes (16-byte aligned scratch
+ * of this call, stream-ordered; not looked at where that is not needed: rows held in
+ * registers without dw and db).  No rows: dw and db become zeros.
+ * More than VBH_NORM_BWD_MAX_VALUES values, or 2^22 rows: VBH_E_RANGE.
+ * No reference counterpart (ViperBench/layer_norm and rms_norm are forward only). */
+#define VBH_NORM_BWD_MAX_VALUES (INT64_C(1) << 46)
+int vbh_layer_norm_bwd(const void* dy, const void* x, const void* w, void* dx, void* dw, void* db,
+                       int64_t rows, int64_t cols, float eps, int dtype, int w_dtype,
+                       void* workspace, int64_t workspace_bytes, void* stream);
+int vbh_rms_norm_bwd(const void* dy, const void* x, const void* w, void* dx, void* dw,
+                     int64_t rows, int64_t cols, float eps, int dtype, int w_dtype,
+                     void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Workspace bytes of those calls, a pure function of the arguments (0 for invalid ones). */
+int64_t vbh_norm_bwd_workspace_bytes(int64_t rows, int64_t cols, int dtype, int layer_norm);
+
 /* Softmax (log_mode = 0) or log-softmax (log_mode = 1) over the last axis.
  * x: [rows, cols] of `in_dtype`; y: [rows, cols] of `out_dtype`.
  * Supported (in, out): (F32,F32) (F16,F16) (BF16,BF16) (F16,F32) (BF16,F32).
