@@ -103,6 +103,11 @@ SIGNATURES = {
         [_vp, _vp, _vp, _vp, _vp, _i32, _i32, _i64, _i64, _i64, _i64, _i64, _f32, _f32, _f32,
          _i64, _i64, _i64, _i32, _vp],
     ),
+    "vbh_linear_cross_entropy_fwd": (
+        _i32, [_vp] * 6 + [_i64] * 5 + [_f32] * 3 + [_i64] * 3 + [_i32] * 3 + [_vp, _i64, _vp]),
+    "vbh_linear_cross_entropy_bwd": (
+        _i32, [_vp] * 7 + [_i64] * 5 + [_f32] * 3 + [_i64] * 3 + [_i32] * 2 + [_vp, _i64, _vp]),
+    "vbh_linear_cross_entropy_workspace_bytes": (_i64, [_i64] * 3 + [_i32] * 3),
     "vbh_reduce_fwd": (_i32, [_vp, _vp, _vp, _i64, _i64, _i64, _i32, _i32, _i32, _vp]),
     "vbh_reduce_fwd_ws": (_i32, [_vp, _vp, _vp, _i64, _i64, _i64, _i32, _i32, _i32, _vp, _i64,
                                  _vp]),
@@ -128,6 +133,7 @@ FAST_ENTRY_POINTS = (
     "vbh_softmax_dim_fwd",
     "vbh_logsumexp_fwd", "vbh_logsumexp_fwd_ws", "vbh_cross_entropy_fwd",
     "vbh_cross_entropy_fwd_ws", "vbh_cross_entropy_fwd_noalloc", "vbh_cross_entropy_bwd",
+    "vbh_linear_cross_entropy_fwd", "vbh_linear_cross_entropy_bwd",
     "vbh_reduce_fwd", "vbh_reduce_fwd_ws", "vbh_rope_fwd", "vbh_rope_bwd",
     "vbh_qk_norm_rope_fwd", "vbh_qk_norm_rope_bwd", "vbh_stream_copy", "vbh_stream_read",
 )

@@ -391,6 +391,12 @@ Geometry geometry_for(int op, int64_t cols, int vec, int64_t units, int64_t out_
   return g;
 }
 
+// The products' loads take rows of `hidden` values as whole 16-byte pieces, at offsets of up to
+// 256 rows from a tile's first; others are copied for them.
+bool linear_ce_direct(const void* p, int64_t stride, int64_t hidden, int64_t e) {
+  return aligned16(p) && stride * e % 16 == 0 && hidden * e % 16 == 0 && stride * e <= (1 << 20);
+}
+
 constexpr int64_t kMaxCols = (int64_t(1) << 31) - 1;
 constexpr int64_t kMaxWorkItems = (int64_t(1) << 32) - 1;
 
@@ -1480,6 +1486,127 @@ int vbh_cross_entropy_bwd(const void* dloss, const void* logits, const void* lse
   a.wt = a.nt && wt;
   return hip_status(launch_cross_entropy_bwd(a, static_cast<hipStream_t>(stream)),
                     "cross_entropy_bwd launch");
+}
+
+// What both directions of the projection's cross entropy check; fills `a` but for the pointers
+// of one direction.
+static int linear_ce_args(const char* what, LceArgs* a, const void* x, const void* w,
+                          const void* labels, int64_t tokens, int64_t hidden, int64_t vocab,
+                          int64_t x_stride, int64_t w_stride, float smoothing, float logit_scale,
+                          float lse_square_scale, int64_t ignored_index, int64_t total_classes,
+                          int64_t class_start_idx, int dtype, int label_dtype) {
+  if (!is_float(dtype)) return fail(VBH_E_DTYPE, "%s: unsupported dtype %d", what, dtype);
+  if (label_dtype != kI32 && label_dtype != kI64)
+    return fail(VBH_E_DTYPE, "%s: labels must be int32 or int64", what);
+  if (tokens < 0 || hidden < 1 || vocab < 1)
+    return fail(VBH_E_INVALID, "%s: negative size, or no hidden values or classes", what);
+  if (tokens > VBH_LINEAR_CE_MAX_TOKENS || hidden > VBH_LINEAR_CE_MAX_HIDDEN ||
+      vocab > VBH_LINEAR_CE_MAX_VOCAB || mul_sat(vocab, hidden) > VBH_LINEAR_CE_MAX_WEIGHTS)
+    return fail(VBH_E_RANGE, "%s: %lld tokens x %lld hidden x %lld classes is out of range", what,
+                static_cast<long long>(tokens), static_cast<long long>(hidden),
+                static_cast<long long>(vocab));
+  if (x_stride < hidden || w_stride < hidden)
+    return fail(VBH_E_INVALID, "%s: a row stride below hidden", what);
+  if (x_stride > VBH_LINEAR_CE_MAX_STRIDE || w_stride > VBH_LINEAR_CE_MAX_STRIDE)
+    return fail(VBH_E_RANGE, "%s: row stride too large", what);
+  if (total_classes < 1) return fail(VBH_E_INVALID, "%s: total_classes must be positive", what);
+  if (class_start_idx < 0) return fail(VBH_E_INVALID, "%s: class_start_idx is negative", what);
+  if (tokens > 0 && (!x || !w || !labels)) return fail(VBH_E_INVALID, "%s: null pointer", what);
+  const int64_t e = elt_size(dtype);
+  a->x = x;
+  a->labels = labels;
+  a->tokens = tokens;
+  a->hidden = hidden;
+  a->vocab = vocab;
+  a->x_stride = x_stride;
+  a->x_direct = linear_ce_direct(x, x_stride, hidden, e);
+  if (linear_ce_direct(w, w_stride, hidden, e)) {
+    a->w = w;
+    a->w_stride = w_stride;
+  } else {
+    a->w_given = w;
+    a->w_given_stride = w_stride;
+  }
+  a->ignored = ignored_index;
+  a->class_start = class_start_idx;
+  a->total_classes = static_cast<float>(total_classes);
+  a->smoothing = smoothing;
+  a->scale = logit_scale;
+  a->lse_square_scale = lse_square_scale;
+  a->label_i64 = label_dtype == kI64;
+  return 0;
+}
+
+static int linear_ce_workspace_ok(const char* what, const LceArgs& a, int dtype, bool backward,
+                                  const void* workspace, int64_t workspace_bytes) {
+  const int64_t need = linear_ce_workspace_bytes(a.tokens, a.hidden, a.vocab, dtype,
+                                                 a.w == nullptr, backward);
+  if (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 255u) != 0)
+    return fail(VBH_E_INVALID, "%s: needs a workspace of %lld bytes, aligned to 256", what,
+                static_cast<long long>(need));
+  return 0;
+}
+
+int64_t vbh_linear_cross_entropy_workspace_bytes(int64_t tokens, int64_t hidden, int64_t vocab,
+                                                 int dtype, int pad_weight, int backward) {
+  if (!is_float(dtype) || tokens <= 0 || hidden <= 0 || vocab <= 0 ||
+      tokens > VBH_LINEAR_CE_MAX_TOKENS || hidden > VBH_LINEAR_CE_MAX_HIDDEN ||
+      vocab > VBH_LINEAR_CE_MAX_VOCAB || mul_sat(vocab, hidden) > VBH_LINEAR_CE_MAX_WEIGHTS)
+    return 0;
+  return linear_ce_workspace_bytes(tokens, hidden, vocab, dtype, pad_weight != 0, backward != 0);
+}
+
+int vbh_linear_cross_entropy_fwd(const void* x, const void* w, const void* labels, void* loss,
+                                 void* lse, void* z_loss, int64_t tokens, int64_t hidden,
+                                 int64_t vocab, int64_t x_stride, int64_t w_stride,
+                                 float smoothing, float logit_scale, float lse_square_scale,
+                                 int64_t ignored_index, int64_t total_classes,
+                                 int64_t class_start_idx, int dtype, int label_dtype, int split,
+                                 void* workspace, int64_t workspace_bytes, void* stream) {
+  const char* what = "linear_cross_entropy_fwd";
+  LceArgs a;
+  if (int rc = linear_ce_args(what, &a, x, w, labels, tokens, hidden, vocab, x_stride, w_stride,
+                              smoothing, logit_scale, lse_square_scale, ignored_index,
+                              total_classes, class_start_idx, dtype, label_dtype))
+    return rc;
+  if (tokens == 0) return 0;
+  if (!loss || !lse || !z_loss) return fail(VBH_E_INVALID, "%s: null pointer", what);
+  if (int rc = linear_ce_workspace_ok(what, a, dtype, false, workspace, workspace_bytes)) return rc;
+  a.loss = static_cast<float*>(loss);
+  a.lse = static_cast<float*>(lse);
+  a.z_loss = static_cast<float*>(z_loss);
+  a.split = split != 0;
+  return hip_status(launch_linear_ce(a, dtype, false, workspace, static_cast<hipStream_t>(stream)),
+                    what);
+}
+
+int vbh_linear_cross_entropy_bwd(const void* dloss, const void* x, const void* w, const void* lse,
+                                 const void* labels, void* dx, void* dw, int64_t tokens,
+                                 int64_t hidden, int64_t vocab, int64_t x_stride,
+                                 int64_t w_stride, float smoothing, float logit_scale,
+                                 float lse_square_scale, int64_t ignored_index,
+                                 int64_t total_classes, int64_t class_start_idx, int dtype,
+                                 int label_dtype, void* workspace, int64_t workspace_bytes,
+                                 void* stream) {
+  const char* what = "linear_cross_entropy_bwd";
+  LceArgs a;
+  if (int rc = linear_ce_args(what, &a, x, w, labels, tokens, hidden, vocab, x_stride, w_stride,
+                              smoothing, logit_scale, lse_square_scale, ignored_index,
+                              total_classes, class_start_idx, dtype, label_dtype))
+    return rc;
+  if (!dx && !dw) return 0;
+  if (tokens == 0 && !dw) return 0;
+  if (tokens > 0) {
+    if (!dloss || !lse) return fail(VBH_E_INVALID, "%s: null pointer", what);
+    if (int rc = linear_ce_workspace_ok(what, a, dtype, true, workspace, workspace_bytes))
+      return rc;
+  }
+  a.dloss = static_cast<const float*>(dloss);
+  a.lse_in = static_cast<const float*>(lse);
+  a.dx = dx;
+  a.dw = dw;
+  return hip_status(launch_linear_ce(a, dtype, true, workspace, static_cast<hipStream_t>(stream)),
+                    what);
 }
 
 // Split reductions keep, per segment, an fp32 mean, or an int64 index followed

@@ -397,6 +397,46 @@ bool norm_bwd_needs_workspace(int64_t rows, int64_t cols, int dt, bool sums);
 hipError_t launch_norm_bwd(NormGradArgs a, bool ln, int dt, int wdt, void* dw, void* db,
                            float* workspace, hipStream_t stream);
 
+// Cross entropy of a projection (linear_ce.hip).
+struct LceArgs {
+  const void* x = nullptr;        // [tokens] rows of x_stride
+  const void* w = nullptr;        // [vocab] rows of w_stride; null: to be padded from w_given
+  const void* w_given = nullptr;
+  const void* labels = nullptr;
+  const float* dloss = nullptr;   // backward
+  const float* lse_in = nullptr;
+  void* dx = nullptr;             // null: not wanted
+  void* dw = nullptr;
+  float* loss = nullptr;          // forward
+  float* lse = nullptr;
+  float* z_loss = nullptr;
+  int64_t tokens = 0, hidden = 0, vocab = 0;
+  int64_t x_stride = 0, w_stride = 0, w_given_stride = 0;
+  int64_t ignored = 0, class_start = 0;
+  float total_classes = 0.0f;
+  float smoothing = 0.0f, scale = 1.0f, lse_square_scale = 0.0f;
+  int label_i64 = 0, split = 0;
+  int x_direct = 0;               // x's rows are whole 16-byte pieces
+  // set by the launcher: parts of the workspace, the current piece of the vocabulary
+  int64_t padded = 0;             // hidden, to whole 16-byte pieces
+  void* info = nullptr;           // null: every token counts, in its place
+  int* rows = nullptr;
+  int* place = nullptr;
+  void* x_packed = nullptr;
+  void* w_packed = nullptr;
+  void* parts = nullptr;
+  float* totals = nullptr;
+  float* picked = nullptr;
+  void* piece = nullptr;
+  float* dx_sums = nullptr;       // null: one split of one piece
+  int64_t first = 0, cols = 0, pitch = 0;
+  int64_t split_cols = 0;
+  int splits = 1, col_tiles = 0;
+};
+int64_t linear_ce_workspace_bytes(int64_t tokens, int64_t hidden, int64_t vocab, int dt,
+                                  bool pad_weight, bool backward);
+hipError_t launch_linear_ce(LceArgs a, int dt, bool back, void* workspace, hipStream_t s);
+
 // Reduction over the middle axis.  With c.segs > 1, `parts` holds
 // outer * inner * segs fp32 results, and as many int32 rows for max / argmax.
 hipError_t launch_reduce_cols(const void* x, void* vals, int64_t* idx, void* parts,

@@ -131,6 +131,14 @@ ENTRY(vbh_cross_entropy_fwd_noalloc, "ppiipppqqqfffqqqqiip",
 ENTRY(vbh_cross_entropy_bwd, "pppppiiqqqqqfffqqqip",
       fn_vbh_cross_entropy_bwd(P(0), P(1), P(2), P(3), P(4), I(5), I(6), Q(7), Q(8), Q(9), Q(10),
                             Q(11), F(12), F(13), F(14), Q(15), Q(16), Q(17), I(18), P(19)))
+ENTRY(vbh_linear_cross_entropy_fwd, "ppppppqqqqqfffqqqiiipqp",
+      fn_vbh_linear_cross_entropy_fwd(P(0), P(1), P(2), P(3), P(4), P(5), Q(6), Q(7), Q(8), Q(9),
+                                      Q(10), F(11), F(12), F(13), Q(14), Q(15), Q(16), I(17),
+                                      I(18), I(19), P(20), Q(21), P(22)))
+ENTRY(vbh_linear_cross_entropy_bwd, "pppppppqqqqqfffqqqiipqp",
+      fn_vbh_linear_cross_entropy_bwd(P(0), P(1), P(2), P(3), P(4), P(5), P(6), Q(7), Q(8), Q(9),
+                                      Q(10), Q(11), F(12), F(13), F(14), Q(15), Q(16), Q(17),
+                                      I(18), I(19), P(20), Q(21), P(22)))
 ENTRY(vbh_reduce_fwd, "pppqqqiiip",
       fn_vbh_reduce_fwd(P(0), P(1), P(2), Q(3), Q(4), Q(5), I(6), I(7), I(8), P(9)))
 ENTRY(vbh_reduce_fwd_ws, "pppqqqiiipqp",
@@ -165,6 +173,7 @@ static const struct {
     SLOT(vbh_reduce_fwd_ws),     SLOT(vbh_stream_copy),      SLOT(vbh_stream_read),
     SLOT(vbh_rope_fwd),          SLOT(vbh_rope_bwd),         SLOT(vbh_qk_norm_rope_fwd),
     SLOT(vbh_qk_norm_rope_bwd),  SLOT(vbh_layer_norm_bwd),   SLOT(vbh_rms_norm_bwd),
+    SLOT(vbh_linear_cross_entropy_fwd), SLOT(vbh_linear_cross_entropy_bwd),
 };
 #define N_SLOTS (sizeof(slots) / sizeof(slots[0]))
 
@@ -204,6 +213,7 @@ static PyMethodDef methods[] = {
     METHOD(vbh_reduce_fwd_ws),     METHOD(vbh_stream_copy),       METHOD(vbh_stream_read),
     METHOD(vbh_rope_fwd),          METHOD(vbh_rope_bwd),          METHOD(vbh_qk_norm_rope_fwd),
     METHOD(vbh_qk_norm_rope_bwd),  METHOD(vbh_layer_norm_bwd),    METHOD(vbh_rms_norm_bwd),
+    METHOD(vbh_linear_cross_entropy_fwd), METHOD(vbh_linear_cross_entropy_bwd),
     {NULL, NULL, 0, NULL},
 };
 

@@ -238,6 +238,50 @@ int vbh_cross_entropy_bwd(const void* dloss, const void* logits, const void* lse
                           int64_t total_classes, int64_t class_start_idx,
                           int has_smoothing, void* stream);
 
+/* Softmax cross entropy of a projection onto a vocabulary, without the logits in memory:
+ * vbh_cross_entropy_fwd over logits = x w^T in 32 bits, one column block per row.
+ * x: [tokens] rows of `hidden` values, x_stride apart; w: [vocab] rows, w_stride apart; both of
+ * `dtype`.  loss, lse, z_loss: [tokens] fp32.  An ignored token's x is not read for any
+ * result: its loss, lse and z_loss are 0.  With `split` loss is left without the lse and
+ * z_loss parts (w is a slice of the classes from class_start_idx on; see
+ * vbh_cross_entropy_fwd).  Sums in fp32, in a fixed order.
+ * The workspace of vbh_linear_cross_entropy_workspace_bytes bytes is 256-byte aligned scratch
+ * of this call (stream-ordered); `pad_weight`: w's rows are not whole 16-byte pieces at
+ * multiples of 16 bytes, or more than 1 MiB apart, and are copied.
+ * No reference counterpart (ViperBench/cross_entropy takes logits). */
+#define VBH_LINEAR_CE_MAX_TOKENS (INT64_C(1) << 24)
+#define VBH_LINEAR_CE_MAX_HIDDEN (INT64_C(1) << 16)
+#define VBH_LINEAR_CE_MAX_VOCAB (INT64_C(1) << 24)
+#define VBH_LINEAR_CE_MAX_WEIGHTS (INT64_C(1) << 36) /* vocab * hidden            */
+#define VBH_LINEAR_CE_MAX_STRIDE (INT64_C(1) << 32)  /* of x and w               */
+int vbh_linear_cross_entropy_fwd(const void* x, const void* w, const void* labels, void* loss,
+                                 void* lse, void* z_loss, int64_t tokens, int64_t hidden,
+                                 int64_t vocab, int64_t x_stride, int64_t w_stride,
+                                 float smoothing, float logit_scale, float lse_square_scale,
+                                 int64_t ignored_index, int64_t total_classes,
+                                 int64_t class_start_idx, int dtype, int label_dtype, int split,
+                                 void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Its gradients, in pieces of the vocabulary: with L = logit_scale x w^T formed again,
+ *   dL = dloss logit_scale (exp(L - lse) (1 + 2 lse_square_scale lse) - target),
+ *   dx = dL w, dw = dL^T x,
+ * dL rounded to `dtype` (scaled, so that fp16 keeps it), sums in fp32 in a fixed order.
+ * dloss, lse: [tokens] fp32 (lse of the forward, or of all slices of the classes).
+ * dx: [tokens, hidden], dw: [vocab, hidden], contiguous, of `dtype`, each null where not
+ * wanted.  Ignored tokens: dx is 0, and nothing of theirs enters dw.  No tokens: dw becomes 0. */
+int vbh_linear_cross_entropy_bwd(const void* dloss, const void* x, const void* w, const void* lse,
+                                 const void* labels, void* dx, void* dw, int64_t tokens,
+                                 int64_t hidden, int64_t vocab, int64_t x_stride,
+                                 int64_t w_stride, float smoothing, float logit_scale,
+                                 float lse_square_scale, int64_t ignored_index,
+                                 int64_t total_classes, int64_t class_start_idx, int dtype,
+                                 int label_dtype, void* workspace, int64_t workspace_bytes,
+                                 void* stream);
+
+/* Workspace bytes of those calls, a pure function of the arguments (0 for invalid ones). */
+int64_t vbh_linear_cross_entropy_workspace_bytes(int64_t tokens, int64_t hidden, int64_t vocab,
+                                                 int dtype, int pad_weight, int backward);
+
 /* Mean, max or argmax over the middle axis of a contiguous [outer, n, inner]
  * tensor x of `in_dtype` (inner == 1 is the last axis).
  *   VBH_REDUCE_MEAN:   values[outer * inner] of `out_dtype` (in_dtype, or F32
