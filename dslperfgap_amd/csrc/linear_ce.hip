@@ -252,44 +252,45 @@ __global__ __launch_bounds__(G::kLanes) void lce_forward(const LceArgs a) {
   G g;
   logits<T>(a, g, at, live, c0, a.vocab - c0, p0, p1, q0, q1);
 
-  const int lane = static_cast<int>(threadIdx.x) & (kWave - 1), half = lane >> 5;
+  const int lane = static_cast<int>(threadIdx.x) & (kWave - 1), quarter = lane >> 4;
   const int64_t r0 = static_cast<int64_t>(at.row) * G::BR;
-  // columns of the tile that the vocabulary has; of the lane's, those at 8 (i / 4) + 4 half + i % 4
+  // columns of the wave's that the vocabulary has (a lane holds those at 4 quarter + i of a block)
   const int left = static_cast<int>(min(a.vocab - c0, static_cast<int64_t>(G::BC))) - g.wave_col();
   LsePart* parts = reinterpret_cast<LsePart*>(p1);           // [WC][BR]
   float* totals = reinterpret_cast<float*>(parts + G::WC * G::BR);  // [WC][BR]
-  static_assert(G::WC * G::BR * 12 <= G::P::kBytes, "parts fit one buffer");
+  static_assert(G::WC * G::BR * 12 <= static_cast<int>(sizeof(p1)), "parts fit one buffer");
 #pragma unroll
   for (int r = 0; r < G::RB; ++r) {
-    const int row = g.wave_row() + r * 32 + (lane & 31);
-    // block by block: 16 logits of a token at a time
+    const int row = g.wave_row() + r * kBlockRows + (lane & 15);
+    // a few blocks at a time: up to 16 logits of a token
+    constexpr int kSome = G::CB < 4 ? G::CB : 4;
     LsePart mine{-__builtin_huge_valf(), 0.0f};
     float total = 0.0f;
 #pragma unroll
-    for (int c = 0; c < G::CB; ++c) {
-      float v[16];
+    for (int c = 0; c < G::CB; c += kSome) {
+      float v[4 * kSome];
 #pragma unroll
-      for (int i = 0; i < 16; ++i) v[i] = mul_rn(g.sums[r][c][i], a.scale);
-      if (c * 32 + 32 > left) {  // (the vocabulary ends here)
+      for (int i = 0; i < 4 * kSome; ++i) v[i] = mul_rn(g.sums[r][c + i / 4][i % 4], a.scale);
+      if ((c + kSome) * kBlockRows > left) {  // (the vocabulary ends here)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const bool in = c * 32 + 8 * (i / 4) + 4 * half + i % 4 < left;
+        for (int i = 0; i < 4 * kSome; ++i) {
+          const bool in = (c + i / 4) * kBlockRows + 4 * quarter + i % 4 < left;
           if (a.smoothing != 0.0f) total += in ? v[i] : 0.0f;
           v[i] = in ? v[i] : -__builtin_huge_valf();
         }
       } else if (a.smoothing != 0.0f) {
 #pragma unroll
-        for (int i = 0; i < 16; ++i) total += v[i];
+        for (int i = 0; i < 4 * kSome; ++i) total += v[i];
       }
       float m = mine.m;
 #pragma unroll
-      for (int i = 0; i < 16; ++i) m = max_nan(m, v[i]);
+      for (int i = 0; i < 4 * kSome; ++i) m = max_nan(m, v[i]);
       const float by = shift_of(m);
       float s = mine.s * fast_exp(mine.m - by);
 #pragma unroll
-      for (int i = 0; i < 16; ++i) s += fast_exp(v[i] - by);
+      for (int i = 0; i < 4 * kSome; ++i) s += fast_exp(v[i] - by);
       mine = LsePart{m, s};
-      __builtin_amdgcn_sched_barrier(0);  // one block's values in registers at a time
+      __builtin_amdgcn_sched_barrier(0);  // the next ones' values stay out of the registers
     }
     // the label's logit
     const bool own = r0 + row < live;
@@ -297,20 +298,22 @@ __global__ __launch_bounds__(G::kLanes) void lce_forward(const LceArgs a) {
                                     : static_cast<int>(r0 + row))
                           : 0;
     const int64_t label = own ? label_at(a, t) - a.class_start - c0 - g.wave_col() : -1;
-    const bool has = label >= 0 && label < left && label < G::BC / G::WC && ((label >> 2) & 1) == half;
+    const bool has = label >= 0 && label < left && label < G::BC / G::WC && ((label >> 2) & 3) == quarter;
     if (__ballot(has) != 0) {
       float v = 0.0f;
 #pragma unroll
       for (int c = 0; c < G::CB; ++c) {
 #pragma unroll
-        for (int i = 0; i < 16; ++i)
-          v = label == c * 32 + 8 * (i / 4) + 4 * half + i % 4 ? g.sums[r][c][i] : v;
+        for (int i = 0; i < 4; ++i)
+          v = label == c * kBlockRows + 4 * quarter + i ? g.sums[r][c][i] : v;
       }
       if (has) store_one(a.picked + r0 + row, v * a.scale, VBH_SPAN(a.picked, a.tokens));
     }
+    mine = join(mine, LsePart{swap16_partner(mine.m), swap16_partner(mine.s)});
     mine = join(mine, LsePart{swap32_partner(mine.m), swap32_partner(mine.s)});
+    total += swap16_partner(total);
     total += swap32_partner(total);
-    if (half == 0) {
+    if (quarter == 0) {
       const int wc = g.wave_col() / (G::BC / G::WC);
       parts[wc * G::BR + row] = mine;
       totals[wc * G::BR + row] = total;
@@ -398,7 +401,7 @@ __global__ __launch_bounds__(G::kLanes) void lce_dlogits(const LceArgs a) {
   G g;
   logits<T>(a, g, at, info.live, a.first + c0, a.cols - c0, p0, p1, q0, q1);
 
-  const int lane = static_cast<int>(threadIdx.x) & (kWave - 1), half = lane >> 5;
+  const int lane = static_cast<int>(threadIdx.x) & (kWave - 1), quarter = lane >> 4;
   const int64_t r0 = static_cast<int64_t>(at.row) * G::BR;
   const int left = static_cast<int>(min(a.cols - c0, static_cast<int64_t>(G::BC))) - g.wave_col();
   const int padded = static_cast<int>(min(a.pitch - c0, static_cast<int64_t>(G::BC))) - g.wave_col();
@@ -407,7 +410,7 @@ __global__ __launch_bounds__(G::kLanes) void lce_dlogits(const LceArgs a) {
   const Span sp = VBH_SPAN(piece, info.live * a.pitch);
 #pragma unroll
   for (int r = 0; r < G::RB; ++r) {
-    const int row = g.wave_row() + r * 32 + (lane & 31);
+    const int row = g.wave_row() + r * kBlockRows + (lane & 15);
     if (r0 + row >= info.live) continue;
     const int64_t t = load_one(a.rows + r0 + row, VBH_SPAN(a.rows, a.tokens));
     const int64_t label = label_at(a, t) - a.class_start - a.first - c0 - g.wave_col();
@@ -417,19 +420,16 @@ __global__ __launch_bounds__(G::kLanes) void lce_dlogits(const LceArgs a) {
     T* to = piece + (r0 + row) * a.pitch + c0 + g.wave_col();
 #pragma unroll
     for (int c = 0; c < G::CB; ++c) {
+      const int col = c * kBlockRows + 4 * quarter;
+      float o[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int col = c * 32 + 8 * i + 4 * half;
-        float o[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float p = fast_exp(g.sums[r][c][4 * i + j] * a.scale - lse);
-          float q = fmaf(p, f, -even);
-          if (label == col + j) q -= 1.0f - a.smoothing;
-          o[j] = col + j < left ? by * q : 0.0f;
-        }
-        if (col < padded) store_any<T, 4, false>(to + col, o, sp);
+      for (int j = 0; j < 4; ++j) {
+        const float p = fast_exp(g.sums[r][c][j] * a.scale - lse);
+        float q = fmaf(p, f, -even);
+        if (label == col + j) q -= 1.0f - a.smoothing;
+        o[j] = col + j < left ? by * q : 0.0f;
       }
+      if (col < padded) store_any<T, 4, false>(to + col, o, sp);
     }
   }
 }
@@ -465,11 +465,11 @@ __global__ __launch_bounds__(G::kLanes) void lce_dweight(const LceArgs a) {
   g.run(p, q, info.live, p0, p1, q0, q1);
   T* dw = static_cast<T*>(a.dw);
   const Span sd = VBH_SPAN(dw, a.vocab * a.hidden);
-  g.each([&](int row, int col, int r, int c, int i) {
+  g.each([&](int row, int col, const f32x4& sums) {
     if (r0 + row >= a.cols) return;
     float o[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) o[j] = ldexpf(g.sums[r][c][4 * i + j], -info.shift);
+    for (int j = 0; j < 4; ++j) o[j] = ldexpf(sums[j], -info.shift);
     store_four(dw + (a.first + r0 + row) * a.hidden, c0 + col, cols, o, sd);
   });
 }
@@ -496,12 +496,12 @@ __global__ __launch_bounds__(G::kLanes) void lce_dx(const LceArgs a, int more) {
   T* dx = static_cast<T*>(a.dx);
   const Span sd = VBH_SPAN(dx, a.tokens * a.hidden);
   const Span ss = VBH_SPAN(a.dx_sums, a.splits * a.tokens * a.padded);
-  g.each([&](int row, int col, int r, int c, int i) {
+  g.each([&](int row, int col, const f32x4& sums) {
     if (r0 + row >= info.live || c0 + col >= a.hidden) return;
     float o[4];
     if (a.dx_sums == nullptr) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) o[j] = ldexpf(g.sums[r][c][4 * i + j], -info.shift);
+      for (int j = 0; j < 4; ++j) o[j] = ldexpf(sums[j], -info.shift);
       const int64_t t = load_one(a.rows + r0 + row, VBH_SPAN(a.rows, a.tokens));
       store_four(dx + t * a.hidden, c0 + col, a.hidden, o, sd);
       return;
@@ -514,7 +514,7 @@ __global__ __launch_bounds__(G::kLanes) void lce_dx(const LceArgs a, int more) {
       for (int j = 0; j < 4; ++j) o[j] = 0.0f;
     }
 #pragma unroll
-    for (int j = 0; j < 4; ++j) o[j] += g.sums[r][c][4 * i + j];
+    for (int j = 0; j < 4; ++j) o[j] += sums[j];
     store_from_f32<float, 4>(to, o, ss);
   });
 }
@@ -554,31 +554,58 @@ __global__ __launch_bounds__(kGatherRows* kWave) void lce_zero(T* p, int64_t n) 
 // launches
 // ---------------------------------------------------------------------------
 
-// Tiles by tokens: 256 x 256 on 8 waves; for few tokens 64 or 32 by 128 on 4, whose time is the
-// read of W.
+// Tiles, by size and type:
+//   kBig   256 x 256 on 8 waves, one workgroup per CU: 16-bit products that fill the card with them
+//   kMid   128 x 128 on 4 waves, two per CU: 0.85 of kBig's rate (8192 x 8192 x 8192: 1151 against
+//          1375 TFLOP/s), in quarters of its portions; fp32 always, whose matrix instructions take
+//          as long as the reads for either (125-134 TFLOP/s; the library's best 117-122)
+//   kSmall 64 x 128, kTiny 32 x 128 on 4 waves: products of at most as many rows, whose time is
+//          the read of W
+enum Tile { kBig, kMid, kSmall, kTiny };
 template <typename T, bool P_COLUMNS, bool Q_COLUMNS>
 using BigTile = TileProduct<T, 256, 256, 4, 2, P_COLUMNS, Q_COLUMNS>;
+template <typename T, bool P_COLUMNS, bool Q_COLUMNS>
+using MidTile = TileProduct<T, 128, 128, 2, 2, P_COLUMNS, Q_COLUMNS>;
 template <typename T, bool Q_COLUMNS>
 using SmallTile = TileProduct<T, 64, 128, 1, 4, false, Q_COLUMNS>;
 template <typename T, bool Q_COLUMNS>
 using TinyTile = TileProduct<T, 32, 128, 1, 4, false, Q_COLUMNS>;
 
-constexpr int64_t kBigTokens = 64;   // more than these: BigTile
-constexpr int64_t kTinyTokens = 32;
 constexpr int64_t kPlainTokens = 64; // forward of at most these: no numbering of tokens
 constexpr int64_t kPieceBytes = int64_t(256) << 20;
 constexpr int64_t kPieceCols = 4096; // least of a piece
 constexpr int64_t kMostPieceCols = int64_t(1) << 18;
-constexpr int64_t kFill = 256;       // workgroups that fill the card
 constexpr int64_t kSplitCols = 1024; // least of a split of dx
 
 int64_t up(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
 int64_t tiles(int64_t n, int64_t each) { return (n + each - 1) / each; }
 int value_bytes(int dt) { return dt == kF32 ? 4 : 2; }
 
-int64_t bc_of(int64_t tokens) { return tokens > kBigTokens ? 256 : 128; }
-int64_t br_of(int64_t tokens) {
-  return tokens > kBigTokens ? 256 : tokens > kTinyTokens ? 64 : 32;
+// The tile of a product of `rows` (of P, whose lines have k contiguous unless P_COLUMNS) by `cols`.
+Tile tile_of(int64_t rows, int64_t cols, int dt, bool p_columns = false) {
+  if (!p_columns && rows <= 32) return kTiny;
+  if (!p_columns && rows <= 64) return kSmall;
+  if (dt == kF32) return kMid;
+  // rounds of workgroups, by a round's time
+  const int64_t big = tiles(tiles(rows, 256) * tiles(cols, 256), 256) * 100;
+  const int64_t mid = tiles(tiles(rows, 128) * tiles(cols, 128), 512) * 59;
+  return mid < big ? kMid : kBig;
+}
+int64_t tile_rows(Tile t) { return t == kBig ? 256 : t == kMid ? 128 : t == kSmall ? 64 : 32; }
+int64_t tile_cols(Tile t) { return t == kBig ? 256 : 128; }
+int64_t tile_fill(Tile t) { return t == kBig ? 256 : 512; }  // workgroups that fill the card
+
+// f(TypeTag of the TileProduct)
+template <typename T, bool Q_COLUMNS, typename F>
+void with_tile(Tile t, F&& f) {
+  switch (t) {
+    case kBig:
+      if constexpr (sizeof(T) == 2) f(TypeTag<BigTile<T, false, Q_COLUMNS>>{});
+      break;
+    case kMid: f(TypeTag<MidTile<T, false, Q_COLUMNS>>{}); break;
+    case kSmall: f(TypeTag<SmallTile<T, Q_COLUMNS>>{}); break;
+    case kTiny: f(TypeTag<TinyTile<T, Q_COLUMNS>>{}); break;
+  }
 }
 
 // The workspace's parts, each at a multiple of 256 bytes.
@@ -587,7 +614,8 @@ struct LcePlan {
   int64_t pieces = 1, piece_cols = 0, pitch = 0;
   int64_t splits = 1, split_cols = 0;
   bool sums = false;
-  int64_t info = -1, rows = 0, place = 0, x = 0, w = 0, parts = 0, totals = 0, picked = 0,
+  Tile dx_tile = kBig;
+  int64_t info = 0, rows = 0, place = 0, x = 0, w = 0, parts = 0, totals = 0, picked = 0,
           piece = 0, dx_sums = 0, bytes = 0;
 };
 
@@ -607,7 +635,7 @@ LcePlan lce_plan(int64_t tokens, int64_t hidden, int64_t vocab, int dt, bool pad
   p.x = take(tokens * p.padded * e);
   if (pad_weight) p.w = take(vocab * p.padded * e);
   if (!backward) {
-    const int64_t n = tiles(vocab, bc_of(tokens)) * tokens;
+    const int64_t n = tiles(vocab, tile_cols(tile_of(tokens, vocab, dt))) * tokens;
     p.parts = take(n * sizeof(LsePart));
     p.totals = take(n * 4);
     p.picked = take(tokens * 4);
@@ -621,9 +649,10 @@ LcePlan lce_plan(int64_t tokens, int64_t hidden, int64_t vocab, int dt, bool pad
   p.pieces = tiles(vocab, p.piece_cols);
   p.pitch = up(std::min(p.piece_cols, vocab), 16 / e);
   p.piece = take(tokens * p.pitch * e);
-  const int64_t out = tiles(tokens, br_of(tokens)) * tiles(hidden, bc_of(tokens));
   const int64_t cols = std::min(p.piece_cols, vocab);  // of the first piece
-  p.splits = std::max<int64_t>(std::min(tiles(kFill, out), cols / kSplitCols), 1);
+  p.dx_tile = tile_of(tokens, hidden, dt);
+  const int64_t out = tiles(tokens, tile_rows(p.dx_tile)) * tiles(hidden, tile_cols(p.dx_tile));
+  p.splits = std::max<int64_t>(std::min(tiles(tile_fill(p.dx_tile), out), cols / kSplitCols), 1);
   p.split_cols = up(tiles(cols, p.splits), 128);
   p.splits = tiles(cols, p.split_cols);
   p.sums = p.splits > 1 || p.pieces > 1;
@@ -632,7 +661,7 @@ LcePlan lce_plan(int64_t tokens, int64_t hidden, int64_t vocab, int dt, bool pad
 }
 
 template <typename T>
-hipError_t forward(LceArgs a, const LcePlan& p, bool number, hipStream_t s) {
+hipError_t forward(LceArgs a, int dt, bool number, hipStream_t s) {
   const unsigned tokens4 = static_cast<unsigned>(tiles(a.tokens, kGatherRows));
   hipError_t err = hipSuccess;
   auto done = [&] { return (err = hipGetLastError()) == hipSuccess; };
@@ -644,15 +673,13 @@ hipError_t forward(LceArgs a, const LcePlan& p, bool number, hipStream_t s) {
     launch_kernel(lce_gather<T>, dim3(tokens4), dim3(kGatherRows * kWave), 0, s, a);
     if (!done()) return err;
   }
-  a.col_tiles = static_cast<int>(tiles(a.vocab, bc_of(a.tokens)));
-  const int64_t grid = tile_grid(tiles(a.tokens, br_of(a.tokens)), a.col_tiles);
-  auto go = [&](auto tag) {
+  const Tile t = tile_of(a.tokens, a.vocab, dt);
+  a.col_tiles = static_cast<int>(tiles(a.vocab, tile_cols(t)));
+  with_tile<T, false>(t, [&](auto tag) {
     using G = typename decltype(tag)::type;
+    const int64_t grid = tile_grid(tiles(a.tokens, G::BR), a.col_tiles);
     launch_kernel(lce_forward<T, G>, dim3(static_cast<unsigned>(grid)), dim3(G::kLanes), 0, s, a);
-  };
-  if (a.tokens > kBigTokens) go(TypeTag<BigTile<T, false, false>>{});
-  else if (a.tokens > kTinyTokens) go(TypeTag<SmallTile<T, false>>{});
-  else go(TypeTag<TinyTile<T, false>>{});
+  });
   if (!done()) return err;
   launch_kernel(lce_join, dim3(static_cast<unsigned>(tiles(a.tokens, kJoinRows))),
                 dim3(kJoinRows * kJoinLanes), 0, s, a);
@@ -661,7 +688,7 @@ hipError_t forward(LceArgs a, const LcePlan& p, bool number, hipStream_t s) {
 }
 
 template <typename T>
-hipError_t backward(LceArgs a, const LcePlan& p, hipStream_t s) {
+hipError_t backward(LceArgs a, int dt, const LcePlan& p, hipStream_t s) {
   const unsigned tokens4 = static_cast<unsigned>(tiles(a.tokens, kGatherRows));
   hipError_t err = hipSuccess;
   auto done = [&] { return (err = hipGetLastError()) == hipSuccess; };
@@ -669,41 +696,43 @@ hipError_t backward(LceArgs a, const LcePlan& p, hipStream_t s) {
   if (!done()) return err;
   launch_kernel(lce_gather<T>, dim3(tokens4), dim3(kGatherRows * kWave), 0, s, a);
   if (!done()) return err;
-  const int64_t row_tiles = tiles(a.tokens, br_of(a.tokens));
   for (int64_t i = 0; i < p.pieces; ++i) {
     a.first = i * p.piece_cols;
     a.cols = std::min(p.piece_cols, a.vocab - a.first);
     a.pitch = up(a.cols, 16 / static_cast<int64_t>(sizeof(T)));
-    a.col_tiles = static_cast<int>(tiles(a.cols, bc_of(a.tokens)));
-    auto logits_grads = [&](auto tag) {
+    const Tile t = tile_of(a.tokens, a.cols, dt);
+    a.col_tiles = static_cast<int>(tiles(a.cols, tile_cols(t)));
+    with_tile<T, false>(t, [&](auto tag) {
       using G = typename decltype(tag)::type;
-      launch_kernel(lce_dlogits<T, G>, dim3(static_cast<unsigned>(tile_grid(row_tiles, a.col_tiles))),
-                    dim3(G::kLanes), 0, s, a);
-    };
-    if (a.tokens > kBigTokens) logits_grads(TypeTag<BigTile<T, false, false>>{});
-    else if (a.tokens > kTinyTokens) logits_grads(TypeTag<SmallTile<T, false>>{});
-    else logits_grads(TypeTag<TinyTile<T, false>>{});
+      const int64_t grid = tile_grid(tiles(a.tokens, G::BR), a.col_tiles);
+      launch_kernel(lce_dlogits<T, G>, dim3(static_cast<unsigned>(grid)), dim3(G::kLanes), 0, s, a);
+    });
     if (!done()) return err;
     if (a.dw != nullptr) {
-      using G = BigTile<T, true, true>;
-      launch_kernel(lce_dweight<T, G>,
-                    dim3(static_cast<unsigned>(tile_grid(tiles(a.cols, 256), tiles(a.hidden, 256)))),
-                    dim3(G::kLanes), 0, s, a);
+      auto go = [&](auto tag) {
+        using G = typename decltype(tag)::type;
+        const int64_t grid = tile_grid(tiles(a.cols, G::BR), tiles(a.hidden, G::BC));
+        launch_kernel(lce_dweight<T, G>, dim3(static_cast<unsigned>(grid)), dim3(G::kLanes), 0, s,
+                      a);
+      };
+      if constexpr (sizeof(T) == 2) {
+        if (tile_of(a.cols, a.hidden, dt, true) == kBig) go(TypeTag<BigTile<T, true, true>>{});
+        else go(TypeTag<MidTile<T, true, true>>{});
+      } else {
+        go(TypeTag<MidTile<T, true, true>>{});
+      }
       if (!done()) return err;
     }
     if (a.dx == nullptr) continue;
-    auto dx = [&](auto tag) {
+    with_tile<T, true>(p.dx_tile, [&](auto tag) {
       using G = typename decltype(tag)::type;
-      const int64_t grid = tile_grid(row_tiles, tiles(a.hidden, G::BC));
+      const int64_t grid = tile_grid(tiles(a.tokens, G::BR), tiles(a.hidden, G::BC));
       // a shorter last piece may have fewer splits: those before it have summed into all
       launch_kernel(lce_dx<T, G>,
                     dim3(static_cast<unsigned>(grid),
                          static_cast<unsigned>(tiles(a.cols, a.split_cols))),
                     dim3(G::kLanes), 0, s, a, i > 0 ? 1 : 0);
-    };
-    if (a.tokens > kBigTokens) dx(TypeTag<BigTile<T, false, true>>{});
-    else if (a.tokens > kTinyTokens) dx(TypeTag<SmallTile<T, true>>{});
-    else dx(TypeTag<TinyTile<T, true>>{});
+    });
     if (!done()) return err;
   }
   if (a.dx != nullptr && p.sums) {
@@ -763,7 +792,7 @@ hipError_t launch_linear_ce(LceArgs a, int dt, bool back, void* workspace, hipSt
       err = hipGetLastError();
       if (err != hipSuccess) return;
     }
-    err = back ? backward<T>(a, p, s) : forward<T>(a, p, number, s);
+    err = back ? backward<T>(a, dt, p, s) : forward<T>(a, dt, number, s);
   });
   return err;
 }

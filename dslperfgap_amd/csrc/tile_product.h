@@ -3,9 +3,9 @@
 //   out[r, c] = sum over k of P[r, k] Q[c, k]
 //
 // A workgroup of WR x WC waves computes a tile of BR rows by BC columns; a wave holds
-// RB x CB blocks of 32 x 32 fp32 sums.  k goes in stages of 128 bytes of each row or
+// RB x CB blocks of 16 x 16 fp32 sums.  k goes in stages of 128 bytes of each row or
 // column (64 values of 16 bits, 32 of fp32), which the buffer loads write straight into
-// the LDS, one stage ahead of the one that the matrix cores work on.
+// the LDS, at least one stage ahead of the one that the matrix cores work on.
 //
 // An operand lies in memory with k contiguous ("rows": [r][k]) or with k the slow axis
 // ("columns": [k][r]).  Columns of 16-bit values are turned on the way from the LDS to the
@@ -13,9 +13,20 @@
 // zeros: by the buffer resource's range, and within a row by an offset beyond it.
 //
 // Bank conflicts: the LDS takes stages as the loads deliver them, 16 bytes per lane in
-// lane order, so lanes ask for their 16-byte pieces in a permuted order instead:
-//   rows: piece p of row r lies at p ^ (r & 7);
-//   columns: piece p of line k lies at p ^ 4 (k & 3), of 32-bit values at p ^ 2 (k & 4).
+// lane order, so lanes ask for their 16-byte pieces in a permuted order instead (SQ counters
+// show none for 16-bit operands; without it every second cycle of the reads is one):
+//   rows: piece p of row r lies at p ^ (r / 2 % 8);
+//   columns: piece p of line k lies at p ^ 4 (k % 4) ^ 2 (k / 8 % 2), of 32-bit values at
+//   p ^ 4 (k / 4 % 2).
+//
+// MI355X, bf16, 256 x 256 tiles, us (TFLOP/s) beside the library's best kernel for the layout:
+// 8192 x 8192 x 8192 deep, rows by rows 781 (1408; library 698, 1574), rows by columns
+// 8192 x 4096 x 16384 823 (1335; 901, 1221), columns by columns 16384 x 4096 x 8192 808
+// (1360; 1030, 1067).  Blocks of 32 x 32 reach 1280, 1170 and 1214 in the same scheme: their
+// sums cross the registers twice as often per operation, and the card's power is the bound
+// (the same loop without its loads runs at 1567, without its LDS reads at 1605, without
+// either at 2120).  4 waves of 128 x 128: 1270.  Four buffers of half a stage: 1223 (rows of 64
+// bytes), 1245 and 1270.
 #pragma once
 
 #include <type_traits>
@@ -24,32 +35,33 @@
 
 namespace vbh {
 
-typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) void lds_void;
 
 template <typename T> struct Frag { typedef T type __attribute__((ext_vector_type(16 / sizeof(T)))); };
 
-// acc[m][n] += sum over the fragments' k of a[m] b[n]: lane l holds row (column) l % 32 and
-// the 16 bytes of k of half l / 32; of the sums column n = l % 32 and rows
-// m = 8 (i / 4) + 4 (l / 32) + i % 4.
-__device__ __forceinline__ f32x16 multiply(const Frag<__bf16>::type& a, const Frag<__bf16>::type& b,
-                                           const f32x16& acc) {
-  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, acc, 0, 0, 0);
+// acc[m][n] += sum over the fragments' k of a[m] b[n]: lane l holds row (column) l % 16 and
+// the 16 bytes of k of quarter l / 16; of the sums column n = l % 16 and rows
+// m = 4 (l / 16) + i.
+__device__ __forceinline__ f32x4 multiply(const Frag<__bf16>::type& a, const Frag<__bf16>::type& b,
+                                           const f32x4& acc) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, acc, 0, 0, 0);
 }
-__device__ __forceinline__ f32x16 multiply(const Frag<_Float16>::type& a,
-                                           const Frag<_Float16>::type& b, const f32x16& acc) {
-  return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, acc, 0, 0, 0);
+__device__ __forceinline__ f32x4 multiply(const Frag<_Float16>::type& a,
+                                           const Frag<_Float16>::type& b, const f32x4& acc) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, acc, 0, 0, 0);
 }
-__device__ __forceinline__ f32x16 multiply(const Frag<float>::type& a, const Frag<float>::type& b,
-                                           f32x16 acc) {
+__device__ __forceinline__ f32x4 multiply(const Frag<float>::type& a, const Frag<float>::type& b,
+                                           f32x4 acc) {
 #pragma unroll
-  for (int j = 0; j < 4; ++j) acc = __builtin_amdgcn_mfma_f32_32x32x2f32(a[j], b[j], acc, 0, 0, 0);
+  for (int j = 0; j < 4; ++j) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(a[j], b[j], acc, 0, 0, 0);
   return acc;
 }
 
 constexpr int kStageBytes = 128;  // of k, per row
 template <typename T> constexpr int kStageValues = kStageBytes / static_cast<int>(sizeof(T));
-constexpr int kSteps = 4;         // fragments per stage
+constexpr int kSteps = 2;         // fragments per stage
+constexpr int kBlockRows = 16;    // of a fragment
 
 // Beyond the range of every resource below.
 constexpr uint32_t kNowhere = 0x7fffff00u;
@@ -64,8 +76,10 @@ struct Operand {
   static constexpr int kLoads = kBytes / 16 / LANES;       // of a lane per stage
   static constexpr int kPieces = COLUMNS ? N * static_cast<int>(sizeof(T)) / 16 : 8;  // of a line
   static constexpr int kLinesPerLoad = LANES / kPieces;
-  static_assert(kBytes % (16 * LANES) == 0 && LANES % kPieces == 0 && kLinesPerLoad % 8 == 0,
+  static_assert(kBytes % (16 * LANES) == 0 && LANES % kPieces == 0 &&
+                    kLinesPerLoad % (COLUMNS && sizeof(T) == 4 ? 8 : 16) == 0,
                 "whole loads, of lines whose permutation does not depend on the load");
+  static_assert(!COLUMNS || kPieces >= 16, "room for the permutation");
 
   __amdgpu_buffer_rsrc_t rsrc;
   const T* base;     // of the resource
@@ -82,9 +96,9 @@ struct Operand {
       : base(from), line(ld * static_cast<int64_t>(sizeof(T))), span(s) {
     const int t = static_cast<int>(threadIdx.x);
     const int at = t / kPieces, slot = t % kPieces;
-    const int piece = !COLUMNS         ? slot ^ (at & 7)
-                      : sizeof(T) == 2 ? slot ^ ((at & 3) << 2)
-                                       : slot ^ ((at & 4) << 1);
+    const int piece = !COLUMNS         ? slot ^ ((at >> 1) & 7)
+                      : sizeof(T) == 2 ? slot ^ ((at & 3) << 2) ^ (((at >> 3) & 1) << 1)
+                                       : slot ^ (at & 4);
     offset = static_cast<uint32_t>(at * line + piece * 16);
     extent = lines > 0 ? (lines - 1) * line + values * static_cast<int64_t>(sizeof(T)) : 0;
     k_left = static_cast<int>(values) - piece * (16 / static_cast<int>(sizeof(T)));
@@ -122,30 +136,34 @@ struct Operand {
     range();
   }
 
-  // The lane's fragment of rows `row` .. `row` + 31 at step `step` of the stage in `lds`.
-  __device__ static __forceinline__ typename Frag<T>::type fragment(const char* lds, int row,
-                                                                    int step) {
+  // The lane's fragment of the 16 rows of block `block` from row `base` (a multiple of 32) on at
+  // step `step` of the stage in `lds`.
+  __device__ static __forceinline__ typename Frag<T>::type fragment(const char* lds, int base,
+                                                                    int block, int step) {
+    const int row = base + block * kBlockRows;
     const int lane = static_cast<int>(threadIdx.x) & (kWave - 1);
-    const int half = lane >> 5;
+    const int quarter = lane >> 4;
     if constexpr (!COLUMNS) {
-      // row is a multiple of 32: one address per step, blocks apart by an immediate offset
-      const int from = (lane & 31) * kStageBytes + (((2 * step + half) ^ (lane & 7)) * 16);
+      // one address per step, blocks apart by an immediate offset
+      const int from =
+          (lane & 15) * kStageBytes + (((4 * step + quarter) ^ ((lane >> 1) & 7)) * 16);
       return *reinterpret_cast<const typename Frag<T>::type*>(lds + from + row * kStageBytes);
     } else if constexpr (sizeof(T) == 4) {
-      // 32 lanes read 128 bytes of a line, the others as much 4 lines on
+      // 16 lanes read 64 bytes of a line, the next ones as much 4 lines on
       typename Frag<T>::type f;
-      const int from = half * 4 * kPieces * 16 + (lane & 31) * 4 + ((row * 4) ^ (half * 128));
+      const int from = quarter * 4 * kPieces * 16 + (lane & 15) * 4 +
+                       (((block & 1) * 64) ^ ((quarter & 1) * 64)) + base * 4 + (block >> 1) * 128;
 #pragma unroll
       for (int j = 0; j < 4; ++j)
-        f[j] = *reinterpret_cast<const float*>(lds + from + (8 * step + j) * kPieces * 16);
+        f[j] = *reinterpret_cast<const float*>(lds + from + (16 * step + j) * kPieces * 16);
       return f;
     } else {
       // 16 lanes read 4 lines of 16 values and get one column of 4 each
       typedef short s16x4 __attribute__((ext_vector_type(4)));
       typedef short s16x8 __attribute__((ext_vector_type(8)));
-      const int r = row + (lane & 16) + (lane & 3) * 4;  // of the lane's 8 bytes
-      const int k = step * 16 + half * 8 + ((lane & 15) >> 2);
-      const int piece = (r >> 3) ^ ((k & 3) << 2);
+      const int r = row + (lane & 3) * 4;  // of the lane's 8 bytes
+      const int k = step * 32 + quarter * 8 + ((lane & 15) >> 2);
+      const int piece = (r >> 3) ^ ((k & 3) << 2) ^ (((k >> 3) & 1) << 1);
       const char* from = lds + (k * kPieces + piece) * 16 + (r & 7) * 2;
       typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
       const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(from));
@@ -169,12 +187,12 @@ template <typename T, int BR_, int BC_, int WR_, int WC_, bool P_COLUMNS, bool Q
 struct TileProduct {
   static constexpr int BR = BR_, BC = BC_, WR = WR_, WC = WC_;
   static constexpr int kLanes = WR * WC * kWave;
-  static constexpr int RB = BR / WR / 32, CB = BC / WC / 32;  // blocks of a wave
+  static constexpr int RB = BR / WR / kBlockRows, CB = BC / WC / kBlockRows;  // blocks of a wave
   typedef Operand<T, BR, kLanes, P_COLUMNS> P;
   typedef Operand<T, BC, kLanes, Q_COLUMNS> Q;
-  static constexpr int kLdsBytes = 2 * (P::kBytes + Q::kBytes);
+  typedef typename Frag<T>::type F;
 
-  f32x16 sums[RB][CB];
+  f32x4 sums[RB][CB];
 
   __device__ static __forceinline__ int wave_row() {
     return (__builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6) / WC) * (BR / WR);
@@ -183,22 +201,13 @@ struct TileProduct {
     return (__builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6) % WC) * (BC / WC);
   }
 
-  __device__ __forceinline__ void stage(const char* p, const char* q) {
-    const int r0 = wave_row(), c0 = wave_col();
-#pragma unroll
-    for (int s = 0; s < kSteps; ++s) {
-      typename Frag<T>::type pf[RB], qf[CB];
-#pragma unroll
-      for (int r = 0; r < RB; ++r) pf[r] = P::fragment(p, r0 + r * 32, s);
-#pragma unroll
-      for (int c = 0; c < CB; ++c) qf[c] = Q::fragment(q, c0 + c * 32, s);
-#pragma unroll
-      for (int r = 0; r < RB; ++r) {
-#pragma unroll
-        for (int c = 0; c < CB; ++c) sums[r][c] = multiply(qf[c], pf[r], sums[r][c]);
-      }
-    }
-  }
+  // A stage's work in units: one fragment of Q against a step's RB fragments of P, RB matrix
+  // instructions.  A fragment of Q is read kAhead units before its own, those of P all at once as
+  // far ahead of their step.  The next stage's first ones are read behind the barrier, which
+  // therefore stands kAhead units before the stage's end: by then nothing of this stage is left to
+  // read, and its buffer takes the stage behind the next.  (kAhead 2, 3, 4 and 5 are within 1% of
+  // each other; the loads ahead of the reads behind the barrier 1% slower.)
+  static constexpr int kUnits = kSteps * CB, kAhead = CB > 3 ? 3 : CB, kBarrier = kUnits - kAhead;
 
   // Over k values of k.  The four buffers are variables of their own, so that the compiler knows
   // which loads a read of the LDS has to wait for.
@@ -207,42 +216,71 @@ struct TileProduct {
 #pragma unroll
     for (int r = 0; r < RB; ++r) {
 #pragma unroll
-      for (int c = 0; c < CB; ++c) {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) sums[r][c][i] = 0.0f;
-      }
+      for (int c = 0; c < CB; ++c) sums[r][c] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     }
     const int stages = static_cast<int>((k + kStageValues<T> - 1) / kStageValues<T>);
+    const int wr = wave_row(), wc = wave_col();
+    F qf[kUnits], qn[kAhead], pf[kSteps][RB], pn[RB];
+    auto unit_of = [&](const char* lds, int u) {
+      return Q::fragment(lds, wc, u % CB, u / CB);
+    };
+    auto rows_of = [&](const char* lds, int step, F(&f)[RB]) {
+#pragma unroll
+      for (int r = 0; r < RB; ++r) f[r] = P::fragment(lds, wr, r, step);
+    };
+    // the stage in (pc, qc), then on to the one in (pn_, qn_)
+    auto turn = [&](char* pc, char* qc, char* pn_, char* qn_) {
+#pragma unroll
+      for (int u = 0; u < kUnits; ++u) {
+        if (u == kBarrier) {
+          stage_barrier<0>();
+          rows_of(pn_, 0, pn);
+          qn[0] = unit_of(qn_, 0);
+          p.load(pc);
+          q.load(qc);
+        } else if (u < kBarrier) {
+          qf[u + kAhead] = unit_of(qc, u + kAhead);
+        } else {
+          qn[u - kBarrier] = unit_of(qn_, u - kBarrier);
+        }
+        if (u % CB == CB - kAhead && u / CB + 1 < kSteps) rows_of(pc, u / CB + 1, pf[u / CB + 1]);
+#pragma unroll
+        for (int r = 0; r < RB; ++r)
+          sums[r][u % CB] = multiply(qf[u], pf[u / CB][r], sums[r][u % CB]);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) qf[u] = qn[u];
+#pragma unroll
+      for (int r = 0; r < RB; ++r) pf[0][r] = pn[r];
+    };
     p.load(p0);
     q.load(q0);
-    // two stages a turn: one behind the last reads as zeros (a branch around it would give its
+    stage_barrier<0>();
+    p.load(p1);
+    q.load(q1);
+    rows_of(p0, 0, pf[0]);
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) qf[u] = unit_of(q0, u);
+    // two stages a turn: those behind the last read as zeros (a branch around one would give its
     // sums registers of their own, and spill)
     for (int s = 0; s < stages; s += 2) {
-      stage_barrier<0>();
-      p.load(p1);
-      q.load(q1);
-      stage(p0, q0);
-      stage_barrier<0>();
-      p.load(p0);
-      q.load(q0);
-      stage(p1, q1);
+      turn(p0, q0, p1, q1);
+      turn(p1, q1, p0, q0);
     }
     stage_barrier<0>();
   }
 
-  // Calls f(row, column of the first of 4 consecutive columns, block row, block column, quarter)
-  // for each group of sums that lie in consecutive columns: values 4 quarter .. + 3 of the block.
-  template <typename F>
-  __device__ __forceinline__ void each(F&& f) const {
+  // Calls f(row, column of the first of 4 consecutive columns, the 4 sums) for the lane's sums.
+  template <typename F_>
+  __device__ __forceinline__ void each(F_&& f) const {
     const int lane = static_cast<int>(threadIdx.x) & (kWave - 1);
 #pragma unroll
     for (int r = 0; r < RB; ++r) {
 #pragma unroll
-      for (int c = 0; c < CB; ++c) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          f(wave_row() + r * 32 + (lane & 31), wave_col() + c * 32 + 8 * i + 4 * (lane >> 5), r, c, i);
-      }
+      for (int c = 0; c < CB; ++c)
+        f(wave_row() + r * kBlockRows + (lane & 15),
+          wave_col() + c * kBlockRows + 4 * (lane >> 4), sums[r][c]);
     }
   }
 };
