@@ -58,19 +58,82 @@ __device__ __forceinline__ void row_sums(float (&v)[N], int tpr, float (*lds)[N]
   }
 }
 
-struct NormBuffers {  // of two rows in turn
-  float mean[2][kMaxWaves][1], dots[2][kMaxWaves][3], again[2][kMaxWaves][1];
+// What a row is reduced to: its mean (RMSNorm: 0), and with d = x - mean the sums of d^2, g d
+// and g.
+struct RowDots {
+  float m, dd, gd, g;
 };
+struct NormBuffers {  // of two rows in turn
+  RowDots dots[2][kMaxWaves];
+  float again[2][kMaxWaves][1];
+  float counts[kMaxWaves];  // LayerNorm: values that each wave has of a row
+};
+
+// `mine`: the dots of the lane's wave (tpr <= 64: of its group, and the row's already) about that
+// wave's own mean.  Those of the row: with M the mean of the waves' means m_w by their counts n_w,
+// d^2 grows by n_w (m_w - M)^2 and g d by (m_w - M) g_w.  One barrier a row where sums about the
+// row's mean would take two.
+template <bool LN>
+__device__ __forceinline__ RowDots row_dots(RowDots mine, int tpr, float inv_n, RowDots* dots,
+                                            const float* counts) {
+  if (tpr <= kWave) return mine;
+  const int wave = static_cast<int>(threadIdx.x) >> 6;
+  const int nwaves = tpr >> 6;
+  const int first = first_wave_of_group(wave, nwaves, tpr);
+  if ((threadIdx.x & (kWave - 1)) == 0) dots[wave] = mine;
+  __syncthreads();
+  RowDots all{0.0f, 0.0f, 0.0f, 0.0f};
+  if constexpr (LN) {
+    for (int w = 0; w < nwaves; ++w) all.m = fmaf(dots[first + w].m, counts[first + w], all.m);
+    all.m *= inv_n;
+  }
+  for (int w = 0; w < nwaves; ++w) {
+    const RowDots o = dots[first + w];
+    const float off = LN ? o.m - all.m : 0.0f;
+    all.dd += LN ? fmaf(off * off, counts[first + w], o.dd) : o.dd;
+    all.gd += LN ? fmaf(off, o.g, o.gd) : o.gd;
+    all.g += o.g;
+  }
+  return all;
+}
 
 __device__ __forceinline__ bool out_of_range(float v) { return !(__builtin_fabsf(v) <= 0x1p127f); }
 
-// The workgroup's rows.  dw, db: the lane's sums.  True where the gradients of a row of
-// the lane's group need sum(g u), which has to wait for r, as sum(g d) leaves the range
-// of 32 bits or may lose terms below 2^-149 (r past 2^20, where eps is next to nothing).
-// AGAIN goes over the rows once more and stores those rows' dx.
-template <typename T, typename W, int V, int IT, bool LN, bool RAGGED, bool AGAIN>
-__device__ __forceinline__ bool norm_rows(const NormGradArgs& a, NormBuffers& lds,
-                                          float (&dw)[IT][V], float (&db)[IT][V]) {
+// V weights in their storage type.
+template <typename W, int V> struct NormWeights {
+  static constexpr int kPart = V * static_cast<int>(sizeof(W)) > 16 ? V / 2 : V;  // one access
+  typename Raw<W, kPart>::type part[V / kPart];
+  __device__ __forceinline__ void load(const W* w, const Span& s) {
+#pragma unroll
+    for (int i = 0; i < V / kPart; ++i) part[i] = load_any<W, kPart, false>(w + i * kPart, s);
+  }
+  __device__ __forceinline__ float at(int k) const {
+    return raw_at<W, kPart>(part[k / kPart], k % kPart);
+  }
+  // keeps 16-bit weights as they are from row to row, instead of their widened values
+  __device__ __forceinline__ void keep() { reload_barrier<W, kPart, V / kPart>(part); }
+};
+
+// The lane's fp32 sums of dw and db.
+template <int V, int IT> struct NormSums {
+  float dw[IT][V], db[IT][V];
+};
+
+// The workgroup's rows.  True where the gradients of a row of the lane's group need sum(g u),
+// which has to wait for r, as sum(g d) leaves the range of 32 bits or may lose terms below 2^-149
+// (r past 2^20, where eps is next to nothing).  AGAIN goes over the rows once more and stores
+// those rows' dx.
+//
+// The next row's loads are in flight while a row is worked on: in registers, or (AHEAD, where a
+// lane has more than two whole vectors of a row) straight into the LDS, each wave's in its own part
+// without a barrier.  There a wave counts what it has to wait for: its loads and stores complete in
+// order, and behind a row's loads come the IT stores of the row before, whatever its lanes have of
+// that (buffer stores, of which those beyond the resource's range are dropped).  (With two vectors a
+// lane, one or two rows ahead in the LDS are slower: 8192 x 4096 bf16 LayerNorm 52.3 and 50.5 us, in
+// registers 46.9.)
+template <typename T, typename W, int V, int IT, bool LN, bool RAGGED, bool AHEAD, bool AGAIN>
+__device__ __forceinline__ bool norm_rows(const NormGradArgs& a, NormBuffers& lds, char* slot,
+                                          NormSums<V, IT>& sums) {
   typedef typename Raw<T, V>::type R;
   const GroupShape gs = group_shape(a.tpr);
   const NormLane<V, IT> l(gs.g, a.tpr, a.cols);
@@ -80,51 +143,97 @@ __device__ __forceinline__ bool norm_rows(const NormGradArgs& a, NormBuffers& ld
   const Span sy = VBH_SPAN(static_cast<T*>(a.dx), a.rows * a.cols);
   const Span sw = VBH_SPAN(static_cast<const W*>(a.w), a.cols);
   const float inv_n = 1.0f / static_cast<float>(a.cols);
-  float w[IT][V];
-#pragma unroll
-  for (int i = 0; i < IT; ++i) {
-    if constexpr (sizeof(W) == sizeof(T)) {
-      const auto raw = load_any<W, V, false>(static_cast<const W*>(a.w) + l.at[i], sw);
-#pragma unroll
-      for (int k = 0; k < V; ++k) w[i][k] = raw_at<W, V>(raw, k);
-    } else {  // fp32 weights of 16-bit rows, in two halves
-      constexpr int H = V > 1 ? V / 2 : 1;
-#pragma unroll
-      for (int h = 0; h < V / H; ++h) {
-        const auto raw = load_any<W, H, false>(static_cast<const W*>(a.w) + l.at[i] + h * H, sw);
-#pragma unroll
-        for (int k = 0; k < H; ++k) w[i][h * H + k] = raw_at<W, H>(raw, k);
-      }
-    }
-  }
+  // lanes with several vectors of a row share it with their whole wave
+  constexpr bool kWaveRow = IT > 1;
+  const int width = kWaveRow || a.tpr > kWave ? kWave : a.tpr;
   // value k of vector i counts
   auto counts = [&](int i, int k) { return RAGGED ? k >= l.skip[i] : l.skip[i] == 0; };
 
   const int64_t step = static_cast<int64_t>(gridDim.x) * gs.per_block;
-  int64_t row = static_cast<int64_t>(blockIdx.x) * gs.per_block + gs.sub;
+  const int64_t base = static_cast<int64_t>(blockIdx.x) * gs.per_block;
   // every group makes as many turns as the workgroup's first (barriers); in turns past
   // the last row it works on row 0 again, and nothing of it counts
-  const int64_t base = static_cast<int64_t>(blockIdx.x) * gs.per_block;
   const int64_t turns = base < a.rows ? (a.rows - base + step - 1) / step : 0;
+  int64_t row = base + (kWaveRow ? __builtin_amdgcn_readfirstlane(gs.sub) : gs.sub);
   bool again = false;
-  R xr[IT], gr[IT];
-  auto load = [&](int64_t to, R (&xs)[IT], R (&gr2)[IT]) {
+  R xr[IT], gr[IT], xn[AHEAD ? 1 : IT], gn[AHEAD ? 1 : IT];
+  auto load = [&](int64_t to, R* xs, R* gs_) {
     const int64_t at = (to < a.rows ? to : 0) * a.cols;
 #pragma unroll
     for (int i = 0; i < IT; ++i) {
-      xs[i] = load_any<T, V, true>(x + at + l.at[i], sx);
-      gr2[i] = load_any<T, V, true>(dy + at + l.at[i], sg);
+      if (a.nt) {
+        xs[i] = load_any<T, V, true>(x + at + l.at[i], sx);
+        gs_[i] = load_any<T, V, true>(dy + at + l.at[i], sg);
+      } else {
+        xs[i] = load_any<T, V, false>(x + at + l.at[i], sx);
+        gs_[i] = load_any<T, V, false>(dy + at + l.at[i], sg);
+      }
     }
   };
-  if (turns > 0) load(row, xr, gr);
+  const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6);
+  const int lane = static_cast<int>(threadIdx.x) & (kWave - 1);
+  auto place = [&](int j) { return slot + (wave * 2 * IT + j) * kWave * 16; };  // j-th access
+  auto stage = [&](int64_t to) {
+    if constexpr (AHEAD) {
+      const int64_t at = (to < a.rows ? to : 0) * a.cols;
+      typedef __attribute__((address_space(1))) const void global_void;
+      typedef __attribute__((address_space(3))) void lds_void;
+#pragma unroll
+      for (int i = 0; i < IT; ++i) {
+        const T* px = x + at + l.at[i];
+        const T* pg = dy + at + l.at[i];
+        if (VBH_IN_SPAN(sx, px, 16))
+          __builtin_amdgcn_global_load_lds((global_void*)px, (lds_void*)place(2 * i), 16, 0, 2);
+        if (VBH_IN_SPAN(sg, pg, 16))
+          __builtin_amdgcn_global_load_lds((global_void*)pg, (lds_void*)place(2 * i + 1), 16, 0,
+                                           2);
+      }
+    }
+  };
+  if (turns > 0) {
+    if constexpr (AHEAD) {
+      stage(row);
+    } else {
+      load(row, xr, gr);
+    }
+  }
+  NormWeights<W, V> w[IT];
+#pragma unroll
+  for (int i = 0; i < IT; ++i) w[i].load(static_cast<const W*>(a.w) + l.at[i], sw);
+  // LayerNorm: values of a row that the lane's wave (tpr < 64: group) holds
+  float inv_mine = 0.0f;
+  if constexpr (LN) {
+    float mine = 0.0f;
+#pragma unroll
+    for (int i = 0; i < IT; ++i) mine += static_cast<float>(RAGGED ? V - l.skip[i] : counts(i, 0) * V);
+    mine = wave_allreduce<Sum>(mine, width);
+    if (lane == 0) lds.counts[wave] = mine;
+    inv_mine = mine > 0.0f ? 1.0f / mine : 0.0f;
+  }
+
   for (int64_t turn = 0; turn < turns; ++turn, row += step) {
     const bool live = row < a.rows;
     const int buf = static_cast<int>(turn & 1);
-    R xn[IT], gn[IT];
-    if (turn + 1 < turns) load(row + step, xn, gn);
-    float m = 0.0f;
+    if constexpr (AHEAD) {
+      if (turn == 0) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      else asm volatile("s_waitcnt vmcnt(%0)" ::"n"(IT) : "memory");
+#pragma unroll
+      for (int i = 0; i < IT; ++i) {
+        xr[i] = *reinterpret_cast<const R*>(place(2 * i) + lane * 16);
+        gr[i] = *reinterpret_cast<const R*>(place(2 * i + 1) + lane * 16);
+      }
+      // read before the next row's loads write there
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      if (turn + 1 < turns) stage(row + step);
+    } else {
+      if (turn + 1 < turns) load(row + step, xn, gn);
+    }
+    if constexpr (IT > 2) {
+#pragma unroll
+      for (int i = 0; i < IT; ++i) w[i].keep();
+    }
+    RowDots dots{0.0f, 0.0f, 0.0f, 0.0f};
     if constexpr (LN) {
-      float sum[1] = {0.0f};
 #pragma unroll
       for (int i = 0; i < IT; ++i) {
         float part = 0.0f;
@@ -133,65 +242,89 @@ __device__ __forceinline__ bool norm_rows(const NormGradArgs& a, NormBuffers& ld
           const float v = raw_at<T, V>(xr[i], k);
           part += RAGGED && !counts(i, k) ? 0.0f : v;
         }
-        sum[0] += RAGGED || counts(i, 0) ? part : 0.0f;
+        dots.m += RAGGED || counts(i, 0) ? part : 0.0f;
       }
-      row_sums<1>(sum, a.tpr, lds.mean[buf]);
-      m = sum[0] * inv_n;
+      dots.m = wave_allreduce<Sum>(dots.m, width) * inv_mine;
       reload_barrier<T, V, IT>(xr);
     }
-    float dots[3] = {0.0f, 0.0f, 0.0f};  // d^2, g d, g
 #pragma unroll
     for (int i = 0; i < IT; ++i) {
       float part[3] = {0.0f, 0.0f, 0.0f};
 #pragma unroll
       for (int k = 0; k < V; ++k) {
         const bool ok = !RAGGED || counts(i, k);
-        const float d = ok ? raw_at<T, V>(xr[i], k) - m : 0.0f;
-        const float g = ok ? raw_at<T, V>(gr[i], k) * w[i][k] : 0.0f;
+        const float d = ok ? raw_at<T, V>(xr[i], k) - dots.m : 0.0f;
+        const float g = ok ? raw_at<T, V>(gr[i], k) * w[i].at(k) : 0.0f;
         part[0] = fmaf(d, d, part[0]);
         part[1] = fmaf(g, d, part[1]);
         if (LN) part[2] += g;
       }
-#pragma unroll
-      for (int j = 0; j < 3; ++j) dots[j] += RAGGED || counts(i, 0) ? part[j] : 0.0f;
+      const bool ok = RAGGED || counts(i, 0);
+      dots.dd += ok ? part[0] : 0.0f;
+      dots.gd += ok ? part[1] : 0.0f;
+      if (LN) dots.g += ok ? part[2] : 0.0f;
     }
-    row_sums<3>(dots, a.tpr, lds.dots[buf]);
+    dots.dd = wave_allreduce<Sum>(dots.dd, width);
+    dots.gd = wave_allreduce<Sum>(dots.gd, width);
+    if constexpr (LN) dots.g = wave_allreduce<Sum>(dots.g, width);
+    dots = row_dots<LN>(dots, a.tpr, inv_n, lds.dots[buf], lds.counts);
     reload_barrier<T, V, IT>(xr);
     reload_barrier<T, V, IT>(gr);
-    const float r = 1.0f / __builtin_sqrtf(fmaf(dots[0], inv_n, a.eps));
-    const bool needs = live && (out_of_range(dots[1]) || r > 0x1p20f);
+    const float r = 1.0f / __builtin_sqrtf(fmaf(dots.dd, inv_n, a.eps));
+    const bool needs = live && (out_of_range(dots.gd) || r > 0x1p20f);
     again = again || needs;
-    float mean_gu = dots[1] * r * inv_n;
+    float mean_gu = dots.gd * r * inv_n;
     if constexpr (AGAIN) {
       float dot[1] = {0.0f};
 #pragma unroll
       for (int i = 0; i < IT; ++i) {
 #pragma unroll
         for (int k = 0; k < V; ++k) {
-          const float u = (raw_at<T, V>(xr[i], k) - m) * r;
-          dot[0] += counts(i, k) ? raw_at<T, V>(gr[i], k) * w[i][k] * u : 0.0f;
+          const float u = (raw_at<T, V>(xr[i], k) - dots.m) * r;
+          dot[0] += counts(i, k) ? raw_at<T, V>(gr[i], k) * w[i].at(k) * u : 0.0f;
         }
       }
       row_sums<1>(dot, a.tpr, lds.again[buf]);
       mean_gu = dot[0] * inv_n;
     }
-    const float mean_g = dots[2] * inv_n;
+    const float mean_g = dots.g * inv_n;
     T* out = static_cast<T*>(a.dx) + (live ? row : 0) * a.cols;
+    // staged: the workgroup's rows of this turn
+    const int64_t at0 = (base + turn * step) * a.cols;
+    const int64_t left = (a.rows * a.cols - at0) * static_cast<int64_t>(sizeof(T));
+    __amdgpu_buffer_rsrc_t rsrc;
+    if constexpr (AHEAD)
+      rsrc = __builtin_amdgcn_make_buffer_rsrc(
+          static_cast<T*>(a.dx) + at0, static_cast<short>(0),
+          __builtin_amdgcn_readfirstlane(static_cast<int>(left < 0x40000000 ? left : 0x40000000)),
+          kRawBufferWord3);
 #pragma unroll
     for (int i = 0; i < IT; ++i) {
       float o[V];
 #pragma unroll
       for (int k = 0; k < V; ++k) {
-        const float u = (raw_at<T, V>(xr[i], k) - m) * r;
+        const float u = (raw_at<T, V>(xr[i], k) - dots.m) * r;
         const float gy = raw_at<T, V>(gr[i], k);
         // r last: g r may leave the range of 32 bits
-        o[k] = r * (fmaf(gy, w[i][k], -mean_g) - u * mean_gu);
+        o[k] = r * (fmaf(gy, w[i].at(k), -mean_g) - u * mean_gu);
         if constexpr (!AGAIN) {
           // sums of values that do not count are not written: only rows that are not
           // the group's have to stay out
-          dw[i][k] = live ? fmaf(gy, u, dw[i][k]) : dw[i][k];
-          if (LN) db[i][k] = live ? db[i][k] + gy : db[i][k];
+          sums.dw[i][k] = live ? fmaf(gy, u, sums.dw[i][k]) : sums.dw[i][k];
+          if (LN) sums.db[i][k] = live ? sums.db[i][k] + gy : sums.db[i][k];
         }
+      }
+      if constexpr (AHEAD) {
+        typedef int i32x4 __attribute__((ext_vector_type(4)));
+        R res;
+#pragma unroll
+        for (int k = 0; k < V; ++k) res[k] = static_cast<T>(o[k]);
+        const bool store = (AGAIN ? needs : live) && l.skip[i] == 0 &&
+                           VBH_IN_SPAN(sy, out + l.at[i], 16);
+        const int to = (gs.sub * a.cols + l.at[i]) * static_cast<int>(sizeof(T));
+        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(i32x4, res), rsrc,
+                                               store ? to : 0x7fffff00, 0, kCacheNtSc1);
+        continue;
       }
       if (AGAIN ? !needs : !live) continue;
       if (l.skip[i] == 0) {
@@ -202,77 +335,111 @@ __device__ __forceinline__ bool norm_rows(const NormGradArgs& a, NormBuffers& ld
           if (counts(i, k)) store_any<T, 1, true>(out + l.at[i] + k, o + k, sy);
       }
     }
+    if constexpr (!AHEAD) {
 #pragma unroll
-    for (int i = 0; i < IT; ++i) {
-      xr[i] = xn[i];
-      gr[i] = gn[i];
+      for (int i = 0; i < IT; ++i) {
+        xr[i] = xn[i];
+        gr[i] = gn[i];
+      }
     }
   }
   return again;
 }
 
-// Lanes of a wave that hold the same columns (groups of tpr < 64 lanes) added up.
+// The workgroup's sums of one vector into row `row` of parts.  Lanes of a wave that hold the same
+// columns are added up first; then groups other than the first leave theirs in the LDS, a lane's
+// next to its neighbour's, and the first one adds them in order.
 template <int V, int IT>
-__device__ __forceinline__ void add_groups(float (&v)[IT][V], int tpr) {
+__device__ __forceinline__ void write_sums(const NormGradArgs& a, float (&v)[IT][V], float* lds,
+                                           int64_t row) {
+  constexpr int F = V < 4 ? 1 : 4;  // values of an access
+  typedef typename Raw<float, F>::type four;
+  const int lane_tpr = a.tpr;
+  const int tpr = max(lane_tpr, kWave);
+  const GroupShape gs = group_shape(tpr);
+  const NormLane<V, IT> l(lane_tpr < kWave ? gs.g & (lane_tpr - 1) : gs.g, lane_tpr, a.cols);
+  if (lane_tpr < kWave) {
 #pragma unroll
-  for (int i = 0; i < IT; ++i) {
+    for (int i = 0; i < IT; ++i) {
 #pragma unroll
-    for (int k = 0; k < V; ++k) {
-      for (int s = tpr; s < kWave; s *= 2) v[i][k] += __shfl_xor(v[i][k], s);
+      for (int k = 0; k < V; ++k) {
+        for (int s = lane_tpr; s < kWave; s *= 2) v[i][k] += __shfl_xor(v[i][k], s);
+      }
     }
   }
-}
-
-// The workgroup's sums of one vector into its row of parts, group after group.
-template <int V, int IT>
-__device__ __forceinline__ void write_sums(const NormGradArgs& a, const float (&v)[IT][V],
-                                           float* sums, int64_t row) {
-  const int tpr = max(a.tpr, kWave);  // a wave's groups are one by now
-  const GroupShape gs = group_shape(tpr);
-  const NormLane<V, IT> l(gs.g & (a.tpr - 1), a.tpr, a.cols);
-  const NormLane<V, IT> lane = a.tpr < kWave ? l : NormLane<V, IT>(gs.g, a.tpr, a.cols);
-  const bool owner = a.tpr >= kWave || gs.g < a.tpr;
-  for (int q = 0; q < gs.per_block; ++q) {
-    if (owner && gs.sub == q) {
+  four* const all = reinterpret_cast<four*>(lds);
+  auto place = [&](int q, int i, int h) { return ((q - 1) * IT + i) * (V / F) * tpr + h * tpr + gs.g; };
+  if (gs.per_block > 1) {
+    __syncthreads();
+    if (gs.sub > 0) {
 #pragma unroll
       for (int i = 0; i < IT; ++i) {
 #pragma unroll
-        for (int k = 0; k < V; ++k) {
-          if (k < lane.skip[i]) continue;
-          float* to = sums + lane.at[i] + k;
-          *to = q == 0 ? v[i][k] : *to + v[i][k];
+        for (int h = 0; h < V / F; ++h) {
+          four f;
+          if constexpr (F == 1) f = v[i][h];
+          else f = four{v[i][4 * h], v[i][4 * h + 1], v[i][4 * h + 2], v[i][4 * h + 3]};
+          all[place(gs.sub, i, h)] = f;
         }
       }
     }
     __syncthreads();
   }
+  if (gs.sub != 0 || gs.g >= lane_tpr) return;
   float* out = a.parts + row * a.pitch;
   const Span sp = VBH_SPAN(a.parts, a.part_rows * a.pitch);
-  for (int c = static_cast<int>(threadIdx.x); c < a.cols; c += static_cast<int>(blockDim.x))
-    store_any<float, 1, false>(out + c, sums + c, sp);
-  __syncthreads();
-}
-
-template <typename T, typename W, int V, int IT, bool LN, bool RAGGED, int BLOCK>
-__global__ __launch_bounds__(BLOCK) void norm_grads(const NormGradArgs a) {
-  extern __shared__ __align__(16) float norm_sums[];
-  __shared__ NormBuffers lds;
-  float dw[IT][V], db[IT][V];
 #pragma unroll
   for (int i = 0; i < IT; ++i) {
 #pragma unroll
-    for (int k = 0; k < V; ++k) dw[i][k] = db[i][k] = 0.0f;
+    for (int h = 0; h < V / F; ++h) {
+      float o[F];
+#pragma unroll
+      for (int k = 0; k < F; ++k) o[k] = v[i][h * F + k];
+      for (int q = 1; q < gs.per_block; ++q) {
+        const four f = all[place(q, i, h)];
+#pragma unroll
+        for (int k = 0; k < F; ++k) {
+          if constexpr (F == 1) o[k] += f;
+          else o[k] += f[k];
+        }
+      }
+      if (l.skip[i] == 0) {
+        store_any<float, F, false>(out + l.at[i] + h * F, o, sp);
+      } else {
+#pragma unroll
+        for (int k = 0; k < F; ++k)
+          if (h * F + k >= l.skip[i])
+            store_any<float, 1, false>(out + l.at[i] + h * F + k, o + k, sp);
+      }
+    }
   }
-  const bool again = norm_rows<T, W, V, IT, LN, RAGGED, false>(a, lds, dw, db);
+}
+
+// Lanes of a workgroup at most: rows of more than two vectors for each of 1024 lanes take 512 lanes
+// of twice the registers (2048 rows of 20480 bf16 values, LayerNorm: 1024 lanes of three vectors
+// spill 40 registers and take 83.6 us, 512 of five 71.3).
+constexpr int norm_lanes(int it) { return it > 2 ? kMaxBlock / 2 : kMaxBlock; }
+
+template <typename T, typename W, int V, int IT, bool LN, bool RAGGED, bool AHEAD>
+__global__ __launch_bounds__(norm_lanes(IT)) void norm_grads(const NormGradArgs a) {
+  // the row ahead; behind them all, the sums of groups other than the first
+  constexpr int kBytes = norm_lanes(IT) * IT * (AHEAD ? 32 : IT > 2 ? 0 : V * 4);
+  __shared__ __align__(16) char slot[kBytes > 0 ? kBytes : 16];
+  __shared__ NormBuffers lds;
+  NormSums<V, IT> sums;
+#pragma unroll
+  for (int i = 0; i < IT; ++i) {
+#pragma unroll
+    for (int k = 0; k < V; ++k) sums.dw[i][k] = sums.db[i][k] = 0.0f;
+  }
+  const bool again =
+      norm_rows<T, W, V, IT, LN, RAGGED, AHEAD, false>(a, lds, slot, sums);
   if (__builtin_expect(__syncthreads_or(again), 0))
-    norm_rows<T, W, V, IT, LN, RAGGED, true>(a, lds, dw, db);
+    norm_rows<T, W, V, IT, LN, RAGGED, AHEAD, true>(a, lds, slot, sums);
   if (a.parts == nullptr) return;
-  add_groups<V, IT>(dw, a.tpr);
-  write_sums<V, IT>(a, dw, norm_sums, blockIdx.x);
-  if constexpr (LN) {
-    add_groups<V, IT>(db, a.tpr);
-    write_sums<V, IT>(a, db, norm_sums, gridDim.x + blockIdx.x);
-  }
+  float* const beside = reinterpret_cast<float*>(slot);
+  write_sums<V, IT>(a, sums.dw, beside, blockIdx.x);
+  if constexpr (LN) write_sums<V, IT>(a, sums.db, beside, gridDim.x + blockIdx.x);
 }
 
 // ---------------------------------------------------------------------------
@@ -365,11 +532,12 @@ __global__ __launch_bounds__(kWideLanes) void norm_wide_apply(const NormGradArgs
 // sums over the rows of parts
 // ---------------------------------------------------------------------------
 
-// A workgroup: 16 columns of one vector, four to a lane and 256 lines of lanes, so that
-// 256 rows take one round of loads.  Lines are added up through the wave, waves through
-// the LDS, in order.
-constexpr int kPartCols = 16;
-constexpr int kPartLanes = 1024;
+// A workgroup: 32 columns of one vector, four to a lane (whole 128-byte lines), and 64 lines of
+// lanes that take up to four rows at a time, so that 256 rows take one round of loads.  Lines are
+// added up through the wave, waves through the LDS, in order.
+constexpr int kPartCols = 32;
+constexpr int kPartLanes = 512;
+constexpr int kPartLines = kPartLanes / (kPartCols / 4);
 
 template <typename W>
 __global__ __launch_bounds__(kPartLanes) void norm_weight_grads(const float* parts, int rows,
@@ -382,22 +550,30 @@ __global__ __launch_bounds__(kPartLanes) void norm_weight_grads(const float* par
   const int lane = static_cast<int>(threadIdx.x) & (kWave - 1);
   const int wave = static_cast<int>(threadIdx.x) >> 6;
   const int64_t col = static_cast<int64_t>(blockIdx.x) * kPartCols;
-  const int line = wave * 16 + lane / 4;
-  const float* from = parts + blockIdx.y * static_cast<int64_t>(rows) * pitch + col + (lane & 3) * 4;
+  const int64_t mine = col + (lane & 7) * 4;
+  const int line = wave * 8 + (lane >> 3);
+  const float* from = parts + blockIdx.y * static_cast<int64_t>(rows) * pitch + mine;
   float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-  if (col + (lane & 3) * 4 < pitch) {
-    for (int r = line; r < rows; r += kPartLanes / 4) {
-      float x[4];
-      load_f32<float, 4>(from + r * pitch, x, sp);
+  if (mine < pitch) {
+    for (int r = line; r < rows; r += 4 * kPartLines) {
+      float x[4][4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) v[i] += x[i];
+      for (int j = 0; j < 4; ++j) {
+        const int at = r + j * kPartLines;  // rows behind the last: the first of them again
+        load_f32<float, 4>(from + static_cast<int64_t>(at < rows ? at : r) * pitch, x[j], sp);
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] += r + j * kPartLines < rows ? x[j][i] : 0.0f;
+      }
     }
   }
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    for (int s = 4; s < kWave; s *= 2) v[i] += __shfl_xor(v[i], s);
+    for (int s = 8; s < kWave; s *= 2) v[i] += __shfl_xor(v[i], s);
   }
-  if (lane < 4) {
+  if (lane < 8) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) sums[wave][lane * 4 + i] = v[i];
   }
@@ -414,7 +590,7 @@ __global__ __launch_bounds__(kPartLanes) void norm_weight_grads(const float* par
 // launches
 // ---------------------------------------------------------------------------
 
-constexpr int kNormMaxIt = 4;
+constexpr int64_t kNormMaxVectors = 4 * kMaxBlock;  // of a row in registers
 constexpr int64_t kNormCus = 256;
 
 // How a launch is laid out, a function of its sizes and types alone.
@@ -429,7 +605,7 @@ NormShape norm_shape(int64_t rows, int64_t cols, int dt) {
   const int vn = dt == kF32 ? 4 : 8;
   s.v = cols >= vn ? vn : 1;
   const int64_t nvec = (cols + s.v - 1) / s.v;
-  if (nvec > int64_t(kNormMaxIt) * kMaxBlock) {
+  if (nvec > kNormMaxVectors) {
     s.wide = true;
     s.grid = std::max<int64_t>(std::min<int64_t>(rows, 64), 1);
     return s;
@@ -437,16 +613,19 @@ NormShape norm_shape(int64_t rows, int64_t cols, int dt) {
   if (nvec <= kWave) {
     s.tpr = 1;
     while (s.tpr < nvec) s.tpr *= 2;
-  } else if (nvec <= int64_t(kNormMaxIt) * kWave) {
-    s.it = static_cast<int>((nvec + kWave - 1) / kWave);
+  } else if (nvec <= 2 * kWave) {
+    s.it = 2;
   } else {
-    s.it = nvec <= 2 * kMaxBlock ? 2 : static_cast<int>((nvec + kMaxBlock - 1) / kMaxBlock);
+    s.it = 2;
+    if (nvec > 2 * kMaxBlock) {
+      s.it = static_cast<int>((nvec + kMaxBlock / 2 - 1) / (kMaxBlock / 2));
+      if (s.it == 7) s.it = 8;
+    }
     s.tpr = static_cast<int>((nvec + int64_t(s.it) * kWave - 1) / (int64_t(s.it) * kWave)) * kWave;
   }
   // as many groups to a workgroup as leave every CU one
-  const int most = s.it > 2 ? 512 : 1024;
   s.block = std::max(s.tpr, 256 / s.tpr * s.tpr);
-  while (s.block + s.tpr <= most && rows >= kNormCus * (s.block / s.tpr + 1)) s.block += s.tpr;
+  while (s.block + s.tpr <= norm_lanes(s.it) && rows >= kNormCus * (s.block / s.tpr + 1)) s.block += s.tpr;
   if (s.tpr < kWave) s.block = std::max(s.block / kWave * kWave, kWave);
   const int64_t per = s.block / s.tpr;
   s.grid = std::max<int64_t>(std::min<int64_t>((rows + per - 1) / per, kNormCus), 1);
@@ -469,25 +648,27 @@ hipError_t launch_norm(NormGradArgs a, const NormShape& s, float* stats, hipStre
     return hipGetLastError();
   }
   a.tpr = s.tpr;
+  // nontemporal loads where the launch moves more than the last-level cache keeps from the kernel
+  // before it (bf16 LayerNorm / RMSNorm, us without and with: 2048 x 8192, 100 MB, 29.5 / 23.5 and
+  // 34.0 / 26.1; 8192 x 4096, 201 MB, 44.9 / 41.7 and 45.0 / 39.9)
+  a.nt = 3 * a.rows * a.cols * static_cast<int64_t>(sizeof(T)) > (int64_t(128) << 20);
+  constexpr int VN = Vec<T>::n;
   auto go = [&](auto kernel) {
-    const unsigned bytes = a.parts != nullptr ? static_cast<unsigned>(a.cols * sizeof(float)) : 0;
-    launch_kernel(kernel, dim3(static_cast<unsigned>(s.grid)), dim3(s.block), bytes, stream, a);
+    launch_kernel(kernel, dim3(static_cast<unsigned>(s.grid)), dim3(s.block), 0, stream, a);
     err = hipGetLastError();
   };
-  constexpr int VN = Vec<T>::n;
-  dispatch_bool(s.v > 1 && a.cols % VN != 0, [&](auto rc) {
-    constexpr bool RAGGED = decltype(rc)::value;
-    auto by_it = [&](auto ic) {
-      constexpr int IT = decltype(ic)::value;
-      if (IT > 2 && s.block <= 512) go(norm_grads<T, W, VN, IT, LN, RAGGED, IT <= 2 ? 1024 : 512>);
-      else go(norm_grads<T, W, VN, IT, LN, RAGGED, 1024>);
-    };
-    if (s.v == 1) go(norm_grads<T, W, 1, 1, LN, false, 1024>);
-    else if (s.it == 1) by_it(std::integral_constant<int, 1>{});
-    else if (s.it == 2) by_it(std::integral_constant<int, 2>{});
-    else if (s.it == 3) by_it(std::integral_constant<int, 3>{});
-    else by_it(std::integral_constant<int, 4>{});
-  });
+  const bool whole = a.cols % VN == 0 && reinterpret_cast<uintptr_t>(a.x) % 16 == 0 &&
+                     reinterpret_cast<uintptr_t>(a.dy) % 16 == 0;
+  auto by_it = [&](auto wc) {
+    constexpr bool WHOLE = decltype(wc)::value;
+    if (s.it == 1) go(norm_grads<T, W, VN, 1, LN, !WHOLE, false>);
+    else if (s.it == 2) go(norm_grads<T, W, VN, 2, LN, !WHOLE, false>);
+    else if (s.it == 5) go(norm_grads<T, W, VN, 5, LN, !WHOLE, WHOLE>);
+    else if (s.it == 6) go(norm_grads<T, W, VN, 6, LN, !WHOLE, WHOLE>);
+    else go(norm_grads<T, W, VN, 8, LN, !WHOLE, WHOLE>);
+  };
+  if (s.v == 1) go(norm_grads<T, W, 1, 1, LN, false, false>);
+  else dispatch_bool(whole, by_it);
   return err;
 }
 

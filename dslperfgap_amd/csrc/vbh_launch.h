@@ -386,6 +386,7 @@ struct NormGradArgs {
   float eps = 0.0f;
   // set by the launcher
   int tpr = 64;                       // lanes per row
+  int nt = 0;                         // nontemporal loads
   float* parts = nullptr;             // [part_rows][pitch]: dw's rows, then db's
   int64_t part_rows = 0, pitch = 0;
 };
