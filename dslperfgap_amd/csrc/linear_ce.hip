@@ -37,9 +37,34 @@ constexpr int kRowsLanes = 1024;
 
 // What the kernels behind lce_rows read of it.
 struct LceInfo {
-  int live;    // tokens that count
-  int shift;   // of dL's power of two
+  int live;        // tokens that count
+  int shift;       // of dL's power of two
+  int splits;      // of a piece's columns in the product that gives dx (dx_splits)
+  int split_cols;  // in each
 };
+
+// How many workgroups share a tile of dx, each with a part of the piece's columns, so that `tiles`
+// tiles of `stages` stages fill the card: by the time of its rounds of workgroups in stages, each
+// with kRoundStages for its start and end, and that of the parts' sums, which pass through memory
+// in kSumBytes a stage.  At most kSplitRounds rounds of workgroups that share.  One count to a lane
+// of a wave.
+constexpr int kSplitRounds = 4, kMostSplits = 16, kLeastSplit = 256;
+constexpr int kRoundStages = 12, kSumBytes = 4 << 20;
+__device__ __forceinline__ int dx_splits(int64_t tiles, int slots, int cols, int value_bytes,
+                                         int64_t out_bytes) {
+  const int s = (static_cast<int>(threadIdx.x) & (kWave - 1)) + 1;
+  if (tiles > kSplitRounds * slots) return 1;
+  const int n = static_cast<int>(tiles) * s;
+  const int stages = (cols * value_bytes + kStageBytes - 1) / kStageBytes;
+  float time = static_cast<float>((n + slots - 1) / slots) *
+               static_cast<float>((stages + s - 1) / s + kRoundStages);
+  if (s > 1) time += 2.0f * s * static_cast<float>(out_bytes) * (1.0f / kSumBytes);
+  if (s > kMostSplits || (s > 1 && (n > kSplitRounds * slots || cols < s * kLeastSplit)))
+    time = __builtin_huge_valf();
+  float least = time;
+  for (int i = 1; i < kWave; i *= 2) least = fminf(least, __shfl_xor(least, i));
+  return __builtin_ctzll(__ballot(time == least)) + 1;
+}
 
 __device__ __forceinline__ int64_t label_at(const LceArgs& a, int64_t t) {
   const Span s64 = VBH_SPAN(static_cast<const int64_t*>(a.labels), a.tokens);
@@ -61,63 +86,86 @@ __device__ __forceinline__ void store_one(T* p, T v, const Span& s) {
   if (VBH_IN_SPAN(s, p, sizeof(T))) *p = v;
 }
 
-// Numbers the tokens that count: rows[i] is the i-th one's, place[t] token t's number or -1.
-// One workgroup, each lane a run of consecutive tokens.  Backward: the largest |dL| that a
-// token's dloss, scale and lse allow.
+// Numbers the tokens that count: rows[i] is the i-th one's, place[t] token t's number or -1.  One
+// workgroup, kRowsEach times as many consecutive tokens at a time as it has lanes, their loads in
+// flight together.  Backward: the largest |dL| that a token's dloss, scale and lse allow, and how
+// dx's product is shared out.
+constexpr int kRowsEach = 8;
+constexpr int kRowsWaves = kRowsLanes / kWave;
+
 __global__ __launch_bounds__(kRowsLanes) void lce_rows(const LceArgs a) {
-  __shared__ int counts[kRowsLanes / kWave];
-  __shared__ float most[kRowsLanes / kWave];
+  __shared__ int counts[2][kRowsEach * kRowsWaves];
+  __shared__ float most[kRowsWaves];
   const int lane = static_cast<int>(threadIdx.x) & (kWave - 1);
   const int wave = static_cast<int>(threadIdx.x) >> 6;
-  const int64_t each = (a.tokens + kRowsLanes - 1) / kRowsLanes;
-  const int64_t first = min(each * threadIdx.x, a.tokens), last = min(first + each, a.tokens);
   const Span sd = VBH_SPAN(a.dloss, a.tokens), sl = VBH_SPAN(a.lse_in, a.tokens);
   const Span sr = VBH_SPAN(a.rows, a.tokens), sp = VBH_SPAN(a.place, a.tokens);
-  int count = 0;
+  int live = 0, turn = 0;
   float size = 0.0f;
-  for (int64_t t = first; t < last; ++t) {
-    if (label_at(a, t) == a.ignored) continue;
-    ++count;
-    if (a.dloss == nullptr) continue;
-    const float f = 1.0f + 2.0f * a.lse_square_scale * load_one(a.lse_in + t, sl);
-    const float b = __builtin_fabsf(load_one(a.dloss + t, sd) * a.scale) * (1.0f + __builtin_fabsf(f));
-    if (b <= 0x1p127f) size = fmaxf(size, b);  // what is not finite stays as it is
+  for (int64_t chunk = 0; chunk < a.tokens; chunk += kRowsLanes * kRowsEach, turn ^= 1) {
+    bool counts_too[kRowsEach];
+    float dloss[kRowsEach], lse[kRowsEach];
+#pragma unroll
+    for (int j = 0; j < kRowsEach; ++j) {
+      const int64_t t = chunk + j * kRowsLanes + threadIdx.x, at = min(t, a.tokens - 1);
+      counts_too[j] = t < a.tokens && label_at(a, at) != a.ignored;
+      if (a.dloss != nullptr) {
+        dloss[j] = load_one(a.dloss + at, sd);
+        lse[j] = load_one(a.lse_in + at, sl);
+      }
+    }
+    uint64_t which[kRowsEach];
+#pragma unroll
+    for (int j = 0; j < kRowsEach; ++j) {
+      which[j] = __ballot(counts_too[j]);
+      if (lane == 0) counts[turn][j * kRowsWaves + wave] = __popcll(which[j]);
+      if (a.dloss == nullptr || !counts_too[j]) continue;
+      const float f = 1.0f + 2.0f * a.lse_square_scale * lse[j];
+      const float b = __builtin_fabsf(dloss[j] * a.scale) * (1.0f + __builtin_fabsf(f));
+      if (b <= 0x1p127f) size = fmaxf(size, b);  // what is not finite stays as it is
+    }
+    __syncthreads();
+    // every wave sums up the counts: two of the 128 to a lane
+    const int mine = counts[turn][2 * lane], next = counts[turn][2 * lane + 1];
+    int sum = mine + next;
+    for (int s = 1; s < kWave; s *= 2) {
+      const int other = __shfl_up(sum, s);
+      if (lane >= s) sum += other;
+    }
+    const int before = sum - mine - next;
+#pragma unroll
+    for (int j = 0; j < kRowsEach; ++j) {
+      const int64_t t = chunk + j * kRowsLanes + threadIdx.x;
+      const int slot = j * kRowsWaves + wave;
+      const int base = __shfl(before, slot / 2) + (slot & 1 ? __shfl(mine, slot / 2) : 0);
+      const int at = live + base + __popcll(which[j] & ((uint64_t(1) << lane) - 1));
+      if (t >= a.tokens) continue;
+      store_one(a.place + t, counts_too[j] ? at : -1, sp);
+      if (counts_too[j]) store_one(a.rows + at, static_cast<int>(t), sr);
+    }
+    live += __shfl(sum, kWave - 1);
   }
-  int before = count;
-  for (int s = 1; s < kWave; s *= 2) {
-    const int other = __shfl_up(before, s);
-    if (lane >= s) before += other;
-    size = fmaxf(size, __shfl_xor(size, s));
-  }
-  if (lane == kWave - 1) {
-    counts[wave] = before;
-    most[wave] = size;
-  }
-  before -= count;
+  for (int s = 1; s < kWave; s *= 2) size = fmaxf(size, __shfl_xor(size, s));
+  if (lane == 0) most[wave] = size;
   __syncthreads();
-  int live = 0;
-  size = 0.0f;
-  for (int w = 0; w < kRowsLanes / kWave; ++w) {
-    if (w < wave) before += counts[w];
-    live += counts[w];
-    size = fmaxf(size, most[w]);
+  if (wave != 0) return;
+  for (int w = 1; w < kRowsWaves; ++w) size = fmaxf(size, most[w]);
+  const int exponent = size > 0.0f ? __builtin_amdgcn_frexp_expf(size) : 10;
+  LceInfo info{live, min(max(10 - exponent, -100), 100), 1, 0};
+  if (a.dx != nullptr) {
+    const int64_t tiles = static_cast<int64_t>((live + a.dx_rows - 1) / a.dx_rows) * a.dx_cols;
+    const int splits = dx_splits(tiles, a.dx_slots, a.first_cols, a.value_bytes,
+                                 live * a.padded * 4);
+    info.split_cols = (a.first_cols + splits * 128 - 1) / (splits * 128) * 128;
+    info.splits = (a.first_cols + info.split_cols - 1) / info.split_cols;
   }
-  for (int64_t t = first; t < last; ++t) {
-    const bool counts_too = label_at(a, t) != a.ignored;
-    store_one(a.place + t, counts_too ? before : -1, sp);
-    if (counts_too) store_one(a.rows + before++, static_cast<int>(t), sr);
-  }
-  if (threadIdx.x == 0) {
-    LceInfo* info = static_cast<LceInfo*>(a.info);
-    const Span si = VBH_SPAN(info, 1);
-    const int exponent = size > 0.0f ? __builtin_amdgcn_frexp_expf(size) : 10;
-    store_one(info, LceInfo{live, min(max(10 - exponent, -100), 100)}, si);
-  }
+  LceInfo* to = static_cast<LceInfo*>(a.info);
+  if (lane == 0) store_one(to, info, VBH_SPAN(to, 1));
 }
 
 __device__ __forceinline__ LceInfo lce_info(const LceArgs& a) {
   const LceInfo* info = static_cast<const LceInfo*>(a.info);
-  if (info == nullptr) return LceInfo{static_cast<int>(a.tokens), 0};
+  if (info == nullptr) return LceInfo{static_cast<int>(a.tokens), 0, 1, 0};
   return load_one(info, VBH_SPAN(info, 1));
 }
 
@@ -200,19 +248,21 @@ __global__ __launch_bounds__(kGatherRows* kWave) void lce_pad_weight(const LceAr
 constexpr int kTileRows = 4;
 constexpr int kDies = 8;
 struct TileAt {
-  int row, col;
+  int row, col, split;
   bool live;
 };
-__device__ __forceinline__ TileAt tile_at(int rows, int cols) {
-  const int n = rows * cols, each = (n + kDies - 1) / kDies;
+__device__ __forceinline__ TileAt tile_at(int rows, int cols, int splits = 1) {
+  const int each_split = rows * cols, n = each_split * splits, each = (n + kDies - 1) / kDies;
   const int i = static_cast<int>(blockIdx.x) / kDies;
-  const int id = static_cast<int>(blockIdx.x) % kDies * each + i;
-  if (i >= each || id >= n) return TileAt{0, 0, false};
+  int id = static_cast<int>(blockIdx.x) % kDies * each + i;
+  if (i >= each || id >= n) return TileAt{0, 0, 0, false};
+  const int split = splits > 1 ? id / each_split : 0;
+  id -= split * each_split;
   const int group = id / (kTileRows * cols), in = id - group * kTileRows * cols;
   const int deep = min(kTileRows, rows - group * kTileRows);
-  return TileAt{group * kTileRows + in % deep, in / deep, true};
+  return TileAt{group * kTileRows + in % deep, in / deep, split, true};
 }
-int64_t tile_grid(int64_t rows, int64_t cols) { return (rows * cols + kDies - 1) / kDies * kDies; }
+int64_t tile_grid(int64_t tiles) { return (tiles + kDies - 1) / kDies * kDies; }
 
 struct LsePart {
   float m, s;  // max, sum of exp(L - m): 0 where m is -inf
@@ -223,9 +273,9 @@ __device__ __forceinline__ LsePart join(const LsePart& a, const LsePart& b) {
   return LsePart{m, a.s * fast_exp(a.m - by) + b.s * fast_exp(b.m - by)};
 }
 
-#define VBH_TILE_BUFFERS(G)                                                         \
-  __shared__ __align__(128) char p0[G::P::kBytes], p1[G::P::kBytes], q0[G::Q::kBytes], \
-      q1[G::Q::kBytes]
+#define VBH_TILE_BUFFERS(G)                                                     \
+  __shared__ __align__(128) char p0[G::kPBuffer], p1[G::kPBuffer], q0[G::kQBuffer], \
+      q1[G::kQBuffer]
 
 // Logits of `rows` x `cols` tiles: x's row tiles against W's from `first` on (`cols_left` rows of
 // W).  The operands of tile `at`.
@@ -239,7 +289,7 @@ __device__ __forceinline__ void logits(const LceArgs& a, G& g, const TileAt& at,
   typename G::P p(x.p + r0 * x.ld, x.ld, live - r0, a.padded, x.span);
   typename G::Q q(w + first * a.w_stride, a.w_stride, cols_left, a.padded,
                   VBH_SPAN(w, (a.vocab - 1) * a.w_stride + a.padded));
-  g.run(p, q, a.padded, p0, p1, q0, q1);
+  g.run(p, q, a.padded, at.col % G::kFroms, p0, p1, q0, q1);
 }
 
 template <typename T, typename G>
@@ -336,13 +386,14 @@ __global__ __launch_bounds__(G::kLanes) void lce_forward(const LceArgs a) {
     store_one(a.totals + to, total, VBH_SPAN(a.totals, a.col_tiles * a.tokens));
 }
 
-// One token per group of kJoinLanes lanes of a workgroup, each with every kJoinLanes-th tile.
-constexpr int kJoinRows = 32;
+// kJoinRows tokens to a workgroup, each kJoinLanes lanes with every kJoinLanes-th tile: 8 of them in
+// a wave, whose parts are joined in it, then 4 waves' through the LDS.
+constexpr int kJoinRows = 8;
 constexpr int kJoinLanes = 32;
 
 __global__ __launch_bounds__(kJoinRows* kJoinLanes) void lce_join(const LceArgs a) {
-  __shared__ LsePart parts[kJoinLanes][kJoinRows];
-  __shared__ float totals[kJoinLanes][kJoinRows];
+  __shared__ LsePart parts[kJoinLanes / 8][kJoinRows];
+  __shared__ float totals[kJoinLanes / 8][kJoinRows];
   const int r = static_cast<int>(threadIdx.x) % kJoinRows;
   const int q = static_cast<int>(threadIdx.x) / kJoinRows;
   const int64_t t = static_cast<int64_t>(blockIdx.x) * kJoinRows + r;
@@ -355,16 +406,33 @@ __global__ __launch_bounds__(kJoinRows* kJoinLanes) void lce_join(const LceArgs 
   LsePart all{-__builtin_huge_valf(), 0.0f};
   float total = 0.0f;
   if (counts) {
-    for (int64_t k = q; k < a.col_tiles; k += kJoinLanes) {
-      all = join(all, load_one(from + k * a.tokens + row, sp));
-      if (a.smoothing != 0.0f) total += load_one(a.totals + k * a.tokens + row, st);
+    for (int64_t k = q; k < a.col_tiles; k += 4 * kJoinLanes) {
+      LsePart part[4];  // four tiles' loads in flight
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int64_t at = k + j * kJoinLanes < a.col_tiles ? k + j * kJoinLanes : k;
+        part[j] = load_one(from + at * a.tokens + row, sp);
+        if (a.smoothing != 0.0f) {
+          const float more = load_one(a.totals + at * a.tokens + row, st);
+          total += j == 0 || at != k ? more : 0.0f;
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (k + j * kJoinLanes < a.col_tiles) all = join(all, part[j]);
     }
   }
-  parts[q][r] = all;
-  totals[q][r] = total;
+  for (int s = kJoinRows; s < kWave; s *= 2) {
+    all = join(all, LsePart{__shfl_xor(all.m, s), __shfl_xor(all.s, s)});
+    total += __shfl_xor(total, s);
+  }
+  if ((threadIdx.x & (kWave - 1)) < kJoinRows) {
+    parts[q / 8][r] = all;
+    totals[q / 8][r] = total;
+  }
   __syncthreads();
   if (q != 0 || t >= a.tokens) return;
-  for (int k = 1; k < kJoinLanes; ++k) {
+  for (int k = 1; k < kJoinLanes / 8; ++k) {
     all = join(all, parts[k][r]);
     total += totals[k][r];
   }
@@ -462,7 +530,7 @@ __global__ __launch_bounds__(G::kLanes) void lce_dweight(const LceArgs a) {
   typename G::P p(piece + r0, a.pitch, info.live, a.pitch - r0, VBH_SPAN(piece, info.live * a.pitch));
   typename G::Q q(x.p + c0, x.ld, info.live, a.padded - c0, x.span);
   G g;
-  g.run(p, q, info.live, p0, p1, q0, q1);
+  g.run(p, q, info.live, 0, p0, p1, q0, q1);
   T* dw = static_cast<T*>(a.dw);
   const Span sd = VBH_SPAN(dw, a.vocab * a.hidden);
   g.each([&](int row, int col, const f32x4& sums) {
@@ -474,39 +542,37 @@ __global__ __launch_bounds__(G::kLanes) void lce_dweight(const LceArgs a) {
   });
 }
 
-// dx's part from the piece's columns of split blockIdx.y: dL W.  One split and one piece: dx
-// itself; else into (`more`: onto) the split's fp32 sums.
+// dx's part from one split's columns of the piece: dL W, into (`more`: onto) the split's fp32 sums,
+// [splits][live][padded]; of a single split the last piece's gives dx itself.
 template <typename T, typename G>
-__global__ __launch_bounds__(G::kLanes) void lce_dx(const LceArgs a, int more) {
+__global__ __launch_bounds__(G::kLanes) void lce_dx(const LceArgs a, int more, int last) {
   VBH_TILE_BUFFERS(G);
   const LceInfo info = lce_info(a);
   const TileAt at = tile_at((info.live + G::BR - 1) / G::BR,
-                            static_cast<int>((a.hidden + G::BC - 1) / G::BC));
+                            static_cast<int>((a.hidden + G::BC - 1) / G::BC), info.splits);
   if (!at.live) return;
   const int64_t r0 = static_cast<int64_t>(at.row) * G::BR, c0 = static_cast<int64_t>(at.col) * G::BC;
-  const int64_t k0 = blockIdx.y * a.split_cols, k = min(a.cols - k0, a.split_cols);
+  const int64_t k0 = static_cast<int64_t>(at.split) * info.split_cols;
+  const int64_t k = min(a.cols - k0, static_cast<int64_t>(info.split_cols));
+  if (k <= 0) return;  // a shorter last piece: those before it have summed into every split
   const T* piece = static_cast<const T*>(a.piece);
   const T* w = static_cast<const T*>(a.w);
   typename G::P p(piece + r0 * a.pitch + k0, a.pitch, info.live - r0,
-                  min(a.pitch - k0, a.split_cols), VBH_SPAN(piece, info.live * a.pitch));
+                  min(a.pitch - k0, static_cast<int64_t>(info.split_cols)),
+                  VBH_SPAN(piece, info.live * a.pitch));
   typename G::Q q(w + (a.first + k0) * a.w_stride + c0, a.w_stride, k, a.padded - c0,
                   VBH_SPAN(w, (a.vocab - 1) * a.w_stride + a.padded));
   G g;
-  g.run(p, q, k, p0, p1, q0, q1);
+  g.run(p, q, k, 0, p0, p1, q0, q1);
   T* dx = static_cast<T*>(a.dx);
   const Span sd = VBH_SPAN(dx, a.tokens * a.hidden);
-  const Span ss = VBH_SPAN(a.dx_sums, a.splits * a.tokens * a.padded);
+  const Span ss = VBH_SPAN(a.dx_sums, a.dx_sum_floats);
+  const bool direct = last && info.splits == 1;
   g.each([&](int row, int col, const f32x4& sums) {
     if (r0 + row >= info.live || c0 + col >= a.hidden) return;
     float o[4];
-    if (a.dx_sums == nullptr) {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) o[j] = ldexpf(sums[j], -info.shift);
-      const int64_t t = load_one(a.rows + r0 + row, VBH_SPAN(a.rows, a.tokens));
-      store_four(dx + t * a.hidden, c0 + col, a.hidden, o, sd);
-      return;
-    }
-    float* to = a.dx_sums + (blockIdx.y * a.tokens + r0 + row) * a.padded + c0 + col;
+    float* to = a.dx_sums +
+                (static_cast<int64_t>(at.split) * info.live + r0 + row) * a.padded + c0 + col;
     if (more) {
       load_f32<float, 4>(to, o, ss);
     } else {
@@ -515,31 +581,48 @@ __global__ __launch_bounds__(G::kLanes) void lce_dx(const LceArgs a, int more) {
     }
 #pragma unroll
     for (int j = 0; j < 4; ++j) o[j] += sums[j];
-    store_from_f32<float, 4>(to, o, ss);
-  });
-}
-
-// dx from the splits' sums.
-template <typename T>
-__global__ __launch_bounds__(kGatherRows* kWave) void lce_dx_join(const LceArgs a) {
-  const LceInfo info = lce_info(a);
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * kGatherRows + (threadIdx.x >> 6);
-  if (row >= info.live) return;
-  const int64_t t = load_one(a.rows + row, VBH_SPAN(a.rows, a.tokens));
-  T* dx = static_cast<T*>(a.dx);
-  const Span sd = VBH_SPAN(dx, a.tokens * a.hidden);
-  const Span ss = VBH_SPAN(a.dx_sums, a.splits * a.tokens * a.padded);
-  for (int64_t c = (threadIdx.x & (kWave - 1)) * 4; c < a.hidden; c += kWave * 4) {
-    float o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int s = 0; s < a.splits; ++s) {
-      float v[4];
-      load_f32<float, 4>(a.dx_sums + (s * a.tokens + row) * a.padded + c, v, ss);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) o[j] += v[j];
+    if (!direct) {
+      store_from_f32<float, 4>(to, o, ss);
+      return;
     }
 #pragma unroll
     for (int j = 0; j < 4; ++j) o[j] = ldexpf(o[j], -info.shift);
-    store_four(dx + t * a.hidden, c, a.hidden, o, sd);
+    const int64_t t = load_one(a.rows + r0 + row, VBH_SPAN(a.rows, a.tokens));
+    store_four(dx + t * a.hidden, c0 + col, a.hidden, o, sd);
+  });
+}
+
+// dx from the splits' sums, four of a row's columns to a lane, kSumRows rows to a workgroup.
+constexpr int kSumLanes = 256;
+constexpr int kSumRows = 4;
+
+template <typename T>
+__global__ __launch_bounds__(kSumLanes) void lce_dx_join(const LceArgs a) {
+  const LceInfo info = lce_info(a);
+  const int64_t c = (static_cast<int64_t>(blockIdx.y) * kSumLanes + threadIdx.x) * 4;
+  if (info.splits == 1 || c >= a.hidden) return;
+  T* dx = static_cast<T*>(a.dx);
+  const Span ss = VBH_SPAN(a.dx_sums, a.dx_sum_floats);
+  const int64_t step = info.live * a.padded;
+  const int64_t first = static_cast<int64_t>(blockIdx.x) * kSumRows;
+  for (int64_t row = first; row < min(first + kSumRows, static_cast<int64_t>(info.live)); ++row) {
+    const int64_t t = load_one(a.rows + row, VBH_SPAN(a.rows, a.tokens));
+    const float* from = a.dx_sums + row * a.padded + c;
+    float o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int s = 0; s < info.splits; s += 4) {
+      float v[4][4];  // four splits' loads in flight
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        load_f32<float, 4>(from + (s + i < info.splits ? s + i : s) * step, v[i], ss);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) o[j] += s + i < info.splits ? v[i][j] : 0.0f;
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) o[j] = ldexpf(o[j], -info.shift);
+    store_four(dx + t * a.hidden, c, a.hidden, o, VBH_SPAN(dx, a.tokens * a.hidden));
   }
 }
 
@@ -554,46 +637,63 @@ __global__ __launch_bounds__(kGatherRows* kWave) void lce_zero(T* p, int64_t n) 
 // launches
 // ---------------------------------------------------------------------------
 
-// Tiles, by size and type:
-//   kBig   256 x 256 on 8 waves, one workgroup per CU: 16-bit products that fill the card with them
-//   kMid   128 x 128 on 4 waves, two per CU: 0.85 of kBig's rate (8192 x 8192 x 8192: 1151 against
-//          1375 TFLOP/s), in quarters of its portions; fp32 always, whose matrix instructions take
-//          as long as the reads for either (125-134 TFLOP/s; the library's best 117-122)
-//   kSmall 64 x 128, kTiny 32 x 128 on 4 waves: products of at most as many rows, whose time is
-//          the read of W
-enum Tile { kBig, kMid, kSmall, kTiny };
+// Tiles.  A CU's time with a share of n tiles is n times the tile's work over its rate, both against
+// kBig's (MI355X, TFLOP/s, bf16 4096 x 8192 x 4096 deep, fp32 2048 x 8192 x 1024):
+//   kBig   256 x 256 on 8 waves, one workgroup per CU          1250 (8192 x 8192 x 8192: 1375)
+//   kMid   128 x 128 on 4 waves, two per CU                     990, fp32 121
+//   kSmall  64 x 128 on 4 waves                                 876, fp32 135
+//   kTiny   32 x 128 on 4 waves                                 600, fp32 126
+//   kDeep   32 x 64 on 4 waves, three stages ahead: rows by rows of at most 32, whose time is the
+//           read of Q
+// (The library's best fp32 kernel reaches 118: its matrix instructions take as long as the reads
+// for any tile.)
+enum Tile { kBig, kMid, kSmall, kTiny, kDeep };
 template <typename T, bool P_COLUMNS, bool Q_COLUMNS>
 using BigTile = TileProduct<T, 256, 256, 4, 2, P_COLUMNS, Q_COLUMNS>;
 template <typename T, bool P_COLUMNS, bool Q_COLUMNS>
 using MidTile = TileProduct<T, 128, 128, 2, 2, P_COLUMNS, Q_COLUMNS>;
 template <typename T, bool Q_COLUMNS>
-using SmallTile = TileProduct<T, 64, 128, 1, 4, false, Q_COLUMNS>;
+using SmallTile = TileProduct<T, 64, 128, 2, 2, false, Q_COLUMNS>;
 template <typename T, bool Q_COLUMNS>
 using TinyTile = TileProduct<T, 32, 128, 1, 4, false, Q_COLUMNS>;
+template <typename T> using DeepTile = TileProduct<T, 32, 64, 2, 2, false, false, true>;
 
 constexpr int64_t kPlainTokens = 64; // forward of at most these: no numbering of tokens
 constexpr int64_t kPieceBytes = int64_t(256) << 20;
 constexpr int64_t kPieceCols = 4096; // least of a piece
 constexpr int64_t kMostPieceCols = int64_t(1) << 18;
-constexpr int64_t kSplitCols = 1024; // least of a split of dx
 
 int64_t up(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
 int64_t tiles(int64_t n, int64_t each) { return (n + each - 1) / each; }
 int value_bytes(int dt) { return dt == kF32 ? 4 : 2; }
 
-// The tile of a product of `rows` (of P, whose lines have k contiguous unless P_COLUMNS) by `cols`.
-Tile tile_of(int64_t rows, int64_t cols, int dt, bool p_columns = false) {
-  if (!p_columns && rows <= 32) return kTiny;
-  if (!p_columns && rows <= 64) return kSmall;
-  if (dt == kF32) return kMid;
-  // rounds of workgroups, by a round's time
-  const int64_t big = tiles(tiles(rows, 256) * tiles(cols, 256), 256) * 100;
-  const int64_t mid = tiles(tiles(rows, 128) * tiles(cols, 128), 512) * 59;
-  return mid < big ? kMid : kBig;
-}
 int64_t tile_rows(Tile t) { return t == kBig ? 256 : t == kMid ? 128 : t == kSmall ? 64 : 32; }
-int64_t tile_cols(Tile t) { return t == kBig ? 256 : 128; }
-int64_t tile_fill(Tile t) { return t == kBig ? 256 : 512; }  // workgroups that fill the card
+int64_t tile_cols(Tile t) { return t == kBig ? 256 : t == kDeep ? 64 : 128; }
+int64_t tile_slots(Tile t) { return t == kBig ? 256 : t == kMid ? 512 : 768; }  // fill the card
+
+// The tile of a product of `rows` by `cols`, whose tiles up to `most_splits` workgroups share;
+// P_COLUMNS, Q_COLUMNS: operands with k the slow axis.
+Tile tile_of(int64_t rows, int64_t cols, int dt, bool p_columns, bool q_columns,
+             int64_t most_splits = 1) {
+  if (!p_columns && rows <= 32) return q_columns ? kTiny : kDeep;
+  const bool f32 = dt == kF32;
+  const struct {
+    Tile tile;
+    int64_t work;  // percent of kBig's work, over its rate
+  } all[] = {{kBig, 100}, {kMid, f32 ? 27 : 31}, {kSmall, f32 ? 13 : 18}, {kTiny, f32 ? 7 : 14}};
+  Tile best = kMid;
+  int64_t least = int64_t(1) << 62;
+  for (const auto& t : all) {
+    if (t.tile == kBig ? f32 : t.tile > kMid && p_columns) continue;
+    const int64_t n = tiles(rows, tile_rows(t.tile)) * tiles(cols, tile_cols(t.tile));
+    const int64_t time = tiles(n * most_splits, 256) * t.work;
+    if (time < least) {
+      least = time;
+      best = t.tile;
+    }
+  }
+  return best;
+}
 
 // f(TypeTag of the TileProduct)
 template <typename T, bool Q_COLUMNS, typename F>
@@ -605,6 +705,9 @@ void with_tile(Tile t, F&& f) {
     case kMid: f(TypeTag<MidTile<T, false, Q_COLUMNS>>{}); break;
     case kSmall: f(TypeTag<SmallTile<T, Q_COLUMNS>>{}); break;
     case kTiny: f(TypeTag<TinyTile<T, Q_COLUMNS>>{}); break;
+    case kDeep:
+      if constexpr (!Q_COLUMNS) f(TypeTag<DeepTile<T>>{});
+      break;
   }
 }
 
@@ -612,9 +715,9 @@ void with_tile(Tile t, F&& f) {
 struct LcePlan {
   int64_t padded = 0;
   int64_t pieces = 1, piece_cols = 0, pitch = 0;
-  int64_t splits = 1, split_cols = 0;
-  bool sums = false;
+  int64_t dx_sum_floats = 0;
   Tile dx_tile = kBig;
+  int64_t dx_grid = 0;
   int64_t info = 0, rows = 0, place = 0, x = 0, w = 0, parts = 0, totals = 0, picked = 0,
           piece = 0, dx_sums = 0, bytes = 0;
 };
@@ -635,7 +738,7 @@ LcePlan lce_plan(int64_t tokens, int64_t hidden, int64_t vocab, int dt, bool pad
   p.x = take(tokens * p.padded * e);
   if (pad_weight) p.w = take(vocab * p.padded * e);
   if (!backward) {
-    const int64_t n = tiles(vocab, tile_cols(tile_of(tokens, vocab, dt))) * tokens;
+    const int64_t n = tiles(vocab, tile_cols(tile_of(tokens, vocab, dt, false, false))) * tokens;
     p.parts = take(n * sizeof(LsePart));
     p.totals = take(n * 4);
     p.picked = take(tokens * 4);
@@ -649,14 +752,16 @@ LcePlan lce_plan(int64_t tokens, int64_t hidden, int64_t vocab, int dt, bool pad
   p.pieces = tiles(vocab, p.piece_cols);
   p.pitch = up(std::min(p.piece_cols, vocab), 16 / e);
   p.piece = take(tokens * p.pitch * e);
-  const int64_t cols = std::min(p.piece_cols, vocab);  // of the first piece
-  p.dx_tile = tile_of(tokens, hidden, dt);
-  const int64_t out = tiles(tokens, tile_rows(p.dx_tile)) * tiles(hidden, tile_cols(p.dx_tile));
-  p.splits = std::max<int64_t>(std::min(tiles(tile_fill(p.dx_tile), out), cols / kSplitCols), 1);
-  p.split_cols = up(tiles(cols, p.splits), 128);
-  p.splits = tiles(cols, p.split_cols);
-  p.sums = p.splits > 1 || p.pieces > 1;
-  if (p.sums) p.dx_sums = take(p.splits * tokens * p.padded * 4);
+  p.dx_tile = tile_of(tokens, hidden, dt, false, true,
+                      std::max<int64_t>(std::min<int64_t>(p.pitch / kLeastSplit, kMostSplits), 1));
+  // splits are chosen where the number of tokens that count is known: one, or as many as make
+  // kSplitRounds rounds of workgroups at most
+  const int64_t br = tile_rows(p.dx_tile), across = tiles(hidden, tile_cols(p.dx_tile));
+  const int64_t shared = std::min(kSplitRounds * tile_slots(p.dx_tile) / across * br,
+                                  kMostSplits * up(tokens, br));
+  p.dx_grid = std::max(tiles(tokens, br) * across, kSplitRounds * tile_slots(p.dx_tile));
+  p.dx_sum_floats = std::max(tokens, shared) * p.padded;
+  p.dx_sums = take(p.dx_sum_floats * 4);
   return p;
 }
 
@@ -673,11 +778,11 @@ hipError_t forward(LceArgs a, int dt, bool number, hipStream_t s) {
     launch_kernel(lce_gather<T>, dim3(tokens4), dim3(kGatherRows * kWave), 0, s, a);
     if (!done()) return err;
   }
-  const Tile t = tile_of(a.tokens, a.vocab, dt);
+  const Tile t = tile_of(a.tokens, a.vocab, dt, false, false);
   a.col_tiles = static_cast<int>(tiles(a.vocab, tile_cols(t)));
   with_tile<T, false>(t, [&](auto tag) {
     using G = typename decltype(tag)::type;
-    const int64_t grid = tile_grid(tiles(a.tokens, G::BR), a.col_tiles);
+    const int64_t grid = tile_grid(tiles(a.tokens, G::BR) * a.col_tiles);
     launch_kernel(lce_forward<T, G>, dim3(static_cast<unsigned>(grid)), dim3(G::kLanes), 0, s, a);
   });
   if (!done()) return err;
@@ -700,23 +805,23 @@ hipError_t backward(LceArgs a, int dt, const LcePlan& p, hipStream_t s) {
     a.first = i * p.piece_cols;
     a.cols = std::min(p.piece_cols, a.vocab - a.first);
     a.pitch = up(a.cols, 16 / static_cast<int64_t>(sizeof(T)));
-    const Tile t = tile_of(a.tokens, a.cols, dt);
+    const Tile t = tile_of(a.tokens, a.cols, dt, false, false);
     a.col_tiles = static_cast<int>(tiles(a.cols, tile_cols(t)));
     with_tile<T, false>(t, [&](auto tag) {
       using G = typename decltype(tag)::type;
-      const int64_t grid = tile_grid(tiles(a.tokens, G::BR), a.col_tiles);
+      const int64_t grid = tile_grid(tiles(a.tokens, G::BR) * a.col_tiles);
       launch_kernel(lce_dlogits<T, G>, dim3(static_cast<unsigned>(grid)), dim3(G::kLanes), 0, s, a);
     });
     if (!done()) return err;
     if (a.dw != nullptr) {
       auto go = [&](auto tag) {
         using G = typename decltype(tag)::type;
-        const int64_t grid = tile_grid(tiles(a.cols, G::BR), tiles(a.hidden, G::BC));
+        const int64_t grid = tile_grid(tiles(a.cols, G::BR) * tiles(a.hidden, G::BC));
         launch_kernel(lce_dweight<T, G>, dim3(static_cast<unsigned>(grid)), dim3(G::kLanes), 0, s,
                       a);
       };
       if constexpr (sizeof(T) == 2) {
-        if (tile_of(a.cols, a.hidden, dt, true) == kBig) go(TypeTag<BigTile<T, true, true>>{});
+                if (tile_of(a.cols, a.hidden, dt, true, true) == kBig) go(TypeTag<BigTile<T, true, true>>{});
         else go(TypeTag<MidTile<T, true, true>>{});
       } else {
         go(TypeTag<MidTile<T, true, true>>{});
@@ -726,17 +831,16 @@ hipError_t backward(LceArgs a, int dt, const LcePlan& p, hipStream_t s) {
     if (a.dx == nullptr) continue;
     with_tile<T, true>(p.dx_tile, [&](auto tag) {
       using G = typename decltype(tag)::type;
-      const int64_t grid = tile_grid(tiles(a.tokens, G::BR), tiles(a.hidden, G::BC));
-      // a shorter last piece may have fewer splits: those before it have summed into all
-      launch_kernel(lce_dx<T, G>,
-                    dim3(static_cast<unsigned>(grid),
-                         static_cast<unsigned>(tiles(a.cols, a.split_cols))),
-                    dim3(G::kLanes), 0, s, a, i > 0 ? 1 : 0);
+      launch_kernel(lce_dx<T, G>, dim3(static_cast<unsigned>(tile_grid(p.dx_grid))),
+                    dim3(G::kLanes), 0, s, a, i > 0 ? 1 : 0, i + 1 == p.pieces ? 1 : 0);
     });
     if (!done()) return err;
   }
-  if (a.dx != nullptr && p.sums) {
-    launch_kernel(lce_dx_join<T>, dim3(tokens4), dim3(kGatherRows * kWave), 0, s, a);
+  if (a.dx != nullptr) {
+    launch_kernel(lce_dx_join<T>,
+                  dim3(static_cast<unsigned>(tiles(a.tokens, kSumRows)),
+                       static_cast<unsigned>(tiles(a.hidden, 4 * kSumLanes))),
+                  dim3(kSumLanes), 0, s, a);
     done();
   }
   return err;
@@ -774,9 +878,13 @@ hipError_t launch_linear_ce(LceArgs a, int dt, bool back, void* workspace, hipSt
   }
   if (back) {
     a.piece = ws + p.piece;
-    a.splits = static_cast<int>(p.splits);
-    a.split_cols = p.split_cols;
-    if (p.sums) a.dx_sums = reinterpret_cast<float*>(ws + p.dx_sums);
+    a.dx_sums = reinterpret_cast<float*>(ws + p.dx_sums);
+    a.dx_sum_floats = p.dx_sum_floats;
+    a.dx_rows = static_cast<int>(tile_rows(p.dx_tile));
+    a.dx_cols = static_cast<int>(tiles(a.hidden, tile_cols(p.dx_tile)));
+    a.dx_slots = static_cast<int>(tile_slots(p.dx_tile));
+    a.first_cols = static_cast<int>(std::min(p.piece_cols, a.vocab));
+    a.value_bytes = value_bytes(dt);
   } else {
     a.parts = ws + p.parts;
     a.totals = reinterpret_cast<float*>(ws + p.totals);

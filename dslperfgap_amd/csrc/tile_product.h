@@ -82,15 +82,15 @@ struct Operand {
   static_assert(!COLUMNS || kPieces >= 16, "room for the permutation");
 
   __amdgpu_buffer_rsrc_t rsrc;
-  const T* base;     // of the resource
+  const T* base;     // of the resource: the next stage's first line
   int64_t line;      // bytes from one line to the next
   int64_t extent;    // bytes from base to the operand's end
-  uint32_t offset;   // of the lane's first piece from the resource's base
+  uint32_t offset;   // of the lane's first piece from base
   int k_left;        // rows: values of k that the lane's pieces have ahead of them
   Span span;
 
-  // `base`: the tile's first line (columns: and first row) at k = 0; `lines`: lines from there on
-  // that the operand has; `values`: values of a line from base on.
+  // `from`: the tile's first line (columns: and first row) at k = 0; `lines`: lines from there on
+  // that the operand has; `values`: values of a line from there on.
   __device__ __forceinline__ Operand(const T* from, int64_t ld, int64_t lines, int64_t values,
                                      const Span& s)
       : base(from), line(ld * static_cast<int64_t>(sizeof(T))), span(s) {
@@ -109,6 +109,14 @@ struct Operand {
     rsrc = __builtin_amdgcn_make_buffer_rsrc(
         const_cast<T*>(base), static_cast<short>(0),
         __builtin_amdgcn_readfirstlane(static_cast<int>(bytes)), kRawBufferWord3);
+  }
+  // On (or back) by `stages`.
+  __device__ __forceinline__ void move(int stages) {
+    const int64_t by = stages * (COLUMNS ? kStageValues<T> * line : kStageBytes);
+    base = reinterpret_cast<const T*>(reinterpret_cast<const char*>(base) + by);
+    extent -= by;
+    k_left -= stages * kStageValues<T>;
+    range();
   }
 
   // The next stage into `lds` (kBytes), and on to the one behind it.
@@ -129,11 +137,7 @@ struct Operand {
       __builtin_amdgcn_raw_ptr_buffer_load_lds(
           rsrc, (lds_void*)(lds + (j * LANES + wave * kWave) * 16), 16, at, more, 0, 0);
     }
-    const int64_t step = COLUMNS ? kStageValues<T> * line : kStageBytes;
-    base = reinterpret_cast<const T*>(reinterpret_cast<const char*>(base) + step);
-    extent -= step;
-    k_left -= kStageValues<T>;
-    range();
+    move(1);
   }
 
   // The lane's fragment of the 16 rows of block `block` from row `base` (a multiple of 32) on at
@@ -183,7 +187,10 @@ __device__ __forceinline__ void stage_barrier() {
   asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(PENDING) : "memory");
 }
 
-template <typename T, int BR_, int BC_, int WR_, int WC_, bool P_COLUMNS, bool Q_COLUMNS>
+// DEEP: four buffers of a whole stage instead of two, three stages ahead, for products of so few rows
+// that their time is the read of Q.
+template <typename T, int BR_, int BC_, int WR_, int WC_, bool P_COLUMNS, bool Q_COLUMNS,
+          bool DEEP = false>
 struct TileProduct {
   static constexpr int BR = BR_, BC = BC_, WR = WR_, WC = WC_;
   static constexpr int kLanes = WR * WC * kWave;
@@ -191,6 +198,9 @@ struct TileProduct {
   typedef Operand<T, BR, kLanes, P_COLUMNS> P;
   typedef Operand<T, BC, kLanes, Q_COLUMNS> Q;
   typedef typename Frag<T>::type F;
+  // of the kernel's four buffers
+  static constexpr int kPBuffer = DEEP ? P::kBytes + Q::kBytes : P::kBytes;
+  static constexpr int kQBuffer = DEEP ? P::kBytes + Q::kBytes : Q::kBytes;
 
   f32x4 sums[RB][CB];
 
@@ -209,9 +219,14 @@ struct TileProduct {
   // each other; the loads ahead of the reads behind the barrier 1% slower.)
   static constexpr int kUnits = kSteps * CB, kAhead = CB > 3 ? 3 : CB, kBarrier = kUnits - kAhead;
 
-  // Over k values of k.  The four buffers are variables of their own, so that the compiler knows
+  // Over k values of k.  The buffers are variables of their own, so that the compiler knows
   // which loads a read of the LDS has to wait for.
-  __device__ __forceinline__ void run(P& p, Q& q, int64_t k, char* p0, char* p1, char* q0,
+  // DEEP: stages are taken in a circle, from the part `from` / kFroms of them on: workgroups that
+  // walk over equally aligned lines in step ask the same memory channels at a time (4 tokens by a
+  // bf16 W of 32000 x 4096: 58.2 us, with each workgroup from a stage of its own 54.5; it makes no
+  // difference to tiles that are bound by the matrix cores).
+  static constexpr int kFroms = 64;
+  __device__ __forceinline__ void run(P& p, Q& q, int64_t k, int from, char* p0, char* p1, char* q0,
                                       char* q1) {
 #pragma unroll
     for (int r = 0; r < RB; ++r) {
@@ -220,6 +235,54 @@ struct TileProduct {
     }
     const int stages = static_cast<int>((k + kStageValues<T> - 1) / kStageValues<T>);
     const int wr = wave_row(), wc = wave_col();
+    if constexpr (DEEP) {
+      constexpr int kLoads = P::kLoads + Q::kLoads;
+      const int first = static_cast<int>(static_cast<int64_t>(stages) * from / kFroms);
+      int loaded = first;  // from the first stage on; past them all, zeros
+      p.move(first);
+      q.move(first);
+      auto load = [&](char* to) {
+        if (loaded == stages) {  // back to the first; behind the last again, past the end
+          p.move(-stages);
+          q.move(-stages);
+        }
+        if (loaded == stages + first) {
+          p.move(stages);
+          q.move(stages);
+        }
+        ++loaded;
+        p.load(to);
+        q.load(to + P::kBytes);
+      };
+      auto work = [&](char* at, char* before) {
+        stage_barrier<2 * kLoads>();
+        load(before);
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) {
+          F a[RB], b[CB];
+#pragma unroll
+          for (int r = 0; r < RB; ++r) a[r] = P::fragment(at, wr, r, s);
+#pragma unroll
+          for (int c = 0; c < CB; ++c) b[c] = Q::fragment(at + P::kBytes, wc, c, s);
+#pragma unroll
+          for (int r = 0; r < RB; ++r) {
+#pragma unroll
+            for (int c = 0; c < CB; ++c) sums[r][c] = multiply(b[c], a[r], sums[r][c]);
+          }
+        }
+      };
+      load(p0);
+      load(p1);
+      load(q0);
+      for (int s = 0; s < stages; s += 4) {
+        work(p0, q1);
+        work(p1, p0);
+        work(q0, p1);
+        work(q1, q0);
+      }
+      stage_barrier<0>();
+      return;
+    }
     F qf[kUnits], qn[kAhead], pf[kSteps][RB], pn[RB];
     auto unit_of = [&](const char* lds, int u) {
       return Q::fragment(lds, wc, u % CB, u / CB);

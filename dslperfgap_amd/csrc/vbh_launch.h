@@ -429,10 +429,13 @@ struct LceArgs {
   float* totals = nullptr;
   float* picked = nullptr;
   void* piece = nullptr;
-  float* dx_sums = nullptr;       // null: one split of one piece
+  float* dx_sums = nullptr;
+  int64_t dx_sum_floats = 0;
   int64_t first = 0, cols = 0, pitch = 0;
-  int64_t split_cols = 0;
-  int splits = 1, col_tiles = 0;
+  int col_tiles = 0;
+  int dx_rows = 1, dx_cols = 1, dx_slots = 1;  // a tile's rows, tiles across, workgroups at once
+  int first_cols = 0;                          // of the first piece
+  int value_bytes = 2;
 };
 int64_t linear_ce_workspace_bytes(int64_t tokens, int64_t hidden, int64_t vocab, int dt,
                                   bool pad_weight, bool backward);

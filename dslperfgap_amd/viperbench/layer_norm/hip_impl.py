@@ -100,6 +100,9 @@ def layer_norm_bwd(dy, x, weight, bias, eps=1e-5):
     if eps != 1e-5:
         raise ValueError(f"Only eps=1e-5 is supported (got {eps}). "
                          "The Triton kernel hardcodes eps=1e-5.")
+    got = _norm_bwd.common(dy, x, weight, bias, 1e-5, True)
+    if got is not None:
+        return got
     what = "layer_norm_bwd"
     norm_shape = tuple(weight.shape)
     k = len(norm_shape)

@@ -91,10 +91,61 @@ def _workspace(x, weight, code, backward):
     return _bridge.empty(x, (nbytes,), torch.uint8), nbytes
 
 
+_raw_device, _raw_stream = _bridge._raw_device, _bridge._raw_stream
+# (shapes and dtypes of x, weight and labels, backward) of a call on contiguous tensors whose weight
+# begins at a multiple of 16 bytes -> (tokens, hidden, classes, type codes, workspace bytes, entry
+# point), or False where a call needs the general path (which raises the errors of invalid calls)
+_PLANS = _bridge.PlanCache()
+
+
+def _plan(xs, ws, dtype, wdtype, ls, ldtype, backward):
+    code, lcode = _bridge.FLOAT_CODES.get(dtype), _bridge.LABEL_CODES.get(ldtype)
+    if (code is None or lcode is None or wdtype is not dtype or len(xs) != 2 or len(ws) != 2 or
+            len(ls) != 1 or xs[1] != ws[1] or ls[0] != xs[0] or 0 in xs or 0 in ws):
+        return False
+    pad = xs[1] * dtype.itemsize % 16 != 0 or xs[1] * dtype.itemsize > 1 << 20
+    nbytes = _workspace_bytes(xs[0], xs[1], ws[0], code, int(pad), int(backward))
+    if not nbytes:
+        return False
+    return (xs[0], xs[1], ws[0], code, lcode, nbytes,
+            _lib.entry("vbh_linear_cross_entropy_bwd" if backward else
+                       "vbh_linear_cross_entropy_fwd"))
+
+
+def _common(x, weight, labels, backward):
+    """The plan of a common call and its device, or (None, -1)."""
+    key = (x.shape, weight.shape, x.dtype, weight.dtype, labels.shape, labels.dtype, backward)
+    p = _PLANS.get(key)
+    if p is None:
+        p = _PLANS.put(key, _plan(*key))
+    if p:
+        dev = x.get_device()
+        if (dev >= 0 and dev == _raw_device() and weight.get_device() == dev and
+                labels.get_device() == dev and x.is_contiguous() and weight.is_contiguous() and
+                labels.is_contiguous() and weight.data_ptr() % 16 == 0):
+            return p, dev
+    return None, -1
+
+
 def linear_cross_entropy_fwd(x, weight, labels, smoothing=0.0, logit_scale=1.0,
                              lse_square_scale=0.0, ignored_index=-100, total_classes=None,
                              class_start_idx=0, SPLIT=False):
     """Per-token loss, lse and z_loss of x @ weight.T against labels; see the module docstring."""
+    p, dev = _common(x, weight, labels, False)
+    if p is not None:
+        tokens, hidden, vocab, code, lcode, nbytes, fn = p
+        loss = x.new_empty_strided((tokens,), (1,), dtype=torch.float32)
+        lse, z_loss = torch.empty_like(loss), torch.empty_like(loss)
+        ws = x.new_empty_strided((nbytes,), (1,), dtype=torch.uint8)
+        rc = fn(x.data_ptr(), weight.data_ptr(), labels.data_ptr(), loss.data_ptr(),
+                lse.data_ptr(), z_loss.data_ptr(), tokens, hidden, vocab, hidden, hidden,
+                float(smoothing), float(logit_scale), float(lse_square_scale),
+                int(ignored_index), vocab if total_classes is None else int(total_classes),
+                int(class_start_idx), code, lcode, int(bool(SPLIT)), ws.data_ptr(), nbytes,
+                _raw_stream(dev))
+        if rc != 0:
+            raise _lib.VbhError("vbh_linear_cross_entropy_fwd", rc, _lib.last_error())
+        return loss, lse, z_loss
     what = "linear_cross_entropy_fwd"
     x, weight, labels, args = _check(what, x, weight, labels, smoothing, logit_scale,
                                      lse_square_scale, ignored_index, total_classes,
@@ -112,6 +163,25 @@ def linear_cross_entropy_bwd(dloss, x, weight, lse, labels, smoothing=0.0, logit
                              lse_square_scale=0.0, ignored_index=-100, total_classes=None,
                              class_start_idx=0, weight_grad=True):
     """The gradients of linear_cross_entropy_fwd's x and weight from that of its loss."""
+    f32 = torch.float32
+    if (dloss.dtype is f32 and lse.dtype is f32 and dloss.shape == labels.shape and
+            lse.shape == labels.shape):
+        p, dev = _common(x, weight, labels, True)
+        if (p is not None and dloss.get_device() == dev and lse.get_device() == dev and
+                dloss.is_contiguous() and lse.is_contiguous()):
+            tokens, hidden, vocab, code, lcode, nbytes, fn = p
+            dx = torch.empty_like(x)
+            dw = torch.empty_like(weight) if weight_grad else None
+            ws = x.new_empty_strided((nbytes,), (1,), dtype=torch.uint8)
+            rc = fn(dloss.data_ptr(), x.data_ptr(), weight.data_ptr(), lse.data_ptr(),
+                    labels.data_ptr(), dx.data_ptr(), dw.data_ptr() if weight_grad else None,
+                    tokens, hidden, vocab, hidden, hidden, float(smoothing), float(logit_scale),
+                    float(lse_square_scale), int(ignored_index),
+                    vocab if total_classes is None else int(total_classes), int(class_start_idx),
+                    code, lcode, ws.data_ptr(), nbytes, _raw_stream(dev))
+            if rc != 0:
+                raise _lib.VbhError("vbh_linear_cross_entropy_bwd", rc, _lib.last_error())
+            return dx, dw
     what = "linear_cross_entropy_bwd"
     x, weight, labels, args = _check(what, x, weight, labels, smoothing, logit_scale,
                                      lse_square_scale, ignored_index, total_classes,

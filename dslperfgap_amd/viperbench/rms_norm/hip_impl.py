@@ -86,6 +86,12 @@ def rms_norm_bwd(dy, x, normalized_shape, weight, eps=1e-5):
     dtype).  The weight's gradient is summed in fp32 in a fixed order and has the weight's
     shape and dtype."""
     what = "rms_norm_bwd"
+    if not (float(eps) >= 0.0 and float(eps) < float("inf")):
+        raise ValueError(f"{what}: eps must be finite and not negative, got {eps}")
+    if tuple(normalized_shape) == tuple(weight.shape):
+        got = _norm_bwd.common(dy, x, weight, None, float(eps), False)
+        if got is not None:
+            return got[:2]
     k = len(tuple(normalized_shape))
     if k > x.dim():
         raise RuntimeError(f"{what}: normalized_shape {tuple(normalized_shape)} has more dims "
@@ -94,8 +100,6 @@ def rms_norm_bwd(dy, x, normalized_shape, weight, eps=1e-5):
     if weight.numel() != cols:
         raise RuntimeError(f"{what}: weight has {weight.numel()} elements, the normalized "
                            f"dims hold {cols}")
-    if not (float(eps) >= 0.0 and float(eps) < float("inf")):
-        raise ValueError(f"{what}: eps must be finite and not negative, got {eps}")
     wide = weight.dtype in (x.dtype, torch.float32)
     dev, dx, dw, args = _norm_bwd.prepare(what, dy, x, weight if wide else weight.float(), None,
                                           eps, False)
