@@ -57,6 +57,15 @@ def test_sizes(dtype, wdtype, layer_norm):
 
 
 @pytest.mark.parametrize("layer_norm", [True, False])
+@pytest.mark.parametrize("dtype,wdtype", [(F32, F32), (BF16, F32), (F16, F16)])
+@pytest.mark.parametrize("rows,cols", [(700, 20480), (513, 24580), (300, 12000), (600, 16384),
+                                       (3000, 2048), (9001, 72), (2049, 520)])
+def test_several_rows_after_each_other(rows, cols, dtype, wdtype, layer_norm):
+    """More rows than the launch holds at once, in each way that rows lie over lanes."""
+    _check(*_make(rows, cols, dtype, wdtype), layer_norm)
+
+
+@pytest.mark.parametrize("layer_norm", [True, False])
 def test_no_rows_give_zero_weight_gradients(layer_norm):
     x, dy, w, b = _make(0, 96, BF16, F32)
     got = layer_norm_bwd(dy, x, w, b) if layer_norm else rms_norm_bwd(dy, x, (96,), w)
