@@ -986,7 +986,7 @@ static int norm_bwd(const char* what, bool ln, const void* dy, const void* x, co
     return fail(VBH_E_INVALID, "%s: negative size", what);
   if (cols > kMaxCols) return fail(VBH_E_RANGE, "%s: cols %lld too large", what,
                                    static_cast<long long>(cols));
-  if (rows > kMaxWorkItems / kMaxBlock || mul_sat(rows, cols) > VBH_NORM_BWD_MAX_VALUES)
+  if (rows > kMaxCols || mul_sat(rows, cols) > VBH_NORM_BWD_MAX_VALUES)
     return fail(VBH_E_RANGE, "%s: %lld x %lld values are more than one launch takes", what,
                 static_cast<long long>(rows), static_cast<long long>(cols));
   if (cols == 0) return 0;
@@ -1541,6 +1541,9 @@ static int linear_ce_workspace_ok(const char* what, const LceArgs& a, int dtype,
                                   const void* workspace, int64_t workspace_bytes) {
   const int64_t need = linear_ce_workspace_bytes(a.tokens, a.hidden, a.vocab, dtype,
                                                  a.w == nullptr, backward);
+  if (need == 0)
+    return fail(VBH_E_RANGE, "%s: %lld tokens x %lld classes are more than one launch takes", what,
+                static_cast<long long>(a.tokens), static_cast<long long>(a.vocab));
   if (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 255u) != 0)
     return fail(VBH_E_INVALID, "%s: needs a workspace of %lld bytes, aligned to 256", what,
                 static_cast<long long>(need));

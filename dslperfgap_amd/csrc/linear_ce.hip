@@ -151,7 +151,7 @@ __global__ __launch_bounds__(kRowsLanes) void lce_rows(const LceArgs a) {
   if (wave != 0) return;
   for (int w = 1; w < kRowsWaves; ++w) size = fmaxf(size, most[w]);
   const int exponent = size > 0.0f ? __builtin_amdgcn_frexp_expf(size) : 10;
-  LceInfo info{live, min(max(10 - exponent, -100), 100), 1, 0};
+  LceInfo info{live, min(max(10 - exponent, -120), 100), 1, 0};
   if (a.dx != nullptr) {
     const int64_t tiles = static_cast<int64_t>((live + a.dx_rows - 1) / a.dx_rows) * a.dx_cols;
     const int splits = dx_splits(tiles, a.dx_slots, a.first_cols, a.value_bytes,
@@ -629,8 +629,9 @@ __global__ __launch_bounds__(kSumLanes) void lce_dx_join(const LceArgs a) {
 // dW where there are no tokens at all.
 template <typename T>
 __global__ __launch_bounds__(kGatherRows* kWave) void lce_zero(T* p, int64_t n) {
-  const int64_t i = static_cast<int64_t>(blockIdx.x) * (kGatherRows * kWave) + threadIdx.x;
-  if (i < n) store_one(p + i, static_cast<T>(0.0f), VBH_SPAN(p, n));
+  constexpr int kEach = kGatherRows * kWave;
+  for (int64_t i = int64_t(blockIdx.x) * kEach + threadIdx.x; i < n; i += int64_t(gridDim.x) * kEach)
+    store_one(p + i, static_cast<T>(0.0f), VBH_SPAN(p, n));
 }
 
 // ---------------------------------------------------------------------------
@@ -767,7 +768,7 @@ LcePlan lce_plan(int64_t tokens, int64_t hidden, int64_t vocab, int dt, bool pad
 
 template <typename T>
 hipError_t forward(LceArgs a, int dt, bool number, hipStream_t s) {
-  const unsigned tokens4 = static_cast<unsigned>(tiles(a.tokens, kGatherRows));
+  const unsigned line_groups = static_cast<unsigned>(tiles(a.tokens, kGatherRows));
   hipError_t err = hipSuccess;
   auto done = [&] { return (err = hipGetLastError()) == hipSuccess; };
   if (number) {
@@ -775,7 +776,7 @@ hipError_t forward(LceArgs a, int dt, bool number, hipStream_t s) {
     if (!done()) return err;
   }
   if (number || !a.x_direct) {
-    launch_kernel(lce_gather<T>, dim3(tokens4), dim3(kGatherRows * kWave), 0, s, a);
+    launch_kernel(lce_gather<T>, dim3(line_groups), dim3(kGatherRows * kWave), 0, s, a);
     if (!done()) return err;
   }
   const Tile t = tile_of(a.tokens, a.vocab, dt, false, false);
@@ -794,12 +795,12 @@ hipError_t forward(LceArgs a, int dt, bool number, hipStream_t s) {
 
 template <typename T>
 hipError_t backward(LceArgs a, int dt, const LcePlan& p, hipStream_t s) {
-  const unsigned tokens4 = static_cast<unsigned>(tiles(a.tokens, kGatherRows));
+  const unsigned line_groups = static_cast<unsigned>(tiles(a.tokens, kGatherRows));
   hipError_t err = hipSuccess;
   auto done = [&] { return (err = hipGetLastError()) == hipSuccess; };
   launch_kernel(lce_rows, dim3(1), dim3(kRowsLanes), 0, s, a);
   if (!done()) return err;
-  launch_kernel(lce_gather<T>, dim3(tokens4), dim3(kGatherRows * kWave), 0, s, a);
+  launch_kernel(lce_gather<T>, dim3(line_groups), dim3(kGatherRows * kWave), 0, s, a);
   if (!done()) return err;
   for (int64_t i = 0; i < p.pieces; ++i) {
     a.first = i * p.piece_cols;
@@ -821,7 +822,7 @@ hipError_t backward(LceArgs a, int dt, const LcePlan& p, hipStream_t s) {
                       a);
       };
       if constexpr (sizeof(T) == 2) {
-                if (tile_of(a.cols, a.hidden, dt, true, true) == kBig) go(TypeTag<BigTile<T, true, true>>{});
+        if (tile_of(a.cols, a.hidden, dt, true, true) == kBig) go(TypeTag<BigTile<T, true, true>>{});
         else go(TypeTag<MidTile<T, true, true>>{});
       } else {
         go(TypeTag<MidTile<T, true, true>>{});
@@ -850,6 +851,12 @@ hipError_t backward(LceArgs a, int dt, const LcePlan& p, hipStream_t s) {
 
 int64_t linear_ce_workspace_bytes(int64_t tokens, int64_t hidden, int64_t vocab, int dt,
                                   bool pad_weight, bool backward) {
+  // a launch has fewer than 2^32 lanes (the backward's pieces, of 2^36 logits at most, always do)
+  const Tile t = tile_of(tokens, vocab, dt, false, false);
+  const int64_t lanes = t == kBig ? 512 : 256;
+  if (!backward &&
+      tile_grid(tiles(tokens, tile_rows(t)) * tiles(vocab, tile_cols(t))) >= (int64_t(1) << 32) / lanes)
+    return 0;
   return lce_plan(tokens, hidden, vocab, dt, pad_weight, backward).bytes;
 }
 
@@ -859,8 +866,9 @@ hipError_t launch_linear_ce(LceArgs a, int dt, bool back, void* workspace, hipSt
     dispatch_float_type(dt, [&](auto tag) {
       using T = typename decltype(tag)::type;
       const int64_t n = a.vocab * a.hidden;
-      launch_kernel(lce_zero<T>, dim3(static_cast<unsigned>(tiles(n, kGatherRows * kWave))),
-                    dim3(kGatherRows * kWave), 0, s, static_cast<T*>(a.dw), n);
+      const int64_t grid = std::min<int64_t>(tiles(n, kGatherRows * kWave), 1 << 16);
+      launch_kernel(lce_zero<T>, dim3(static_cast<unsigned>(grid)), dim3(kGatherRows * kWave), 0, s,
+                    static_cast<T*>(a.dw), n);
       err = hipGetLastError();
     });
     return err;

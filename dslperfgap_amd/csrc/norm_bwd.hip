@@ -448,52 +448,55 @@ __global__ __launch_bounds__(norm_lanes(IT)) void norm_grads(const NormGradArgs 
 // ---------------------------------------------------------------------------
 
 constexpr int kWideLanes = 256;
+constexpr int kWideRows = 1 << 16;  // workgroups of a row each at a time
 
 struct WideStat {
   float m, r, mean_g, mean_gu;
 };
 
-// One workgroup per row, value by value in three passes over the row (the second and
-// third from the L2).
+// One workgroup per row and every gridDim.x-th, value by value in three passes over the row (the
+// second and third from the L2).
 template <typename T, typename W, bool LN>
 __global__ __launch_bounds__(kMaxBlock) void norm_wide_stats(const NormGradArgs a, float* stats) {
   __shared__ float mean[kMaxWaves][1], squares[kMaxWaves][1], dots[kMaxWaves][2];
-  const int64_t row = blockIdx.x;
-  const T* x = static_cast<const T*>(a.x) + row * a.cols;
-  const T* dy = static_cast<const T*>(a.dy) + row * a.cols;
   const W* w = static_cast<const W*>(a.w);
-  const Span sx = VBH_SPAN(x, a.cols), sg = VBH_SPAN(dy, a.cols), sw = VBH_SPAN(w, a.cols);
+  const Span sw = VBH_SPAN(w, a.cols);
   const float inv_n = 1.0f / static_cast<float>(a.cols);
   const int first = static_cast<int>(threadIdx.x), block = static_cast<int>(blockDim.x);
-  WideStat s{0.0f, 0.0f, 0.0f, 0.0f};
   auto at = [](const auto* p, int64_t c, const Span& sp) {
     float v;
     load_f32<std::decay_t<decltype(*p)>, 1>(p + c, &v, sp);
     return v;
   };
-  if constexpr (LN) {
-    float sum[1] = {0.0f};
-    for (int64_t c = first; c < a.cols; c += block) sum[0] += at(x, c, sx);
-    row_sums<1>(sum, block, mean);
-    s.m = sum[0] * inv_n;
-  }
-  float sq[1] = {0.0f};
-  for (int64_t c = first; c < a.cols; c += block) {
-    const float d = at(x, c, sx) - s.m;
-    sq[0] = fmaf(d, d, sq[0]);
-  }
-  row_sums<1>(sq, block, squares);
-  s.r = 1.0f / __builtin_sqrtf(fmaf(sq[0], inv_n, a.eps));
-  float dot[2] = {0.0f, 0.0f};
-  for (int64_t c = first; c < a.cols; c += block) {
-    const float g = at(dy, c, sg) * at(w, c, sw);
-    dot[0] = fmaf(g, (at(x, c, sx) - s.m) * s.r, dot[0]);
-    if (LN) dot[1] += g;
-  }
-  row_sums<2>(dot, block, dots);
-  if (threadIdx.x == 0) {
-    const float o[4] = {s.m, s.r, dot[1] * inv_n, dot[0] * inv_n};
-    store_any<float, 4, false>(stats + row * 4, o, VBH_SPAN(stats, a.rows * 4));
+  for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+    const T* x = static_cast<const T*>(a.x) + row * a.cols;
+    const T* dy = static_cast<const T*>(a.dy) + row * a.cols;
+    const Span sx = VBH_SPAN(x, a.cols), sg = VBH_SPAN(dy, a.cols);
+    WideStat s{0.0f, 0.0f, 0.0f, 0.0f};
+    if constexpr (LN) {
+      float sum[1] = {0.0f};
+      for (int64_t c = first; c < a.cols; c += block) sum[0] += at(x, c, sx);
+      row_sums<1>(sum, block, mean);
+      s.m = sum[0] * inv_n;
+    }
+    float sq[1] = {0.0f};
+    for (int64_t c = first; c < a.cols; c += block) {
+      const float d = at(x, c, sx) - s.m;
+      sq[0] = fmaf(d, d, sq[0]);
+    }
+    row_sums<1>(sq, block, squares);
+    s.r = 1.0f / __builtin_sqrtf(fmaf(sq[0], inv_n, a.eps));
+    float dot[2] = {0.0f, 0.0f};
+    for (int64_t c = first; c < a.cols; c += block) {
+      const float g = at(dy, c, sg) * at(w, c, sw);
+      dot[0] = fmaf(g, (at(x, c, sx) - s.m) * s.r, dot[0]);
+      if (LN) dot[1] += g;
+    }
+    row_sums<2>(dot, block, dots);
+    if (threadIdx.x == 0) {
+      const float o[4] = {s.m, s.r, dot[1] * inv_n, dot[0] * inv_n};
+      store_any<float, 4, false>(stats + row * 4, o, VBH_SPAN(stats, a.rows * 4));
+    }
   }
 }
 
@@ -638,8 +641,8 @@ template <typename T, typename W, bool LN>
 hipError_t launch_norm(NormGradArgs a, const NormShape& s, float* stats, hipStream_t stream) {
   hipError_t err = hipSuccess;
   if (s.wide) {
-    launch_kernel(norm_wide_stats<T, W, LN>, dim3(static_cast<unsigned>(a.rows)), dim3(kMaxBlock),
-                  0, stream, a, stats);
+    const unsigned groups = static_cast<unsigned>(std::min<int64_t>(a.rows, kWideRows));
+    launch_kernel(norm_wide_stats<T, W, LN>, dim3(groups), dim3(kMaxBlock), 0, stream, a, stats);
     err = hipGetLastError();
     if (err != hipSuccess) return err;
     const unsigned tiles = static_cast<unsigned>((a.cols + kWideLanes - 1) / kWideLanes);
@@ -658,7 +661,8 @@ hipError_t launch_norm(NormGradArgs a, const NormShape& s, float* stats, hipStre
     err = hipGetLastError();
   };
   const bool whole = a.cols % VN == 0 && reinterpret_cast<uintptr_t>(a.x) % 16 == 0 &&
-                     reinterpret_cast<uintptr_t>(a.dy) % 16 == 0;
+                     reinterpret_cast<uintptr_t>(a.dy) % 16 == 0 &&
+                     reinterpret_cast<uintptr_t>(a.dx) % 16 == 0;
   auto by_it = [&](auto wc) {
     constexpr bool WHOLE = decltype(wc)::value;
     if (s.it == 1) go(norm_grads<T, W, VN, 1, LN, !WHOLE, false>);

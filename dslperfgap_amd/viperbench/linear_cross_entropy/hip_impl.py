@@ -103,7 +103,7 @@ def _plan(xs, ws, dtype, wdtype, ls, ldtype, backward):
     if (code is None or lcode is None or wdtype is not dtype or len(xs) != 2 or len(ws) != 2 or
             len(ls) != 1 or xs[1] != ws[1] or ls[0] != xs[0] or 0 in xs or 0 in ws):
         return False
-    pad = xs[1] * dtype.itemsize % 16 != 0 or xs[1] * dtype.itemsize > 1 << 20
+    pad = xs[1] * dtype.itemsize % 16 != 0
     nbytes = _workspace_bytes(xs[0], xs[1], ws[0], code, int(pad), int(backward))
     if not nbytes:
         return False

@@ -85,7 +85,7 @@ int vbh_rms_norm_fwd(const void* x, const void* w, void* y,
  * through a workspace of vbh_norm_bwd_workspace_bytes bytes (16-byte aligned scratch
  * of this call, stream-ordered; not looked at where that is not needed: rows held in
  * registers without dw and db).  No rows: dw and db become zeros.
- * More than VBH_NORM_BWD_MAX_VALUES values, or 2^22 rows: VBH_E_RANGE.
+ * More than VBH_NORM_BWD_MAX_VALUES values, or 2^31 - 1 rows: VBH_E_RANGE.
  * No reference counterpart (ViperBench/layer_norm and rms_norm are forward only). */
 #define VBH_NORM_BWD_MAX_VALUES (INT64_C(1) << 46)
 int vbh_layer_norm_bwd(const void* dy, const void* x, const void* w, void* dx, void* dw, void* db,
@@ -278,7 +278,9 @@ int vbh_linear_cross_entropy_bwd(const void* dloss, const void* x, const void* w
                                  int label_dtype, void* workspace, int64_t workspace_bytes,
                                  void* stream);
 
-/* Workspace bytes of those calls, a pure function of the arguments (0 for invalid ones). */
+/* Workspace bytes of those calls, a pure function of the arguments: 0 for invalid ones, and for a
+ * forward of more logits than one launch takes (about 2^37 in 32 bits, 2^39 in 16), whose call
+ * is VBH_E_RANGE. */
 int64_t vbh_linear_cross_entropy_workspace_bytes(int64_t tokens, int64_t hidden, int64_t vocab,
                                                  int dtype, int pad_weight, int backward);
 

@@ -66,6 +66,12 @@ def test_several_rows_after_each_other(rows, cols, dtype, wdtype, layer_norm):
 
 
 @pytest.mark.parametrize("layer_norm", [True, False])
+def test_many_short_rows(layer_norm):
+    """More rows than a launch of one workgroup per row could have."""
+    _check(*_make((1 << 22) + 5, 8, BF16, BF16), layer_norm)
+
+
+@pytest.mark.parametrize("layer_norm", [True, False])
 def test_no_rows_give_zero_weight_gradients(layer_norm):
     x, dy, w, b = _make(0, 96, BF16, F32)
     got = layer_norm_bwd(dy, x, w, b) if layer_norm else rms_norm_bwd(dy, x, (96,), w)

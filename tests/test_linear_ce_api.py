@@ -147,3 +147,16 @@ def test_workspace_is_a_function_of_the_sizes():
     assert size(8192, 4096, 128000, 2, 0, 1) < whole
     # and the forward keeps a hundredth of the logits
     assert size(8192, 4096, 128000, 2, 0, 0) - 8192 * 4096 * 2 < whole / 20
+
+
+@pytest.mark.parametrize("dtype,logits", [(2, 1 << 39), (1, 1 << 39), (0, 1 << 37)])
+def test_more_logits_than_one_launch_takes(dtype, logits):
+    size = _lib.lib().vbh_linear_cross_entropy_workspace_bytes
+    for tokens in (1 << 24, 1 << 20):
+        assert size(tokens, 64, logits // tokens // 2, dtype, 0, 0) > 0
+        vocab = min(logits // tokens * 2, 1 << 24)
+        assert size(tokens, 64, vocab, dtype, 0, 0) == 0
+        _fails(_lib.E_RANGE, "more than one launch", *_fwd(tokens=tokens, hidden=64, vocab=vocab,
+                                                           xs=64, ws=64, dt=dtype))
+        # the gradients come in pieces
+        assert size(tokens, 64, vocab, dtype, 0, 1) > 0
