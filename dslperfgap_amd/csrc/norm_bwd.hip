@@ -347,8 +347,8 @@ __device__ __forceinline__ bool norm_rows(const NormGradArgs& a, NormBuffers& ld
 }
 
 // The workgroup's sums of one vector into row `row` of parts.  Lanes of a wave that hold the same
-// columns are added up first; then groups other than the first leave theirs in the LDS, a lane's
-// next to its neighbour's, and the first one adds them in order.
+// columns are added up first.  Several groups leave theirs in the LDS, a lane's next to its
+// neighbour's, and the workgroup's lanes, each with a few columns, add them in order.
 template <int V, int IT>
 __device__ __forceinline__ void write_sums(const NormGradArgs& a, float (&v)[IT][V], float* lds,
                                            int64_t row) {
@@ -357,7 +357,6 @@ __device__ __forceinline__ void write_sums(const NormGradArgs& a, float (&v)[IT]
   const int lane_tpr = a.tpr;
   const int tpr = max(lane_tpr, kWave);
   const GroupShape gs = group_shape(tpr);
-  const NormLane<V, IT> l(lane_tpr < kWave ? gs.g & (lane_tpr - 1) : gs.g, lane_tpr, a.cols);
   if (lane_tpr < kWave) {
 #pragma unroll
     for (int i = 0; i < IT; ++i) {
@@ -367,51 +366,62 @@ __device__ __forceinline__ void write_sums(const NormGradArgs& a, float (&v)[IT]
       }
     }
   }
-  four* const all = reinterpret_cast<four*>(lds);
-  auto place = [&](int q, int i, int h) { return ((q - 1) * IT + i) * (V / F) * tpr + h * tpr + gs.g; };
-  if (gs.per_block > 1) {
-    __syncthreads();
-    if (gs.sub > 0) {
-#pragma unroll
-      for (int i = 0; i < IT; ++i) {
-#pragma unroll
-        for (int h = 0; h < V / F; ++h) {
-          four f;
-          if constexpr (F == 1) f = v[i][h];
-          else f = four{v[i][4 * h], v[i][4 * h + 1], v[i][4 * h + 2], v[i][4 * h + 3]};
-          all[place(gs.sub, i, h)] = f;
-        }
-      }
-    }
-    __syncthreads();
-  }
-  if (gs.sub != 0 || gs.g >= lane_tpr) return;
   float* out = a.parts + row * a.pitch;
   const Span sp = VBH_SPAN(a.parts, a.part_rows * a.pitch);
+  // values [h F, h F + F) of vector i of lane g
+  auto write = [&](int g, int i, int h, const float (&o)[F]) {
+    const int first = (g + i * lane_tpr) * V, at = min(first, a.cols - V), skip = first - at;
+    if (skip == 0) {
+      store_any<float, F, false>(out + at + h * F, o, sp);
+    } else {
+#pragma unroll
+      for (int k = 0; k < F; ++k)
+        if (h * F + k >= skip) store_any<float, 1, false>(out + at + h * F + k, o + k, sp);
+    }
+  };
+  if (gs.per_block == 1) {
+    if (gs.g >= lane_tpr) return;
+#pragma unroll
+    for (int i = 0; i < IT; ++i) {
+#pragma unroll
+      for (int h = 0; h < V / F; ++h) {
+        float o[F];
+#pragma unroll
+        for (int k = 0; k < F; ++k) o[k] = v[i][h * F + k];
+        write(gs.g, i, h, o);
+      }
+    }
+    return;
+  }
+  four* const all = reinterpret_cast<four*>(lds);
+  const int each = IT * (V / F) * tpr;  // of a group
+  __syncthreads();
 #pragma unroll
   for (int i = 0; i < IT; ++i) {
 #pragma unroll
     for (int h = 0; h < V / F; ++h) {
-      float o[F];
+      four f;
+      if constexpr (F == 1) f = v[i][h];
+      else f = four{v[i][4 * h], v[i][4 * h + 1], v[i][4 * h + 2], v[i][4 * h + 3]};
+      all[gs.sub * each + (i * (V / F) + h) * tpr + gs.g] = f;
+    }
+  }
+  __syncthreads();
+  for (int j = static_cast<int>(threadIdx.x); j < each; j += static_cast<int>(blockDim.x)) {
+    const int ih = j / tpr, g = j - ih * tpr;
+    if (g >= lane_tpr) continue;
+    float o[F];
 #pragma unroll
-      for (int k = 0; k < F; ++k) o[k] = v[i][h * F + k];
-      for (int q = 1; q < gs.per_block; ++q) {
-        const four f = all[place(q, i, h)];
+    for (int k = 0; k < F; ++k) o[k] = 0.0f;
+    for (int q = 0; q < gs.per_block; ++q) {
+      const four f = all[q * each + j];
 #pragma unroll
-        for (int k = 0; k < F; ++k) {
-          if constexpr (F == 1) o[k] += f;
-          else o[k] += f[k];
-        }
-      }
-      if (l.skip[i] == 0) {
-        store_any<float, F, false>(out + l.at[i] + h * F, o, sp);
-      } else {
-#pragma unroll
-        for (int k = 0; k < F; ++k)
-          if (h * F + k >= l.skip[i])
-            store_any<float, 1, false>(out + l.at[i] + h * F + k, o + k, sp);
+      for (int k = 0; k < F; ++k) {
+        if constexpr (F == 1) o[k] += f;
+        else o[k] += f[k];
       }
     }
+    write(g, ih / (V / F), ih % (V / F), o);
   }
 }
 
