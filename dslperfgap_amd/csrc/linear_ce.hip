@@ -86,20 +86,23 @@ __device__ __forceinline__ void store_one(T* p, T v, const Span& s) {
   if (VBH_IN_SPAN(s, p, sizeof(T))) *p = v;
 }
 
-// Numbers the tokens that count: rows[i] is the i-th one's, place[t] token t's number or -1.  One
-// workgroup, kRowsEach times as many consecutive tokens at a time as it has lanes, their loads in
+// Numbers the tokens that count: rows[i] is the i-th one's, place[t] token t's number or -1.
+// kRowsEach times as many consecutive tokens at a time as the workgroup has lanes, their loads in
 // flight together.  Backward: the largest |dL| that a token's dloss, scale and lse allow, and how
 // dx's product is shared out.
 constexpr int kRowsEach = 8;
 constexpr int kRowsWaves = kRowsLanes / kWave;
 
-__global__ __launch_bounds__(kRowsLanes) void lce_rows(const LceArgs a) {
+// Gives the number of tokens that count, to every lane, and, of the kRowsWaves tokens from `line` on,
+// their places (`places` in the LDS; -1 where they have none).  The `first` workgroup writes.
+__device__ __forceinline__ int number_tokens(const LceArgs& a, bool first, int64_t line, int* places) {
   __shared__ int counts[2][kRowsEach * kRowsWaves];
   __shared__ float most[kRowsWaves];
   const int lane = static_cast<int>(threadIdx.x) & (kWave - 1);
   const int wave = static_cast<int>(threadIdx.x) >> 6;
   const Span sd = VBH_SPAN(a.dloss, a.tokens), sl = VBH_SPAN(a.lse_in, a.tokens);
   const Span sr = VBH_SPAN(a.rows, a.tokens), sp = VBH_SPAN(a.place, a.tokens);
+  const bool sizes = first && a.dloss != nullptr;
   int live = 0, turn = 0;
   float size = 0.0f;
   for (int64_t chunk = 0; chunk < a.tokens; chunk += kRowsLanes * kRowsEach, turn ^= 1) {
@@ -109,7 +112,7 @@ __global__ __launch_bounds__(kRowsLanes) void lce_rows(const LceArgs a) {
     for (int j = 0; j < kRowsEach; ++j) {
       const int64_t t = chunk + j * kRowsLanes + threadIdx.x, at = min(t, a.tokens - 1);
       counts_too[j] = t < a.tokens && label_at(a, at) != a.ignored;
-      if (a.dloss != nullptr) {
+      if (sizes) {
         dloss[j] = load_one(a.dloss + at, sd);
         lse[j] = load_one(a.lse_in + at, sl);
       }
@@ -119,7 +122,7 @@ __global__ __launch_bounds__(kRowsLanes) void lce_rows(const LceArgs a) {
     for (int j = 0; j < kRowsEach; ++j) {
       which[j] = __ballot(counts_too[j]);
       if (lane == 0) counts[turn][j * kRowsWaves + wave] = __popcll(which[j]);
-      if (a.dloss == nullptr || !counts_too[j]) continue;
+      if (!sizes || !counts_too[j]) continue;
       const float f = 1.0f + 2.0f * a.lse_square_scale * lse[j];
       const float b = __builtin_fabsf(dloss[j] * a.scale) * (1.0f + __builtin_fabsf(f));
       if (b <= 0x1p127f) size = fmaxf(size, b);  // what is not finite stays as it is
@@ -140,6 +143,9 @@ __global__ __launch_bounds__(kRowsLanes) void lce_rows(const LceArgs a) {
       const int base = __shfl(before, slot / 2) + (slot & 1 ? __shfl(mine, slot / 2) : 0);
       const int at = live + base + __popcll(which[j] & ((uint64_t(1) << lane) - 1));
       if (t >= a.tokens) continue;
+      if (places != nullptr && t >= line && t < line + kRowsWaves)
+        places[t - line] = counts_too[j] ? at : -1;
+      if (!first) continue;
       store_one(a.place + t, counts_too[j] ? at : -1, sp);
       if (counts_too[j]) store_one(a.rows + at, static_cast<int>(t), sr);
     }
@@ -148,7 +154,7 @@ __global__ __launch_bounds__(kRowsLanes) void lce_rows(const LceArgs a) {
   for (int s = 1; s < kWave; s *= 2) size = fmaxf(size, __shfl_xor(size, s));
   if (lane == 0) most[wave] = size;
   __syncthreads();
-  if (wave != 0) return;
+  if (!first || wave != 0) return live;
   for (int w = 1; w < kRowsWaves; ++w) size = fmaxf(size, most[w]);
   const int exponent = size > 0.0f ? __builtin_amdgcn_frexp_expf(size) : 10;
   LceInfo info{live, min(max(10 - exponent, -120), 100), 1, 0};
@@ -161,6 +167,12 @@ __global__ __launch_bounds__(kRowsLanes) void lce_rows(const LceArgs a) {
   }
   LceInfo* to = static_cast<LceInfo*>(a.info);
   if (lane == 0) store_one(to, info, VBH_SPAN(to, 1));
+  return live;
+}
+
+// One workgroup; lce_gather follows.
+__global__ __launch_bounds__(kRowsLanes) void lce_rows(const LceArgs a) {
+  number_tokens(a, true, 0, nullptr);
 }
 
 __device__ __forceinline__ LceInfo lce_info(const LceArgs& a) {
@@ -205,14 +217,9 @@ __device__ __forceinline__ void copy_line(const T* from, T* to, int64_t hidden, 
   }
 }
 
-// x's rows that count, in their order, and zeros for dx of the others.
+// Token t's row of x to place `at`; where it has none, zeros for its dx.
 template <typename T>
-__global__ __launch_bounds__(kGatherRows* kWave) void lce_gather(const LceArgs a) {
-  const int live = lce_info(a).live;
-  if (live == a.tokens && a.x_direct) return;
-  const int64_t t = static_cast<int64_t>(blockIdx.x) * kGatherRows + (threadIdx.x >> 6);
-  if (t >= a.tokens) return;
-  const int at = a.place ? load_one(a.place + t, VBH_SPAN(a.place, a.tokens)) : static_cast<int>(t);
+__device__ __forceinline__ void gather_line(const LceArgs& a, int64_t t, int at) {
   if (at >= 0) {
     const T* x = static_cast<const T*>(a.x);
     T* to = static_cast<T*>(a.x_packed);
@@ -225,6 +232,30 @@ __global__ __launch_bounds__(kGatherRows* kWave) void lce_gather(const LceArgs a
     for (int64_t c = threadIdx.x & (kWave - 1); c < a.hidden; c += kWave)
       store_one(dx + t * a.hidden + c, static_cast<T>(0.0f), sd);
   }
+}
+
+// x's rows that count, in their order.
+template <typename T>
+__global__ __launch_bounds__(kGatherRows* kWave) void lce_gather(const LceArgs a) {
+  const int live = lce_info(a).live;
+  if (live == a.tokens && a.x_direct) return;
+  const int64_t t = static_cast<int64_t>(blockIdx.x) * kGatherRows + (threadIdx.x >> 6);
+  if (t >= a.tokens) return;
+  gather_line<T>(a, t, a.place ? load_one(a.place + t, VBH_SPAN(a.place, a.tokens))
+                               : static_cast<int>(t));
+}
+
+// lce_rows and lce_gather in one, for tokens of one round of loads: every workgroup numbers them all,
+// a row of x to each of its waves (1037 tokens of 2048 fp16 values, forward by 50257 classes: 175 us,
+// with two launches 181).
+template <typename T>
+__global__ __launch_bounds__(kRowsLanes) void lce_rows_gather(const LceArgs a) {
+  __shared__ int places[kRowsWaves];
+  const int64_t line = static_cast<int64_t>(blockIdx.x) * kRowsWaves;
+  const int live = number_tokens(a, blockIdx.x == 0, line, places);
+  const int wave = static_cast<int>(threadIdx.x) >> 6;
+  if ((live == a.tokens && a.x_direct) || line + wave >= a.tokens) return;
+  gather_line<T>(a, line + wave, __builtin_amdgcn_readfirstlane(places[wave]));
 }
 
 // W's rows at multiples of 16 bytes.
@@ -657,8 +688,8 @@ template <typename T, bool P_COLUMNS, bool Q_COLUMNS>
 using BigTile = TileProduct<T, 256, 256, 4, 2, P_COLUMNS, Q_COLUMNS>;
 template <typename T, bool P_COLUMNS, bool Q_COLUMNS>
 using MidTile = TileProduct<T, 128, 128, 2, 2, P_COLUMNS, Q_COLUMNS>;
-template <typename T, bool Q_COLUMNS>
-using SmallTile = TileProduct<T, 64, 128, 2, 2, false, Q_COLUMNS>;
+template <typename T, bool P_COLUMNS, bool Q_COLUMNS>
+using SmallTile = TileProduct<T, 64, 128, 2, 2, P_COLUMNS, Q_COLUMNS>;
 template <typename T, bool Q_COLUMNS>
 using TinyTile = TileProduct<T, 32, 128, 1, 4, false, Q_COLUMNS>;
 template <typename T> using DeepTile = TileProduct<T, 32, 64, 2, 2, false, false, true>;
@@ -690,7 +721,7 @@ Tile tile_of(int64_t rows, int64_t cols, int dt, bool p_columns, bool q_columns,
   Tile best = kMid;
   int64_t least = int64_t(1) << 62;
   for (const auto& t : all) {
-    if (t.tile == kBig ? f32 : t.tile > kMid && p_columns) continue;
+    if (t.tile == kBig ? f32 : p_columns && t.tile > (f32 ? kSmall : kMid)) continue;
     const int64_t n = tiles(rows, tile_rows(t.tile)) * tiles(cols, tile_cols(t.tile));
     const int64_t time = tiles(n * most_splits, kCus) * t.work;
     if (time < least) {
@@ -717,7 +748,7 @@ void with_tile(Tile t, F&& f) {
       if constexpr (sizeof(T) == 2) f(TypeTag<BigTile<T, false, Q_COLUMNS>>{});
       break;
     case kMid: f(TypeTag<MidTile<T, false, Q_COLUMNS>>{}); break;
-    case kSmall: f(TypeTag<SmallTile<T, Q_COLUMNS>>{}); break;
+    case kSmall: f(TypeTag<SmallTile<T, false, Q_COLUMNS>>{}); break;
     case kTiny: f(TypeTag<TinyTile<T, Q_COLUMNS>>{}); break;
     case kDeep:
       if constexpr (!Q_COLUMNS) f(TypeTag<DeepTile<T>>{});
@@ -779,19 +810,35 @@ LcePlan lce_plan(int64_t tokens, int64_t hidden, int64_t vocab, int dt, bool pad
   return p;
 }
 
+unsigned line_groups(const LceArgs& a) {
+  return static_cast<unsigned>(tiles(a.tokens, kGatherRows));
+}
+
+template <typename T>
+hipError_t number_and_gather(const LceArgs& a, hipStream_t s) {
+  if (a.tokens <= kRowsLanes * kRowsEach) {
+    launch_kernel(lce_rows_gather<T>, dim3(static_cast<unsigned>(tiles(a.tokens, kRowsWaves))),
+                  dim3(kRowsLanes), 0, s, a);
+    return hipGetLastError();
+  }
+  launch_kernel(lce_rows, dim3(1), dim3(kRowsLanes), 0, s, a);
+  const hipError_t err = hipGetLastError();
+  if (err != hipSuccess) return err;
+  launch_kernel(lce_gather<T>, dim3(line_groups(a)), dim3(kGatherRows * kWave), 0, s, a);
+  return hipGetLastError();
+}
+
 template <typename T>
 hipError_t forward(LceArgs a, int dt, bool number, hipStream_t s) {
-  const unsigned line_groups = static_cast<unsigned>(tiles(a.tokens, kGatherRows));
   hipError_t err = hipSuccess;
   auto done = [&] { return (err = hipGetLastError()) == hipSuccess; };
   if (number) {
-    launch_kernel(lce_rows, dim3(1), dim3(kRowsLanes), 0, s, a);
-    if (!done()) return err;
+    err = number_and_gather<T>(a, s);
+  } else if (!a.x_direct) {
+    launch_kernel(lce_gather<T>, dim3(line_groups(a)), dim3(kGatherRows * kWave), 0, s, a);
+    err = hipGetLastError();
   }
-  if (number || !a.x_direct) {
-    launch_kernel(lce_gather<T>, dim3(line_groups), dim3(kGatherRows * kWave), 0, s, a);
-    if (!done()) return err;
-  }
+  if (err != hipSuccess) return err;
   const Tile t = tile_of(a.tokens, a.vocab, dt, false, false);
   a.col_tiles = static_cast<int>(tiles(a.vocab, tile_cols(t)));
   with_tile<T, false>(t, [&](auto tag) {
@@ -808,13 +855,9 @@ hipError_t forward(LceArgs a, int dt, bool number, hipStream_t s) {
 
 template <typename T>
 hipError_t backward(LceArgs a, int dt, const LcePlan& p, hipStream_t s) {
-  const unsigned line_groups = static_cast<unsigned>(tiles(a.tokens, kGatherRows));
   hipError_t err = hipSuccess;
   auto done = [&] { return (err = hipGetLastError()) == hipSuccess; };
-  launch_kernel(lce_rows, dim3(1), dim3(kRowsLanes), 0, s, a);
-  if (!done()) return err;
-  launch_kernel(lce_gather<T>, dim3(line_groups), dim3(kGatherRows * kWave), 0, s, a);
-  if (!done()) return err;
+  if ((err = number_and_gather<T>(a, s)) != hipSuccess) return err;
   for (int64_t i = 0; i < p.pieces; ++i) {
     a.first = i * p.piece_cols;
     a.cols = std::min(p.piece_cols, a.vocab - a.first);
@@ -838,7 +881,8 @@ hipError_t backward(LceArgs a, int dt, const LcePlan& p, hipStream_t s) {
         if (tile_of(a.cols, a.hidden, dt, true, true) == kBig) go(TypeTag<BigTile<T, true, true>>{});
         else go(TypeTag<MidTile<T, true, true>>{});
       } else {
-        go(TypeTag<MidTile<T, true, true>>{});
+        if (tile_of(a.cols, a.hidden, dt, true, true) == kSmall) go(TypeTag<SmallTile<T, true, true>>{});
+        else go(TypeTag<MidTile<T, true, true>>{});
       }
       if (!done()) return err;
     }

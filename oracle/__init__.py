@@ -23,6 +23,13 @@ rope
     The rotation of queries and keys and the per-head norm ahead of it, forward
     and backward in float64, with error bounds for 32-bit evaluation.  The
     reference has no such operator.
+norm_grads
+    The gradients of LayerNorm and RMSNorm in float64, with error bounds for
+    32-bit evaluation.  The reference's norms are forward only.
+linear_ce
+    Cross entropy of a projection, forward and backward in float64, with error
+    bounds for products summed in 32 bits and rounded gradients of the logits.
+    The reference's nearest operator takes the logits.
 
 Pinning (what checks each function; see tests/test_oracle_pins.py):
   layer_norm      numpy fp64 closed form; mean-0 / variance invariants; all-equal
@@ -49,6 +56,10 @@ Pinning (what checks each function; see tests/test_oracle_pins.py):
                   numpy first-occurrence argmax over every dim
   rope            complex multiplication; torch.autograd and differences of the
                   forward for the gradients (tests/test_rope_api.py)
+  norm_grads      torch.autograd of pytorch_impl's norms in fp64 and differences
+                  (tests/test_norm_bwd_api.py)
+  linear_ce       pytorch_impl's cross_entropy_fwd of its logits; torch.autograd and
+                  differences for the gradients (tests/test_linear_ce_api.py)
 The reference itself ships no golden vectors or fixtures for this path, and its
 Python was not imported or run: every function above is pinned by the checks
 listed, none is "parity unpinned".
