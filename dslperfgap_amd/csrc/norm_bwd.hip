@@ -212,7 +212,9 @@ __device__ __forceinline__ bool norm_rows(const NormGradArgs& a, NormBuffers& ld
   }
 
   for (int64_t turn = 0; turn < turns; ++turn, row += step) {
-    const bool live = row < a.rows;
+    // (AHEAD: one row to a workgroup.  A constant saves two selects per value: 2048 rows of 20480 bf16
+    // values, LayerNorm, 68.3 us against 72.9)
+    const bool live = AHEAD || row < a.rows;
     const int buf = static_cast<int>(turn & 1);
     if constexpr (AHEAD) {
       if (turn == 0) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
