@@ -6,6 +6,10 @@ from pathlib import Path
 import pytest
 import torch
 
+from dslperfgap_amd.viperbench.linear_cross_entropy.hip_impl import (linear_cross_entropy_bwd,
+                                                                     linear_cross_entropy_fwd)
+from dslperfgap_amd.viperbench.rms_norm.hip_impl import rms_norm_bwd
+
 sys.path.insert(0, str(Path(__file__).parent))
 from test_gpu_linear_ce import _check, _make  # noqa: E402
 
@@ -40,3 +44,47 @@ def test_pieces_shared_between_workgroups(ignored):
     piece with fewer columns than workgroups share."""
     _check(*_make(20001, 64, 16100, BF16, ignored))
     _check(*_make(20001, 32, 8230, F32, ignored))
+
+
+@pytest.mark.parametrize("tokens", [8191, 8192, 8193, 16385])
+def test_tokens_numbered_in_one_round_and_in_more(tokens):
+    _check(*_make(tokens, 40, 1000, BF16, 0.3))
+    _check(*_make(tokens, 33, 40, F32, 0.7))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("tokens", [600, 9000])
+def test_what_ignored_tokens_hold_reaches_no_tile(tokens, dtype):
+    """Enough tiles for the forward to drop the ignored tokens."""
+    x, w, lab, dloss = _make(tokens, 64, 20000, dtype, 0.3)
+    want = _check(x, w, lab, dloss)
+    drop = lab == -100
+    x[drop], dloss[drop] = float("nan"), float("inf")
+    got = linear_cross_entropy_fwd(x, w, lab)
+    grads = linear_cross_entropy_bwd(dloss, x, w, got[1], lab)
+    for p, q in zip((*want[0], *want[1]), (*got, *grads)):
+        assert torch.equal(p, q)
+
+
+def test_two_calls_at_once():
+    """Calls on two streams, and their norms' gradients, in flight together: each its own bits."""
+    jobs = [_make(900, 256, 9000, BF16, 0.3), _make(257, 512, 8000, F32, 0.1, seed=1)]
+
+    def run(x, w, lab, dloss):
+        loss, lse, z = linear_cross_entropy_fwd(x, w, lab)
+        dx, dw = linear_cross_entropy_bwd(dloss, x, w, lse, lab)
+        return (loss, lse, z, dx, dw, *rms_norm_bwd(dx, x, (x.shape[1],), w[0]))
+
+    want = [run(*job) for job in jobs]
+    streams = [torch.cuda.Stream() for _ in jobs]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(5):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(run(*jobs[i]))
+    torch.cuda.synchronize()
+    for i, expected in enumerate(want):
+        for outs in got[i]:
+            for p, q in zip(expected, outs):
+                assert torch.equal(p, q)
