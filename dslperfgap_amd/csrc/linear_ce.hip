@@ -108,8 +108,11 @@ __device__ __forceinline__ int number_tokens(const LceArgs& a, bool first, int64
   for (int64_t chunk = 0; chunk < a.tokens; chunk += kRowsLanes * kRowsEach, turn ^= 1) {
     bool counts_too[kRowsEach];
     float dloss[kRowsEach], lse[kRowsEach];
+    const int64_t left = a.tokens - chunk;  // (fewer than a round: its unused parts are skipped)
 #pragma unroll
     for (int j = 0; j < kRowsEach; ++j) {
+      counts_too[j] = false;
+      if (j * kRowsLanes >= left) continue;
       const int64_t t = chunk + j * kRowsLanes + threadIdx.x, at = min(t, a.tokens - 1);
       counts_too[j] = t < a.tokens && label_at(a, at) != a.ignored;
       if (sizes) {
@@ -120,7 +123,7 @@ __device__ __forceinline__ int number_tokens(const LceArgs& a, bool first, int64
     uint64_t which[kRowsEach];
 #pragma unroll
     for (int j = 0; j < kRowsEach; ++j) {
-      which[j] = __ballot(counts_too[j]);
+      which[j] = j * kRowsLanes < left ? __ballot(counts_too[j]) : 0;
       if (lane == 0) counts[turn][j * kRowsWaves + wave] = __popcll(which[j]);
       if (!sizes || !counts_too[j]) continue;
       const float f = 1.0f + 2.0f * a.lse_square_scale * lse[j];
@@ -138,6 +141,7 @@ __device__ __forceinline__ int number_tokens(const LceArgs& a, bool first, int64
     const int before = sum - mine - next;
 #pragma unroll
     for (int j = 0; j < kRowsEach; ++j) {
+      if (j * kRowsLanes >= left) continue;
       const int64_t t = chunk + j * kRowsLanes + threadIdx.x;
       const int slot = j * kRowsWaves + wave;
       const int base = __shfl(before, slot / 2) + (slot & 1 ? __shfl(mine, slot / 2) : 0);
@@ -201,8 +205,21 @@ constexpr int kGatherRows = 4;  // waves of a workgroup, one row each
 template <typename T>
 __device__ __forceinline__ void copy_line(const T* from, T* to, int64_t hidden, int64_t padded,
                                           const Span& sf, const Span& st) {
-  constexpr int V = Vec<T>::n;
-  for (int64_t c = (threadIdx.x & (kWave - 1)) * V; c < padded; c += kWave * V) {
+  constexpr int V = Vec<T>::n, kStep = kWave * V, kEach = 4;  // loads in flight
+  int64_t c = (threadIdx.x & (kWave - 1)) * V;
+  for (; c + (kEach - 1) * kStep + V <= hidden; c += kEach * kStep) {
+    typename Raw<T, V>::type raw[kEach];
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) raw[i] = load_any<T, V, false>(from + c + i * kStep, sf);
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      float v[V];
+#pragma unroll
+      for (int k = 0; k < V; ++k) v[k] = raw_at<T, V>(raw[i], k);
+      store_raw<T, V, false>(to + c + i * kStep, v, st);
+    }
+  }
+  for (; c < padded; c += kStep) {
     float v[V];
     if (c + V <= hidden) {
       const auto raw = load_any<T, V, false>(from + c, sf);
@@ -246,8 +263,8 @@ __global__ __launch_bounds__(kGatherRows* kWave) void lce_gather(const LceArgs a
 }
 
 // lce_rows and lce_gather in one, for tokens of one round of loads: every workgroup numbers them all,
-// a row of x to each of its waves (1037 tokens of 2048 fp16 values, forward by 50257 classes: 175 us,
-// with two launches 181).
+// a row of x to each of its waves (1037 tokens of 2048 fp16 values, forward by 50257 classes: 170 us,
+// with two launches 176).
 template <typename T>
 __global__ __launch_bounds__(kRowsLanes) void lce_rows_gather(const LceArgs a) {
   __shared__ int places[kRowsWaves];
