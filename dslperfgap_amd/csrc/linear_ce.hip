@@ -262,9 +262,11 @@ __global__ __launch_bounds__(kGatherRows* kWave) void lce_gather(const LceArgs a
                                : static_cast<int>(t));
 }
 
-// lce_rows and lce_gather in one, for tokens of one round of loads: every workgroup numbers them all,
+// lce_rows and lce_gather in one, for up to kTogether tokens: every workgroup numbers them all, with
 // a row of x to each of its waves (1037 tokens of 2048 fp16 values, forward by 50257 classes: 170 us,
-// with two launches 176).
+// with two launches 176; at 8192 tokens the numbering by all of them takes 14 us, by one 7 and the
+// other launch 4).
+constexpr int kTogether = kRowsLanes * kRowsEach / 2;
 template <typename T>
 __global__ __launch_bounds__(kRowsLanes) void lce_rows_gather(const LceArgs a) {
   __shared__ int places[kRowsWaves];
@@ -833,7 +835,7 @@ unsigned line_groups(const LceArgs& a) {
 
 template <typename T>
 hipError_t number_and_gather(const LceArgs& a, hipStream_t s) {
-  if (a.tokens <= kRowsLanes * kRowsEach) {
+  if (a.tokens <= kTogether) {
     launch_kernel(lce_rows_gather<T>, dim3(static_cast<unsigned>(tiles(a.tokens, kRowsWaves))),
                   dim3(kRowsLanes), 0, s, a);
     return hipGetLastError();

@@ -46,8 +46,8 @@ def test_pieces_shared_between_workgroups(ignored):
     _check(*_make(20001, 32, 8230, F32, ignored))
 
 
-@pytest.mark.parametrize("tokens", [8191, 8192, 8193, 16385])
-def test_tokens_numbered_in_one_round_and_in_more(tokens):
+@pytest.mark.parametrize("tokens", [4096, 4097, 8191, 8192, 8193, 16385])
+def test_tokens_numbered_at_once_and_in_rounds(tokens):
     _check(*_make(tokens, 40, 1000, BF16, 0.3))
     _check(*_make(tokens, 33, 40, F32, 0.7))
 
