@@ -21,10 +21,13 @@
 // any is ignored x is gathered in that order.  What an ignored token's x holds, infinities and
 // NaN among it, reaches no output.
 //
-// dL is scaled by a power of two that brings its largest possible value to 2^10 (taken off again
-// where dx and dW are rounded): fp16 then keeps probabilities down to 2^-24 of the largest as
-// normal numbers whatever the loss is divided by.
+// dL is scaled by a power of two that brings its largest possible value to 2^14 (taken off again
+// where dx and dW are rounded): fp16 then keeps values down to 2^-28 of the largest as normal
+// numbers whatever the loss is divided by.  A token of fp16 whose own largest lies below 2^10 then
+// has a power of two of its own for dx, whose sums are its alone; ahead of dW, which sums over
+// tokens, its dL comes back to the common one.
 #include <algorithm>
+#include <type_traits>
 
 #include "tile_product.h"
 #include "vbh_launch.h"
@@ -39,6 +42,7 @@ constexpr int kRowsLanes = 1024;
 struct LceInfo {
   int live;        // tokens that count
   int shift;       // of dL's power of two
+  int spread;      // some token's has more of its own (token_shift)
   int splits;      // of a piece's columns in the product that gives dx (dx_splits)
   int split_cols;  // in each
 };
@@ -64,6 +68,20 @@ __device__ __forceinline__ int dx_splits(int64_t tiles, int slots, int cols, int
   float least = time;
   for (int i = 1; i < kWave; i *= 2) least = fminf(least, __shfl_xor(least, i));
   return __builtin_ctzll(__ballot(time == least)) + 1;
+}
+
+// |dL| at most of a token with this loss gradient and logsumexp; 0 where that is not finite.
+__device__ __forceinline__ float most_dlogit(const LceArgs& a, float dloss, float lse) {
+  const float f = 1.0f + 2.0f * a.lse_square_scale * lse;
+  const float most = __builtin_fabsf(dloss * a.scale) * (1.0f + __builtin_fabsf(f));
+  return most <= 0x1p127f ? most : 0.0f;
+}
+// Powers of two that bring a token's dL from the call's scale up to a largest value of 2^kTop: none
+// where that is within kNear of it, so that gradients alike in size need no second scale.
+constexpr int kTop = 14, kNear = 4;
+__device__ __forceinline__ int own_shift(float most, int shift) {
+  const int exponent = __builtin_amdgcn_frexp_expf(most) + shift;
+  return most > 0.0f && exponent <= kTop - kNear ? kTop - exponent : 0;
 }
 
 __device__ __forceinline__ int64_t label_at(const LceArgs& a, int64_t t) {
@@ -97,14 +115,14 @@ constexpr int kRowsWaves = kRowsLanes / kWave;
 // their places (`places` in the LDS; -1 where they have none).  The `first` workgroup writes.
 __device__ __forceinline__ int number_tokens(const LceArgs& a, bool first, int64_t line, int* places) {
   __shared__ int counts[2][kRowsEach * kRowsWaves];
-  __shared__ float most[kRowsWaves];
+  __shared__ float most[kRowsWaves], lows[kRowsWaves];
   const int lane = static_cast<int>(threadIdx.x) & (kWave - 1);
   const int wave = static_cast<int>(threadIdx.x) >> 6;
   const Span sd = VBH_SPAN(a.dloss, a.tokens), sl = VBH_SPAN(a.lse_in, a.tokens);
   const Span sr = VBH_SPAN(a.rows, a.tokens), sp = VBH_SPAN(a.place, a.tokens);
   const bool sizes = first && a.dloss != nullptr;
   int live = 0, turn = 0;
-  float size = 0.0f;
+  float size = 0.0f, least = __builtin_huge_valf();
   for (int64_t chunk = 0; chunk < a.tokens; chunk += kRowsLanes * kRowsEach, turn ^= 1) {
     bool counts_too[kRowsEach];
     float dloss[kRowsEach], lse[kRowsEach];
@@ -126,9 +144,9 @@ __device__ __forceinline__ int number_tokens(const LceArgs& a, bool first, int64
       which[j] = j * kRowsLanes < left ? __ballot(counts_too[j]) : 0;
       if (lane == 0) counts[turn][j * kRowsWaves + wave] = __popcll(which[j]);
       if (!sizes || !counts_too[j]) continue;
-      const float f = 1.0f + 2.0f * a.lse_square_scale * lse[j];
-      const float b = __builtin_fabsf(dloss[j] * a.scale) * (1.0f + __builtin_fabsf(f));
-      if (b <= 0x1p127f) size = fmaxf(size, b);  // what is not finite stays as it is
+      const float b = most_dlogit(a, dloss[j], lse[j]);  // (what is not finite stays as it is)
+      size = fmaxf(size, b);
+      if (b > 0.0f) least = fminf(least, b);
     }
     __syncthreads();
     // every wave sums up the counts: two of the 128 to a lane
@@ -155,13 +173,20 @@ __device__ __forceinline__ int number_tokens(const LceArgs& a, bool first, int64
     }
     live += __shfl(sum, kWave - 1);
   }
-  for (int s = 1; s < kWave; s *= 2) size = fmaxf(size, __shfl_xor(size, s));
-  if (lane == 0) most[wave] = size;
+  for (int s = 1; s < kWave; s *= 2) {
+    size = fmaxf(size, __shfl_xor(size, s));
+    least = fminf(least, __shfl_xor(least, s));
+  }
+  if (lane == 0) most[wave] = size, lows[wave] = least;
   __syncthreads();
   if (!first || wave != 0) return live;
-  for (int w = 1; w < kRowsWaves; ++w) size = fmaxf(size, most[w]);
-  const int exponent = size > 0.0f ? __builtin_amdgcn_frexp_expf(size) : 10;
-  LceInfo info{live, min(max(10 - exponent, -120), 100), 1, 0};
+  for (int w = 0; w < kRowsWaves; ++w) {
+    size = fmaxf(size, most[w]);
+    least = fminf(least, lows[w]);
+  }
+  const int exponent = size > 0.0f ? __builtin_amdgcn_frexp_expf(size) : kTop;
+  LceInfo info{live, min(max(kTop - exponent, -120), 100), 0, 1, 0};
+  info.spread = a.own_scales && size > 0.0f && own_shift(least, info.shift) > 0;
   if (a.dx != nullptr) {
     const int64_t tiles = static_cast<int64_t>((live + a.dx_rows - 1) / a.dx_rows) * a.dx_cols;
     const int splits = dx_splits(tiles, a.dx_slots, a.first_cols, a.value_bytes,
@@ -181,8 +206,21 @@ __global__ __launch_bounds__(kRowsLanes) void lce_rows(const LceArgs a) {
 
 __device__ __forceinline__ LceInfo lce_info(const LceArgs& a) {
   const LceInfo* info = static_cast<const LceInfo*>(a.info);
-  if (info == nullptr) return LceInfo{static_cast<int>(a.tokens), 0, 1, 0};
+  if (info == nullptr) return LceInfo{static_cast<int>(a.tokens), 0, 0, 1, 0};
   return load_one(info, VBH_SPAN(info, 1));
+}
+
+// The power of two in token t's dL as dx's product reads it.
+template <typename T>
+__device__ __forceinline__ int token_shift(const LceArgs& a, const LceInfo& info, int64_t t) {
+  if constexpr (std::is_same_v<T, _Float16>) {
+    if (info.spread) {
+      const float dloss = load_one(a.dloss + t, VBH_SPAN(a.dloss, a.tokens));
+      const float lse = load_one(a.lse_in + t, VBH_SPAN(a.lse_in, a.tokens));
+      return info.shift + own_shift(most_dlogit(a, dloss, lse), info.shift);
+    }
+  }
+  return info.shift;
 }
 
 // x as the products read it: where it lies, or gathered and padded by lce_gather.
@@ -533,7 +571,8 @@ __global__ __launch_bounds__(G::kLanes) void lce_dlogits(const LceArgs a) {
     const int64_t t = load_one(a.rows + r0 + row, VBH_SPAN(a.rows, a.tokens));
     const int64_t label = label_at(a, t) - a.class_start - a.first - c0 - g.wave_col();
     const float lse = load_one(a.lse_in + t, VBH_SPAN(a.lse_in, a.tokens));
-    const float by = ldexpf(load_one(a.dloss + t, VBH_SPAN(a.dloss, a.tokens)) * a.scale, info.shift);
+    const float by = ldexpf(load_one(a.dloss + t, VBH_SPAN(a.dloss, a.tokens)) * a.scale,
+                            token_shift<T>(a, info, t));
     const float f = 1.0f + 2.0f * a.lse_square_scale * lse;
     T* to = piece + (r0 + row) * a.pitch + c0 + g.wave_col();
 #pragma unroll
@@ -635,21 +674,49 @@ __global__ __launch_bounds__(G::kLanes) void lce_dx(const LceArgs a, int more, i
       store_from_f32<float, 4>(to, o, ss);
       return;
     }
-#pragma unroll
-    for (int j = 0; j < 4; ++j) o[j] = ldexpf(o[j], -info.shift);
     const int64_t t = load_one(a.rows + r0 + row, VBH_SPAN(a.rows, a.tokens));
+    const int shift = token_shift<T>(a, info, t);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) o[j] = ldexpf(o[j], -shift);
     store_four(dx + t * a.hidden, c0 + col, a.hidden, o, sd);
   });
 }
 
-// dx from the splits' sums, four values of a row to a lane.
 constexpr int kSumLanes = 256;
 constexpr int kSumGroups = 4096;  // at most
 
+// dL of the tokens with powers of two of their own, a row at a time, back to the call's: one more
+// rounding where that leaves fp16's normal numbers.  (Backward by 32000 classes, loss gradients alike
+// and over 20 powers of two: 2048 tokens of 2048 values 720 and 744 us, 8192 of 4096 5174 and 5290.)
+__device__ __forceinline__ void level_piece(const LceArgs& a, const LceInfo& info) {
+  typedef _Float16 T;
+  constexpr int V = Vec<T>::n;
+  T* piece = static_cast<T*>(a.piece);
+  const Span sp = VBH_SPAN(piece, info.live * a.pitch);
+  for (int64_t row = blockIdx.x; row < info.live; row += gridDim.x) {
+    const int64_t t = load_one(a.rows + row, VBH_SPAN(a.rows, a.tokens));
+    const int own = token_shift<T>(a, info, t) - info.shift;
+    if (own == 0) continue;
+    for (int64_t c = static_cast<int64_t>(threadIdx.x) * V; c < a.pitch; c += kSumLanes * V) {
+      T* at = piece + row * a.pitch + c;
+      const auto raw = load_raw<T, V, false>(at, sp);
+      float o[V];
+#pragma unroll
+      for (int k = 0; k < V; ++k) o[k] = ldexpf(raw_at<T, V>(raw, k), -own);
+      store_raw<T, V, false>(at, o, sp);
+    }
+  }
+}
+
+// dx from the splits' sums behind the last piece, four values of a row to a lane; `level`: the
+// piece's dL to the call's scale, for dW.
 template <typename T>
-__global__ __launch_bounds__(kSumLanes) void lce_dx_join(const LceArgs a) {
+__global__ __launch_bounds__(kSumLanes) void lce_dx_join(const LceArgs a, int level, int last) {
   const LceInfo info = lce_info(a);
-  if (info.splits == 1) return;
+  if constexpr (std::is_same_v<T, _Float16>) {
+    if (level && info.spread) level_piece(a, info);
+  }
+  if (!last || info.splits == 1) return;
   T* dx = static_cast<T*>(a.dx);
   const Span ss = VBH_SPAN(a.dx_sums, a.dx_sum_floats);
   const int64_t step = info.live * a.padded;
@@ -674,8 +741,9 @@ __global__ __launch_bounds__(kSumLanes) void lce_dx_join(const LceArgs a) {
         for (int j = 0; j < 4; ++j) o[j] += s + i < info.splits ? v[i][j] : 0.0f;
       }
     }
+    const int shift = token_shift<T>(a, info, t);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) o[j] = ldexpf(o[j], -info.shift);
+    for (int j = 0; j < 4; ++j) o[j] = ldexpf(o[j], -shift);
     store_four(dx + t * a.hidden, c, a.hidden, o, VBH_SPAN(dx, a.tokens * a.hidden));
   }
 }
@@ -889,7 +957,7 @@ hipError_t backward(LceArgs a, int dt, const LcePlan& p, hipStream_t s) {
       launch_kernel(lce_dlogits<T, G>, dim3(static_cast<unsigned>(grid)), dim3(G::kLanes), 0, s, a);
     });
     if (!done()) return err;
-    if (a.dw != nullptr) {
+    auto weight = [&] {
       auto go = [&](auto tag) {
         using G = typename decltype(tag)::type;
         const int64_t grid = tile_grid(tiles(a.cols, G::BR) * tiles(a.hidden, G::BC));
@@ -903,21 +971,31 @@ hipError_t backward(LceArgs a, int dt, const LcePlan& p, hipStream_t s) {
         if (tile_of(a.cols, a.hidden, dt, true, true) == kSmall) go(TypeTag<SmallTile<T, true, true>>{});
         else go(TypeTag<MidTile<T, true, true>>{});
       }
-      if (!done()) return err;
+      return done();
+    };
+    const bool last = i + 1 == p.pieces;
+    auto rows = [&] {
+      with_tile<T, true>(p.dx_tile, [&](auto tag) {
+        using G = typename decltype(tag)::type;
+        launch_kernel(lce_dx<T, G>, dim3(static_cast<unsigned>(tile_grid(p.dx_grid))),
+                      dim3(G::kLanes), 0, s, a, i > 0 ? 1 : 0, last ? 1 : 0);
+      });
+      return done();
+    };
+    auto join = [&](bool level) {
+      const int64_t groups =
+          std::min<int64_t>(tiles(a.tokens * a.padded, 4 * kSumLanes), kSumGroups);
+      launch_kernel(lce_dx_join<T>, dim3(static_cast<unsigned>(groups)), dim3(kSumLanes), 0, s, a,
+                    level ? 1 : 0, last ? 1 : 0);
+      return done();
+    };
+    if (a.own_scales && a.dw != nullptr) {
+      // dx ahead of dW, each with dL at its scale
+      if (!rows() || !join(true) || !weight()) return err;
+      continue;
     }
-    if (a.dx == nullptr) continue;
-    with_tile<T, true>(p.dx_tile, [&](auto tag) {
-      using G = typename decltype(tag)::type;
-      launch_kernel(lce_dx<T, G>, dim3(static_cast<unsigned>(tile_grid(p.dx_grid))),
-                    dim3(G::kLanes), 0, s, a, i > 0 ? 1 : 0, i + 1 == p.pieces ? 1 : 0);
-    });
-    if (!done()) return err;
-  }
-  if (a.dx != nullptr) {
-    const int64_t groups =
-        std::min<int64_t>(tiles(a.tokens * a.padded, 4 * kSumLanes), kSumGroups);
-    launch_kernel(lce_dx_join<T>, dim3(static_cast<unsigned>(groups)), dim3(kSumLanes), 0, s, a);
-    done();
+    if (a.dw != nullptr && !weight()) return err;
+    if (a.dx != nullptr && (!rows() || (last && !join(false)))) return err;
   }
   return err;
 }
@@ -968,6 +1046,7 @@ hipError_t launch_linear_ce(LceArgs a, int dt, bool back, void* workspace, hipSt
     a.dx_slots = static_cast<int>(tile_slots(p.dx_tile));
     a.first_cols = static_cast<int>(std::min(p.piece_cols, a.vocab));
     a.value_bytes = value_bytes(dt);
+    a.own_scales = dt == kF16 && a.dx != nullptr;
   } else {
     a.parts = ws + p.parts;
     a.totals = reinterpret_cast<float*>(ws + p.totals);

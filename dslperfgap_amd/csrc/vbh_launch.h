@@ -436,6 +436,7 @@ struct LceArgs {
   int dx_rows = 1, dx_cols = 1, dx_slots = 1;  // a tile's rows, tiles across, workgroups at once
   int first_cols = 0;                          // of the first piece
   int value_bytes = 2;
+  int own_scales = 0;                          // tokens' dL may have powers of two of their own
 };
 int64_t linear_ce_workspace_bytes(int64_t tokens, int64_t hidden, int64_t vocab, int dt,
                                   bool pad_weight, bool backward);

@@ -265,7 +265,9 @@ int vbh_linear_cross_entropy_fwd(const void* x, const void* w, const void* label
 /* Its gradients, in pieces of the vocabulary: with L = logit_scale x w^T formed again,
  *   dL = dloss logit_scale (exp(L - lse) (1 + 2 lse_square_scale lse) - target),
  *   dx = dL w, dw = dL^T x,
- * dL rounded to `dtype` (scaled, so that fp16 keeps it), sums in fp32 in a fixed order.
+ * dL rounded to `dtype`, sums in fp32 in a fixed order.  fp16: dL is scaled by powers of two, for
+ * dx by each token's own where losses weigh differently; in dw's sums over tokens what lies below
+ * 2^-28 of the largest possible dL of all tokens loses bits, in steps of 2^-38 of it.
  * dloss, lse: [tokens] fp32 (lse of the forward, or of all slices of the classes).
  * dx: [tokens, hidden], dw: [vocab, hidden], contiguous, of `dtype`, each null where not
  * wanted.  Ignored tokens: dx is 0, and nothing of theirs enters dw.  No tokens: dw becomes 0. */

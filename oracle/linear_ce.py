@@ -78,7 +78,8 @@ def backward(dloss, x, w, lse, labels, smoothing=0.0, logit_scale=1.0, lse_squar
 
     p = exp(L - lse) is off, relatively, by L's error and the exponential's (its argument's
     rounding and 4 of its own); dL then meets a rounding to the inputs' type, which for fp16 has
-    a smallest step 2^-34 of the largest possible dL; the products add as in the logits."""
+    a smallest step 2^-34 of the largest possible dL (for dx: of the token's own, whatever the
+    others' losses weigh); the products add as in the logits."""
     total = w.shape[0] if total_classes is None else total_classes
     keep, x = _parts(x, labels, ignored_index)
     logits, off = _logits(x, w, logit_scale)
@@ -92,14 +93,15 @@ def backward(dloss, x, w, lse, labels, smoothing=0.0, logit_scale=1.0, lse_squar
     off_d = scale.abs() * (p.abs() * (off + (arg.abs() + 8) * ULP) + 4 * ULP * target)
     if x.dtype != torch.float32:
         off_d = off_d * 1.01 + torch.finfo(x.dtype).eps / 2 * d.abs()
+    off_x = off_w = off_d
     if x.dtype == torch.float16:
-        off_d = off_d + 2.0 ** -34 * float((scale.abs() * (1 + f.abs())).max())
-    off_d = torch.where(keep[:, None], off_d, 0.0)
+        step = 2.0 ** -34 * scale.abs() * (1 + f.abs())
+        off_x, off_w = off_d + step, off_d + step.max()
+    off_x, off_w = (torch.where(keep[:, None], t, 0.0) for t in (off_x, off_w))
     xd, wd = x.double(), w.double()
-    big = d.abs() + off_d
     wide = _product_steps(w.shape[0], x.dtype) + w.shape[0] / 1024
     deep = _product_steps(x.shape[0], x.dtype)
     out = [torch.matmul(d, wd), torch.matmul(d.T, xd)]
-    bounds = [torch.matmul(off_d + wide * ULP * big, wd.abs()),
-              torch.matmul((off_d + deep * ULP * big).T, xd.abs())]
+    bounds = [torch.matmul(off_x + wide * ULP * (d.abs() + off_x), wd.abs()),
+              torch.matmul((off_w + deep * ULP * (d.abs() + off_w)).T, xd.abs())]
     return out, bounds

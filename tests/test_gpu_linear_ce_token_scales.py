@@ -1,0 +1,103 @@
+"""fp16 gradients of tokens whose losses weigh very differently: each row of dx is as exact as if its
+token were alone, and dw as the largest tokens allow, within the oracle's bounds."""
+import pytest
+import torch
+
+from dslperfgap_amd.viperbench.linear_cross_entropy.hip_impl import (linear_cross_entropy_bwd,
+                                                                     linear_cross_entropy_fwd)
+from oracle import linear_ce as ref
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+F16 = torch.float16
+
+
+def _make(tokens, hidden, vocab, ignored=0.0, seed=0):
+    g = torch.Generator(DEV).manual_seed(seed + tokens + 7 * hidden + 13 * vocab)
+    # classes share a direction: what many small probabilities add up to does not cancel
+    w = (1.5 / hidden ** 0.5 * torch.randn(vocab, hidden, generator=g, device=DEV) + 0.1).to(F16)
+    x = torch.randn(tokens, hidden, generator=g, device=DEV).to(F16)
+    lab = torch.randint(0, vocab, (tokens,), generator=g, device=DEV)
+    lab[torch.randperm(tokens, generator=g, device=DEV)[:round(ignored * tokens)]] = -100
+    return x, w, lab
+
+
+def _spread(tokens, powers, most=2.0 ** 10):
+    """Weights from `most` down to 2^-powers of it, of both signs."""
+    at = torch.randperm(tokens, generator=torch.Generator().manual_seed(tokens)).to(DEV)
+    sign = 1.0 - 2.0 * (at % 3 == 0).float()
+    return sign * most * torch.exp2(-powers * at.float() / max(1, tokens - 1))
+
+
+def _check(x, w, lab, dloss, **how):
+    lse = linear_cross_entropy_fwd(x, w, lab, **how)[1]
+    got = linear_cross_entropy_bwd(dloss, x, w, lse, lab, **how)
+    want, bounds = ref.backward(dloss, x, w, lse, lab, **how)
+    for name, p, q, b in zip(("dx", "dw"), got, want, bounds):
+        off = (p.double() - q).abs() - ref.rounded(b, q, p.dtype)
+        assert float(off.max()) <= 0.0, (name, float(off.max()))
+    return lse, got
+
+
+# dx joined from shared tiles; stored by its product; tiles of 32 rows; several pieces; odd sizes
+@pytest.mark.parametrize("tokens,hidden,vocab,ignored", [
+    (300, 64, 5000, 0.0), (300, 64, 300, 0.3), (20, 264, 9001, 0.0), (20001, 64, 16100, 0.1),
+    (700, 129, 1501, 0.2), (4003, 520, 12001, 0.02), (9001, 40, 3000, 0.5)])
+@pytest.mark.parametrize("powers", [3, 5, 24])
+def test_losses_of_very_different_weights(tokens, hidden, vocab, ignored, powers):
+    print(f"[gpu] token scales {tokens} {hidden} {vocab} {ignored} {powers}", flush=True)
+    _check(*_make(tokens, hidden, vocab, ignored), _spread(tokens, powers))
+
+
+@pytest.mark.parametrize("how", [dict(smoothing=0.1, lse_square_scale=1e-3, logit_scale=1.3),
+                                 dict(logit_scale=0.7)])
+def test_options(how):
+    _check(*_make(333, 72, 2000, 0.2), _spread(333, 22), **how)
+
+
+def test_weights_of_zero_and_a_token_that_is_not_finite():
+    x, w, lab = _make(300, 64, 3000)
+    dloss = _spread(300, 24)
+    dloss[::7] = 0.0
+    lse, got = _check(x, w, lab, dloss)
+    assert float(got[0][::7].abs().max()) == 0.0
+    dloss[3] = float("inf")
+    again = linear_cross_entropy_bwd(dloss, x, w, lse, lab)
+    rows = torch.arange(300, device=DEV) != 3
+    assert torch.equal(again[0][rows], got[0][rows])
+    assert not torch.isfinite(again[0][3]).any()
+
+
+def test_weights_near_the_ends_of_32_bits():
+    """The largest gradients below fp16's range (results are 0, or its smallest numbers), and a token
+    2^-140 of another."""
+    x, w, lab = _make(100, 64, 500)
+    _check(x, w, lab, _spread(100, 24, 2.0 ** -118))
+    dloss = _spread(100, 4)
+    dloss[5] = 2.0 ** -130
+    _check(x, w, lab, dloss)
+
+
+def test_without_the_weights_gradient():
+    x, w, lab = _make(300, 64, 5000, 0.1)
+    dloss = _spread(300, 24)
+    lse, want = _check(x, w, lab, dloss)
+    got = linear_cross_entropy_bwd(dloss, x, w, lse, lab, weight_grad=False)
+    assert got[1] is None and torch.equal(got[0], want[0])
+
+
+def test_equal_and_different_weights_in_one_graph():
+    x, w, lab = _make(600, 128, 3000, 0.3)
+    lse = linear_cross_entropy_fwd(x, w, lab)[1]
+    dloss = _spread(600, 24)
+    linear_cross_entropy_bwd(dloss, x, w, lse, lab)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = linear_cross_entropy_bwd(dloss, x, w, lse, lab)
+    for other in (torch.full((600,), 2.0 ** -9, device=DEV), _spread(600, 24), _spread(600, 3),
+                  torch.zeros(600, device=DEV), _spread(600, 20)):
+        dloss.copy_(other)
+        eager = linear_cross_entropy_bwd(other, x, w, lse, lab)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(held, eager))
