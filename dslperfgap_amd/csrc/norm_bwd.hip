@@ -549,7 +549,9 @@ __global__ __launch_bounds__(kWideLanes) void norm_wide_apply(const NormGradArgs
 
 // A workgroup: 32 columns of one vector, four to a lane (whole 128-byte lines), and 64 lines of
 // lanes that take up to four rows at a time, so that 256 rows take one round of loads.  Lines are
-// added up through the wave, waves through the LDS, in order.
+// added up through the wave, waves through the LDS, in order.  At most kPartGroups workgroups of a
+// vector (a launch has fewer than 2^32 lanes), each with every kPartGroups-th 32 columns.
+constexpr int kPartGroups = 1 << 16;
 constexpr int kPartCols = 32;
 constexpr int kPartLanes = 512;
 constexpr int kPartLines = kPartLanes / (kPartCols / 4);
@@ -564,41 +566,45 @@ __global__ __launch_bounds__(kPartLanes) void norm_weight_grads(const float* par
   const Span sp = VBH_SPAN(parts, static_cast<int64_t>(rows) * gridDim.y * pitch);
   const int lane = static_cast<int>(threadIdx.x) & (kWave - 1);
   const int wave = static_cast<int>(threadIdx.x) >> 6;
-  const int64_t col = static_cast<int64_t>(blockIdx.x) * kPartCols;
-  const int64_t mine = col + (lane & 7) * 4;
   const int line = wave * 8 + (lane >> 3);
-  const float* from = parts + blockIdx.y * static_cast<int64_t>(rows) * pitch + mine;
-  float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-  if (mine < pitch) {
-    for (int r = line; r < rows; r += 4 * kPartLines) {
-      float x[4][4];
+  const int64_t step = static_cast<int64_t>(gridDim.x) * kPartCols;
+  for (int64_t col = static_cast<int64_t>(blockIdx.x) * kPartCols; col < cols; col += step) {
+    const int64_t mine = col + (lane & 7) * 4;
+    const float* from = parts + blockIdx.y * static_cast<int64_t>(rows) * pitch + mine;
+    float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (mine < pitch) {
+      for (int r = line; r < rows; r += 4 * kPartLines) {
+        float x[4][4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int at = r + j * kPartLines;  // rows behind the last: the first of them again
-        load_f32<float, 4>(from + static_cast<int64_t>(at < rows ? at : r) * pitch, x[j], sp);
-      }
+        for (int j = 0; j < 4; ++j) {
+          const int at = r + j * kPartLines;  // rows behind the last: the first of them again
+          load_f32<float, 4>(from + static_cast<int64_t>(at < rows ? at : r) * pitch, x[j], sp);
+        }
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
+        for (int j = 0; j < 4; ++j) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] += r + j * kPartLines < rows ? x[j][i] : 0.0f;
+          for (int i = 0; i < 4; ++i) v[i] += r + j * kPartLines < rows ? x[j][i] : 0.0f;
+        }
       }
     }
-  }
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    for (int s = 8; s < kWave; s *= 2) v[i] += __shfl_xor(v[i], s);
-  }
-  if (lane < 8) {
+    for (int i = 0; i < 4; ++i) {
+      for (int s = 8; s < kWave; s *= 2) v[i] += __shfl_xor(v[i], s);
+    }
+    if (lane < 8) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) sums[wave][lane * 4 + i] = v[i];
-  }
-  __syncthreads();
-  const int c = static_cast<int>(threadIdx.x);
-  if (c >= kPartCols || col + c >= cols) return;
-  float sum = 0.0f;
+      for (int i = 0; i < 4; ++i) sums[wave][lane * 4 + i] = v[i];
+    }
+    __syncthreads();
+    const int c = static_cast<int>(threadIdx.x);
+    if (c < kPartCols && col + c < cols) {
+      float sum = 0.0f;
 #pragma unroll
-  for (int i = 0; i < kPartLanes / kWave; ++i) sum += sums[i][c];
-  store_any<W, 1, false>(out + col + c, &sum, VBH_SPAN(out, cols));
+      for (int i = 0; i < kPartLanes / kWave; ++i) sum += sums[i][c];
+      store_any<W, 1, false>(out + col + c, &sum, VBH_SPAN(out, cols));
+    }
+    if (col + step < cols) __syncthreads();
+  }
 }
 
 // ---------------------------------------------------------------------------
@@ -721,8 +727,9 @@ hipError_t launch_norm_bwd(NormGradArgs a, bool ln, int dt, int wdt, void* dw, v
   if (err != hipSuccess || !sums) return err;
   auto sum = [&](auto tag) {
     using W = typename decltype(tag)::type;
+    const int64_t groups = (static_cast<int64_t>(a.cols) + kPartCols - 1) / kPartCols;
     launch_kernel(norm_weight_grads<W>,
-                  dim3(static_cast<unsigned>((a.cols + kPartCols - 1) / kPartCols), ln ? 2 : 1),
+                  dim3(static_cast<unsigned>(std::min<int64_t>(groups, kPartGroups)), ln ? 2 : 1),
                   dim3(kPartLanes), 0, stream, static_cast<const float*>(a.parts),
                   a.rows > 0 ? static_cast<int>(s.grid) : 0, a.pitch, a.cols,
                   static_cast<W*>(dw), static_cast<W*>(db));
