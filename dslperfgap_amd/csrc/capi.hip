@@ -1533,6 +1533,7 @@ static int linear_ce_args(const char* what, LceArgs* a, const void* x, const voi
   a->smoothing = smoothing;
   a->scale = logit_scale;
   a->lse_square_scale = lse_square_scale;
+  a->target_most = std::fabs(1.0f - smoothing) + std::fabs(smoothing) / a->total_classes;
   a->label_i64 = label_dtype == kI64;
   return 0;
 }

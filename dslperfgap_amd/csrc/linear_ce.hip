@@ -73,7 +73,7 @@ __device__ __forceinline__ int dx_splits(int64_t tiles, int slots, int cols, int
 // |dL| at most of a token with this loss gradient and logsumexp; 0 where that is not finite.
 __device__ __forceinline__ float most_dlogit(const LceArgs& a, float dloss, float lse) {
   const float f = 1.0f + 2.0f * a.lse_square_scale * lse;
-  const float most = __builtin_fabsf(dloss * a.scale) * (1.0f + __builtin_fabsf(f));
+  const float most = __builtin_fabsf(dloss * a.scale) * (a.target_most + __builtin_fabsf(f));
   return most <= 0x1p127f ? most : 0.0f;
 }
 // Powers of two that bring a token's dL from the call's scale up to a largest value of 2^kTop: none

@@ -416,6 +416,7 @@ struct LceArgs {
   int64_t ignored = 0, class_start = 0;
   float total_classes = 0.0f;
   float smoothing = 0.0f, scale = 1.0f, lse_square_scale = 0.0f;
+  float target_most = 1.0f;       // no |share of a class in the smoothed label| is larger
   int label_i64 = 0, split = 0;
   int x_direct = 0;               // x's rows are whole 16-byte pieces
   // set by the launcher: parts of the workspace, the current piece of the vocabulary

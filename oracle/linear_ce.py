@@ -95,7 +95,7 @@ def backward(dloss, x, w, lse, labels, smoothing=0.0, logit_scale=1.0, lse_squar
         off_d = off_d * 1.01 + torch.finfo(x.dtype).eps / 2 * d.abs()
     off_x = off_w = off_d
     if x.dtype == torch.float16:
-        step = 2.0 ** -34 * scale.abs() * (1 + f.abs())
+        step = 2.0 ** -34 * scale.abs() * (abs(1 - smoothing) + abs(smoothing) / total + f.abs())
         off_x, off_w = off_d + step, off_d + step.max()
     off_x, off_w = (torch.where(keep[:, None], t, 0.0) for t in (off_x, off_w))
     xd, wd = x.double(), w.double()

@@ -50,9 +50,9 @@ def test_losses_of_very_different_weights(tokens, hidden, vocab, ignored, powers
 
 
 @pytest.mark.parametrize("how", [dict(smoothing=0.1, lse_square_scale=1e-3, logit_scale=1.3),
-                                 dict(logit_scale=0.7)])
+                                 dict(logit_scale=0.7), dict(smoothing=-9.0), dict(smoothing=1.0)])
 def test_options(how):
-    _check(*_make(333, 72, 2000, 0.2), _spread(333, 22), **how)
+    _check(*_make(333, 72, 2000, 0.2), _spread(333, 22, 61.0), **how)
 
 
 def test_weights_of_zero_and_a_token_that_is_not_finite():
