@@ -9,6 +9,9 @@ import torch
 from . import _bridge, _lib
 
 
+MOST_EPS = torch.finfo(torch.float32).max  # eps is taken in 32 bits
+
+
 @functools.lru_cache(maxsize=4096)
 def _workspace_bytes(rows: int, cols: int, dtype: int, layer_norm: bool) -> int:
     return _lib.lib().vbh_norm_bwd_workspace_bytes(rows, cols, dtype, int(layer_norm))

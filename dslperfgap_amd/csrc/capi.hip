@@ -989,6 +989,8 @@ static int norm_bwd(const char* what, bool ln, const void* dy, const void* x, co
   if (rows > kMaxCols || mul_sat(rows, cols) > VBH_NORM_BWD_MAX_VALUES)
     return fail(VBH_E_RANGE, "%s: %lld x %lld values are more than one launch takes", what,
                 static_cast<long long>(rows), static_cast<long long>(cols));
+  if (!(std::isfinite(eps) && eps >= 0.0f))
+    return fail(VBH_E_INVALID, "%s: eps must be finite and not negative", what);
   if (cols == 0) return 0;
   if (rows > 0 && (!dy || !x || !w || !dx)) return fail(VBH_E_INVALID, "%s: null pointer", what);
   const bool sums = dw != nullptr || db != nullptr;
@@ -1511,6 +1513,9 @@ static int linear_ce_args(const char* what, LceArgs* a, const void* x, const voi
     return fail(VBH_E_RANGE, "%s: row stride too large", what);
   if (total_classes < 1) return fail(VBH_E_INVALID, "%s: total_classes must be positive", what);
   if (class_start_idx < 0) return fail(VBH_E_INVALID, "%s: class_start_idx is negative", what);
+  if (!(std::isfinite(smoothing) && std::isfinite(logit_scale) && std::isfinite(lse_square_scale)))
+    return fail(VBH_E_INVALID,
+                "%s: smoothing, logit_scale and lse_square_scale must be finite in 32 bits", what);
   if (tokens > 0 && (!x || !w || !labels)) return fail(VBH_E_INVALID, "%s: null pointer", what);
   const int64_t e = elt_size(dtype);
   a->x = x;

@@ -86,8 +86,8 @@ def rms_norm_bwd(dy, x, normalized_shape, weight, eps=1e-5):
     dtype).  The weight's gradient is summed in fp32 in a fixed order and has the weight's
     shape and dtype."""
     what = "rms_norm_bwd"
-    if not (float(eps) >= 0.0 and float(eps) < float("inf")):
-        raise ValueError(f"{what}: eps must be finite and not negative, got {eps}")
+    if not 0.0 <= float(eps) <= _norm_bwd.MOST_EPS:
+        raise ValueError(f"{what}: eps must be finite in 32 bits and not negative, got {eps}")
     if tuple(normalized_shape) == tuple(weight.shape):
         got = _norm_bwd.common(dy, x, weight, None, float(eps), False)
         if got is not None:

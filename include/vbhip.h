@@ -85,7 +85,10 @@ int vbh_rms_norm_fwd(const void* x, const void* w, void* y,
  * through a workspace of vbh_norm_bwd_workspace_bytes bytes (16-byte aligned scratch
  * of this call, stream-ordered; not looked at where that is not needed: rows held in
  * registers without dw and db).  No rows: dw and db become zeros.
- * More than VBH_NORM_BWD_MAX_VALUES values, or 2^31 - 1 rows: VBH_E_RANGE.
+ * More than VBH_NORM_BWD_MAX_VALUES values, or 2^31 - 1 rows: VBH_E_RANGE.  eps that is not
+ * finite, or negative: VBH_E_INVALID.  Rows whose squares leave the range of fp32 have the
+ * gradients of the forward's output there: 0 where their sum is infinite, no finite ones where all
+ * are 0 and eps is too.
  * No reference counterpart (ViperBench/layer_norm and rms_norm are forward only). */
 #define VBH_NORM_BWD_MAX_VALUES (INT64_C(1) << 46)
 int vbh_layer_norm_bwd(const void* dy, const void* x, const void* w, void* dx, void* dw, void* db,
@@ -244,7 +247,8 @@ int vbh_cross_entropy_bwd(const void* dloss, const void* logits, const void* lse
  * `dtype`.  loss, lse, z_loss: [tokens] fp32.  An ignored token's x is not read for any
  * result: its loss, lse and z_loss are 0.  With `split` loss is left without the lse and
  * z_loss parts (w is a slice of the classes from class_start_idx on; see
- * vbh_cross_entropy_fwd).  Sums in fp32, in a fixed order.
+ * vbh_cross_entropy_fwd).  Sums in fp32, in a fixed order.  smoothing, logit_scale and
+ * lse_square_scale have to be finite (VBH_E_INVALID).
  * The workspace of vbh_linear_cross_entropy_workspace_bytes bytes is 256-byte aligned scratch
  * of this call (stream-ordered); `pad_weight`: w's rows are not whole 16-byte pieces at
  * multiples of 16 bytes, or more than 1 MiB apart, and are copied.
