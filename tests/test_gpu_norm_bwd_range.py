@@ -38,3 +38,28 @@ def test_sums_beyond_the_largest_number(dtype, rows, cols, layer_norm, scale):
         assert torch.isfinite(q).all() and torch.isfinite(p).all(), name
         off = (p.cpu().double() - q).abs() - ref.rounded(b, q, p.dtype)
         assert float(off.max()) <= 0.0, (name, float(off.max()))
+
+
+@pytest.mark.parametrize("layer_norm", [True, False])
+@pytest.mark.parametrize("dtype,rows,cols", [
+    (F32, 40, 64), (BF16, 600, 1001), (F32, 300, 12000), (BF16, 700, 20480), (BF16, 300, 20481),
+    (F32, 10, 40000)])
+def test_rows_whose_squares_are_infinite_have_no_gradient(dtype, rows, cols, layer_norm):
+    """Their forward is constant in 32 bits: rows of dx are 0, and nothing of them enters dw."""
+    g = torch.Generator(DEV).manual_seed(rows + 7 * cols)
+    x, dy = (torch.randn(rows, cols, generator=g, device=DEV).to(dtype) for _ in range(2))
+    w = (1 + 0.2 * torch.randn(cols, generator=g, device=DEV)).to(dtype)
+    x[::2] *= 1e25
+    far = torch.arange(rows, device=DEV) % 2 == 0
+    kept = dy.clone()
+    kept[far] = 0.0
+    small = x.clone()
+    small[far] = 0.0
+
+    def run(dy, x):
+        return layer_norm_bwd(dy, x, w, w) if layer_norm else rms_norm_bwd(dy, x, (cols,), w)
+
+    got, want = run(dy, x), run(kept, small)
+    assert float(got[0][far].abs().max()) == 0.0
+    assert torch.equal(got[0], want[0])
+    assert torch.equal(got[1], want[1])
