@@ -12,10 +12,12 @@
 // cores from a few hundred tokens on, below by the read of W.
 //
 // Backward, in pieces of the vocabulary: the tiles of L again, dL of the piece rounded to the
-// inputs' type into the workspace, then the two products that read it.  A piece is as wide as
-// keeps dL within kPieceBytes.  dx is summed over pieces, and over parts of a piece where its
-// own tiles are too few to fill the card, in fp32 in the workspace, in a fixed order; dW's rows
-// belong to one piece each.  No atomics.
+// inputs' type into the workspace, then the two products that read it.  (Rounded, because the
+// matrix cores take both factors in one type: fp32 ones run at a thirteenth of the 16-bit rate, and
+// dL in two 16-bit parts would double both products.)  A piece is as wide as keeps dL within
+// kPieceBytes.  dx is summed over pieces, and over parts of a piece where its own tiles are too
+// few to fill the card, in fp32 in the workspace, in a fixed order; dW's rows belong to one piece
+// each.  No atomics.
 //
 // Tokens whose label is ignored take no part: the others' rows are numbered first, and where
 // any is ignored x is gathered in that order.  What an ignored token's x holds, infinities and
@@ -301,8 +303,8 @@ __global__ __launch_bounds__(kGatherRows* kWave) void lce_gather(const LceArgs a
 }
 
 // lce_rows and lce_gather in one, for up to kTogether tokens: every workgroup numbers them all, with
-// a row of x to each of its waves (1037 tokens of 2048 fp16 values, forward by 50257 classes: 170 us,
-// with two launches 176; at 8192 tokens the numbering by all of them takes 14 us, by one 7 and the
+// a row of x to each of its waves (1037 tokens of 2048 fp16 values, forward by 50257 classes over one
+// set of inputs: 170 us, with two launches 176; at 8192 tokens the numbering by all of them takes 14 us, by one 7 and the
 // other launch 4).
 constexpr int kTogether = kRowsLanes * kRowsEach / 2;
 template <typename T>
@@ -709,7 +711,8 @@ __device__ __forceinline__ void level_piece(const LceArgs& a, const LceInfo& inf
 }
 
 // dx from the splits' sums behind the last piece, four values of a row to a lane; `level`: the
-// piece's dL to the call's scale, for dW.
+// piece's dL to the call's scale, for dW.  Launched where nothing is split or levelled too, which only
+// the GPU knows (4 us traced).
 template <typename T>
 __global__ __launch_bounds__(kSumLanes) void lce_dx_join(const LceArgs a, int level, int last) {
   const LceInfo info = lce_info(a);

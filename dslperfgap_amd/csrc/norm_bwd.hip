@@ -10,7 +10,8 @@
 // walks over rows with the next row's loads in flight, its lanes keep the fp32 sums
 // of their columns' dw and db, and its groups' sums are added through the LDS at the
 // end into one row of `parts`; a second kernel adds the rows of parts.  All in a fixed
-// order.
+// order.  Rows of more than 4096 16-byte vectors do not fit: their x is read four times and
+// dy twice (norm_wide_stats, norm_wide_apply).
 #include <algorithm>
 
 #include "vbh_launch.h"
@@ -429,7 +430,12 @@ __device__ __forceinline__ void write_sums(const NormGradArgs& a, float (&v)[IT]
 
 // Lanes of a workgroup at most: rows of more than two vectors for each of 1024 lanes take 512 lanes
 // of twice the registers (2048 rows of 20480 bf16 values, LayerNorm: 1024 lanes of three vectors
-// spill 40 registers and take 83.6 us, 512 of five 71.3).
+// spill 40 registers and take 83.6 us, 512 of five 71.3).  Five vectors of whole rows just fit;
+// beyond them registers spill.  16-bit LayerNorm (RMSNorm): whole rows 20 to 24 (0 to 1) registers
+// at six vectors, 127 to 173 (41 to 43) at eight; ragged ones 49 to 62 (0 to 44) at five, 138 to 163
+// (43 to 81) at six, 386 to 506 (228 to 349) at eight; fp32 only at eight, 12 (0) and 133 (2).
+// 2048 rows, bf16, LayerNorm / RMSNorm, us (6650 GB/s would take): of 24576 values 77 / 66 (45),
+// 32768 133 / 93 (61), 16385 81 / 67 (30), 20481 146 / 83 (38).
 constexpr int norm_lanes(int it) { return it > 2 ? kMaxBlock / 2 : kMaxBlock; }
 
 template <typename T, typename W, int V, int IT, bool LN, bool RAGGED, bool AHEAD>
@@ -456,7 +462,9 @@ __global__ __launch_bounds__(norm_lanes(IT)) void norm_grads(const NormGradArgs 
 
 // ---------------------------------------------------------------------------
 // rows beyond the registers: the row's statistics first, then tiles of columns that
-// read x and dy once more
+// read x and dy once more.  Value by value, which is what bounds them: 2048 bf16 rows of
+// 40000, LayerNorm / RMSNorm, 350 / 292 us, 1024 fp32 rows of 20480 113 / 96 (bytes
+// read and written once at 6650 GB/s: 74 and 38)
 // ---------------------------------------------------------------------------
 
 constexpr int kWideLanes = 256;

@@ -11,7 +11,8 @@
 // ("columns": [k][r]).  Columns of 16-bit values are turned on the way from the LDS to the
 // registers (ds_read_b64_tr_b16).  Rows and values of k beyond the operand's end read as
 // zeros: by the buffer resource's range, and within a row by an offset beyond it.  (Scalar offsets
-// stay within the range too, which costs 0 to 0.7% of a backward call: `more`.)
+// stay within the range too, `more`, which costs 0.5 to 1.8% of a backward call; behind a branch
+// that only a tile's last stages take, 6%.)
 //
 // Bank conflicts: the LDS takes stages as the loads deliver them, 16 bytes per lane in
 // lane order, so lanes ask for their 16-byte pieces in a permuted order instead (SQ counters
